@@ -5,7 +5,8 @@ sparse attention) as hand-written CUDA for NVIDIA B200 behind the reference's Py
 """
 __version__ = "0.1.0"
 
-from .attention import HiraDecodeStep, hira_attention, hira_decode_attention, make_hira_attention, register_hira_attention
+from .attention import (HiraDecodeStep, SharedPrompt, hira_attention, hira_attention_forward, hira_decode_attention,
+                        hira_qk_norm_rope, hira_shared_attention, make_hira_attention, patch_attention, register_hira_attention)
 from .cache import (THRESHOLD_METHODS, CacheOutput, DeviceMode, HiraCache, HiraCacheLayer, HiraConfig,
                     sample_kth, sample_max, sample_mean_topk)
 from .indexer import BaseIndexer, CUDAIndexer
@@ -15,4 +16,5 @@ __all__ = [
     "HiraDecodeStep", "hira_attention", "hira_decode_attention", "make_hira_attention", "register_hira_attention", "THRESHOLD_METHODS", "CacheOutput", "DeviceMode", "HiraCache",
     "HiraCacheLayer", "HiraConfig", "sample_max", "sample_mean_topk", "sample_kth", "BaseIndexer",
     "CUDAIndexer", "BaseSearcher", "CUDASearcher",
+    "SharedPrompt", "hira_shared_attention", "hira_qk_norm_rope", "hira_attention_forward", "patch_attention",
 ]

@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libhira_b200.so"
 HIRA_OK = 0
 HIRA_ERR_ARG, HIRA_ERR_SHAPE, HIRA_ERR_DTYPE, HIRA_ERR_CAPACITY, HIRA_ERR_CUDA = -1, -2, -3, -4, -5
 HIRA_F32, HIRA_BF16 = 0, 1
-HIRA_STATUS_PARENTS_FULL, HIRA_STATUS_GP_FULL, HIRA_STATUS_ASSIGN_FAILED = 1, 2, 4
+HIRA_STATUS_PARENTS_FULL, HIRA_STATUS_GP_FULL, HIRA_STATUS_ASSIGN_FAILED, HIRA_STATUS_BAD_INDEX = 1, 2, 4, 8
 HIRA_GATE_GT, HIRA_GATE_GE = 0x0, 0x1
 HIRA_LEAF_CANDIDATES, HIRA_LEAF_GE, HIRA_LEAF_GT = 0x0, 0x2, 0x4
 HIRA_TAU_SAMPLE_MAX, HIRA_TAU_SAMPLE_MEAN_TOPK, HIRA_TAU_SAMPLE_KTH = 0, 1, 2
@@ -30,6 +30,7 @@ EXPORTED_SYMBOLS = [
     "hira_search_scan", "hira_append_scanned", "hira_step_events_create", "hira_step_events_destroy",
     "hira_decode_step", "hira_q8_refresh", "hira_q8_fallback_count",
     "hira_exchange_bytes", "hira_peer_alloc", "hira_peer_open", "hira_peer_close", "hira_peer_free", "hira_exchange_merge",
+    "hira_shared_attn_workspace_bytes", "hira_shared_attn", "hira_gather", "hira_gather_index", "hira_qk_norm_rope",
 ]
 MAX_PEERS = 16            # HIRA_MAX_PEERS
 PEER_HANDLE_BYTES = 64    # HIRA_PEER_HANDLE_BYTES
@@ -66,6 +67,31 @@ class HiraStepStruct(C.Structure):
         ("n_splits", C.c_int32), ("tile_parents", C.c_int32), ("flags", C.c_int32),
         ("ev_copied", C.c_void_p), ("ev_searched", C.c_void_p), ("ev_appended", C.c_void_p),
     ]
+
+
+class HiraSharedAttnStruct(C.Structure):
+    """Mirror of hira_shared_attn_t."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "prefix_k", "prefix_v", "tail_k", "tail_v", "out", "prefix_lens", "tail_lens")] + \
+               [(n, C.c_int64 * 3) for n in ("q_stride", "prefix_k_stride", "prefix_v_stride", "tail_k_stride", "tail_v_stride",
+                                             "out_stride")] + \
+               [(n, C.c_int32) for n in ("dtype", "n_prompts", "n_branches", "n_kv", "group", "n_q", "dim", "vdim", "prefix_len",
+                                         "tail_len")] + [("sm_scale", C.c_float)]
+
+
+class HiraGatherItemStruct(C.Structure):
+    """Mirror of hira_gather_item_t."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("src_seq_stride", "dst_seq_stride", "src_seg_stride", "dst_seg_stride", "bytes",
+                                         "bytes_filled")] + [("n_seg", C.c_int32), ("fill", C.c_uint32)]
+
+
+class HiraRopeStruct(C.Structure):
+    """Mirror of hira_rope_t."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "cos", "sin")] + \
+               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")] + \
+               [(n, C.c_int64 * 2) for n in ("cos_stride", "sin_stride")] + \
+               [(n, C.c_int32) for n in ("dtype", "table_dtype", "batch", "n_tokens", "q_heads", "k_heads", "dim", "rotary",
+                                         "interleaved")] + [("eps", C.c_float)]
 
 
 _lib = None
@@ -145,6 +171,16 @@ def _declare(lib):
     lib.hira_recompute_radii.argtypes = [IX, P]
     lib.hira_export.restype = C.c_int
     lib.hira_export.argtypes = [IX, I32, I32, P, P, P]
+    lib.hira_shared_attn_workspace_bytes.restype = SZ
+    lib.hira_shared_attn_workspace_bytes.argtypes = [C.POINTER(HiraSharedAttnStruct)]
+    lib.hira_shared_attn.restype = C.c_int
+    lib.hira_shared_attn.argtypes = [C.POINTER(HiraSharedAttnStruct), P, SZ, P]
+    lib.hira_gather.restype = C.c_int
+    lib.hira_gather.argtypes = [C.POINTER(HiraGatherItemStruct), I32, P, I32, I32, I32, P, P]
+    lib.hira_gather_index.restype = C.c_int
+    lib.hira_gather_index.argtypes = [IX, IX, I32, I32, P, P, I64, P, P]
+    lib.hira_qk_norm_rope.restype = C.c_int
+    lib.hira_qk_norm_rope.argtypes = [C.POINTER(HiraRopeStruct), P]
     lib.hira_assign.restype = C.c_int
     lib.hira_assign.argtypes = [P, P, I32, I32, I32, I32, I32, I32, P, P, P, P]
 

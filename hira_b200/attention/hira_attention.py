@@ -72,6 +72,8 @@ def hira_decode_attention(query: torch.Tensor, cache_output, *, scaling: Optiona
     `indexer.update(append_key, value, scanned=True)`.  The search then scores the parent rows it
     reads against that key as well, and the update needs no parent scan of its own."""
     indexer, searcher = cache_output.indexer, cache_output.searcher
+    if indexer is None:
+        raise ValueError("this layer's prompt is shared (HiraCacheLayer.share_prompt) and has no index: use hira_attention")
     st: S.IndexState = indexer.state
     b, hq, lq, d = query.shape
     if lq != 1:
@@ -170,6 +172,11 @@ def hira_attention(module, query: torch.Tensor, key, value=None, attention_mask:
             query, k, v, attn_mask=attention_mask, dropout_p=0.0, is_causal=is_causal, scale=scaling,
             enable_gqa=query.shape[1] != k.shape[1])
         return out.transpose(1, 2).contiguous(), None
+    if getattr(key, "shared", None) is not None:      # continuations of shared prompts: dense, the prompt read once for all
+        b, h, n, _ = query.shape
+        out = torch.empty((b, n, h, key.shared.prefix_values.shape[3]), dtype=query.dtype, device=query.device)
+        key.shared.attend(query, scaling, out=out.transpose(1, 2))
+        return out, None
     cfg = kwargs.get("hira_config")
     opts = {}
     if cfg is not None:

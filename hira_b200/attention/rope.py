@@ -1,0 +1,147 @@
+"""Norms of the query and key heads with the position rotation in one pass, and the attention forward that uses it.
+
+`hira_qk_norm_rope` is what a model does between its projections and `HiraCache.update`: an RMS norm of every query
+and key head (where the model has one) and the rotation by position, fifteen or so elementwise passes otherwise.
+`patch_attention` replaces the forward of a model's attention layers by `hira_attention_forward`: projections,
+`hira_qk_norm_rope`, `HiraCache.update`, `hira_attention`, output projection (the hook of examples/patch_llama.py:22-100).
+"""
+from __future__ import annotations
+
+from types import MethodType
+from typing import Optional
+
+import torch
+
+from .. import index_state as S
+from .shared_attention import refuse_grad
+
+_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _table(t: torch.Tensor, b: int, n: int, name: str) -> torch.Tensor:
+    if t.ndim == 2:
+        t = t.unsqueeze(0)
+    if t.ndim != 3 or t.shape[0] not in (1, b) or t.shape[1] != n:
+        raise ValueError(f"{name} must be ({b} or 1, {n}, R) or ({n}, R), got {tuple(t.shape)}")
+    if t.dtype not in _TYPES:
+        t = t.float()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+                      q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                      interleaved: bool = False, out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
+    """query (B, H_q, L, D), key (B, H_kv, L, D) -> the two normalised and rotated, in their type.
+
+    `cos`, `sin` (B or 1, L, R) or (L, R), R <= D even: the tables of the first R channels as models hand them out
+    (each pair's value twice); channels i and i + R/2 form a pair, or 2i and 2i + 1 when `interleaved`.  The channels
+    behind R are not rotated.  `q_weight` / `k_weight` (D,): RMS norm of that side's heads with this weight; None:
+    no norm.  Computed in fp32 and rounded once.
+
+    fp32 or bf16; D a multiple of 8 up to 256.  Any strides with contiguous, 16-byte aligned rows (a projection's
+    transposed view as it is); others are copied.  `out_q` / `out_k`: where to write, with such rows: the input itself,
+    or memory apart from both inputs (part of a cache, say).  No backward pass."""
+    refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
+    if query.ndim != 4 or key.ndim != 4:
+        raise ValueError(f"query and key must be (B, H, L, D), got {tuple(query.shape)} and {tuple(key.shape)}")
+    b, hq, n, d = query.shape
+    if key.shape[0] != b or key.shape[2] != n or key.shape[3] != d:
+        raise ValueError(f"key {tuple(key.shape)} does not go with query {tuple(query.shape)}")
+    if query.dtype not in _TYPES or key.dtype != query.dtype:
+        raise ValueError(f"query is {query.dtype}, key {key.dtype}: both float32 or both bfloat16")
+    if d % 8 or not 8 <= d <= 256:
+        raise ValueError(f"D={d} must be a multiple of 8 in 8..256")
+    for name, t in (("key", key), ("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight), ("out_q", out_q),
+                    ("out_k", out_k)):
+        if t is not None and t.device != query.device:
+            raise ValueError(f"{name} is on {t.device}, query on {query.device}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (d,) or w.dtype != query.dtype):
+            raise ValueError(f"{name} must be ({d},) {query.dtype}, got {tuple(w.shape)} {w.dtype}")
+    cos, sin = _table(cos, b, n, "cos"), _table(sin, b, n, "sin")
+    if cos.shape[2] != sin.shape[2] or cos.dtype != sin.dtype:
+        raise ValueError(f"cos {tuple(cos.shape)} {cos.dtype} and sin {tuple(sin.shape)} {sin.dtype} differ")
+    r = cos.shape[2]
+    if r % 2 or r > d:
+        raise ValueError(f"{r} rotated channels: must be even and at most {d}")
+    for name, o, x in (("out_q", out_q, query), ("out_k", out_k, key)):
+        if o is None:
+            continue
+        if o.shape != x.shape or o.dtype != x.dtype or not S.writable_rows(o):
+            raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype} with aligned contiguous rows")
+        if not (o.data_ptr() == x.data_ptr() and o.stride() == x.stride()):
+            own = o.untyped_storage().data_ptr()
+            if own in (query.untyped_storage().data_ptr(), key.untyped_storage().data_ptr()):
+                raise ValueError(f"{name} must be its own input or memory apart from both inputs")
+    if not query.is_cuda:
+        raise ValueError("hira_qk_norm_rope needs CUDA tensors (there is no CPU fallback)")
+    if out_q is None:
+        out_q = torch.empty((b, hq, n, d), dtype=query.dtype, device=query.device)
+    if out_k is None:
+        out_k = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    return S.qk_norm_rope(S.with_rows(query), S.with_rows(key), cos, sin, q_weight, k_weight, eps, interleaved, out_q, out_k)
+
+
+def hira_attention_forward(module, hidden_states: torch.Tensor, position_embeddings, attention_mask: Optional[torch.Tensor] = None,
+                           past_key_values=None, hira_config=None, interleaved: bool = False, **kwargs):
+    """Forward of a decoder's attention layer over a HiraCache.  `module` has q_proj, k_proj, v_proj, o_proj, head_dim
+    and layer_idx, and may have q_norm and k_norm (RMS norms of single heads: `weight` (head_dim,) and an epsilon)."""
+    from .hira_attention import hira_attention
+    if past_key_values is None:
+        raise ValueError("hira_attention_forward needs a HiraCache as past_key_values")
+    b, n, _ = hidden_states.shape
+
+    def heads(proj):
+        return proj(hidden_states).view(b, n, -1, module.head_dim).transpose(1, 2)
+    q, k, v = heads(module.q_proj), heads(module.k_proj), heads(module.v_proj)
+    q_norm, k_norm = getattr(module, "q_norm", None), getattr(module, "k_norm", None)
+    cos, sin = position_embeddings
+    eps = {getattr(m, "variance_epsilon", getattr(m, "eps", None)) for m in (q_norm, k_norm) if m is not None}
+    if len(eps) > 1:
+        raise ValueError(f"q_norm and k_norm have different epsilons: {sorted(eps)}")
+    q, k = hira_qk_norm_rope(q, k, cos, sin, q_weight=None if q_norm is None else q_norm.weight,
+                             k_weight=None if k_norm is None else k_norm.weight, eps=eps.pop() if eps else 1e-6,
+                             interleaved=interleaved)
+    cache_output, _ = past_key_values.update(k, v, module.layer_idx)
+    out, _ = hira_attention(module, q, cache_output, None, attention_mask, scaling=getattr(module, "scaling", None),
+                            hira_config=hira_config)
+    return module.o_proj(out.reshape(b, n, -1)), None
+
+
+def _is_head_rms_norm(norm, width: int) -> bool:
+    """Whether `norm` computes x * rsqrt(mean(x^2) + eps) * weight over `width` channels, seen from what it makes of a vector
+    (a norm about the mean, or with weights about one, does not)."""
+    w, eps = getattr(norm, "weight", None), getattr(norm, "variance_epsilon", getattr(norm, "eps", None))
+    if w is None or eps is None or tuple(w.shape) != (width,):
+        return False
+    x = torch.linspace(-1.0, 2.0, width, device=w.device, dtype=torch.float32)
+    with torch.no_grad():
+        got = norm(x.to(w.dtype)).double()
+    want = x.double() * torch.rsqrt(x.double().square().mean() + eps) * w.double()
+    # three roundings of x, x^ and the product, in the weight's type
+    return bool(((got - want).abs() <= 2 * torch.finfo(w.dtype).eps * want.abs() + 1e-6).all())
+
+
+def patch_attention(model, hira_config=None, *, interleaved: bool = False) -> int:
+    """Gives every attention layer of `model` (a module with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx)
+    `hira_attention_forward` as its forward; returns how many there were.  Run the model under `torch.no_grad()` with
+    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.  Layers whose heads are normalised in a way that `hira_qk_norm_rope` does not
+    do (over other widths than a head's) are refused."""
+    layers = [m for m in model.modules()
+              if all(hasattr(m, a) for a in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "layer_idx"))]
+    if not layers:
+        raise ValueError("the model has no attention layer with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx")
+    for m in layers:
+        for name in ("q_norm", "k_norm"):
+            norm = getattr(m, name, None)
+            if norm is None:
+                continue
+            if not _is_head_rms_norm(norm, m.head_dim):
+                raise ValueError(f"{name} of layer {m.layer_idx} is no RMS norm of single heads")
+    for m in layers:
+        def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+            return hira_attention_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values,
+                                          hira_config=hira_config, interleaved=interleaved, **kwargs)
+        m.forward = MethodType(forward, m)
+    return len(layers)

@@ -17,6 +17,7 @@ from typing import Any, Optional
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
+from .. import index_state as S
 from ..indexer import CUDAIndexer
 from ..searcher import CUDASearcher
 from .hira_config import DeviceMode, HiraConfig
@@ -30,6 +31,7 @@ class CacheOutput:
     prefill_values: Optional[torch.Tensor]
     indexer: CUDAIndexer
     searcher: CUDASearcher
+    shared: Optional["SharedPrompt"] = None    # the prompts and tails of a layer after share_prompt; no index then
 
 
 class HiraCacheLayer(CacheLayerMixin):
@@ -44,6 +46,7 @@ class HiraCacheLayer(CacheLayerMixin):
         self.searcher_kwargs = searcher_kwargs
         self.indexer_cls = None
         self.searcher_cls = None
+        self.shared = None
         if self.device_mode == DeviceMode.CUDA_ONLY:
             self.indexer_cls = CUDAIndexer
             self.searcher_cls = CUDASearcher
@@ -106,6 +109,14 @@ class HiraCacheLayer(CacheLayerMixin):
                 None,
             )
         n = key_states.shape[-2]
+        if self.shared is not None:
+            self.shared.append(key_states, value_states)
+            self.queued_len = self.shared.tail_len
+            return (
+                CacheOutput(queued_keys=self.shared.tail_keys, queued_values=self.shared.tail_values,
+                            prefill_keys=None, prefill_values=None, indexer=None, searcher=self.searcher, shared=self.shared),
+                None,
+            )
         if (self.queued_len == 0 and n >= self.update_every and key_states.dtype == self.dtype
                 and value_states.dtype == self.vdtype and key_states.device == self.device == value_states.device
                 and key_states.shape == (self.B, self.H_kv, n, self.dim)
@@ -130,6 +141,64 @@ class HiraCacheLayer(CacheLayerMixin):
         self.indexed_len += self.queued_len
         self._reset_queue()
 
+    # ---- several continuations of one prompt --------------------------------------
+    def share_prompt(self, branches: int, max_tail: int = 0):
+        """From now on the layer holds `branches` continuations of each of its sequences (sequence b continues what was
+        sequence b // branches): what it has stored is kept once for all of them, as dense keys and values in token order
+        instead of an index, and attended to as a whole (`hira_shared_attention`); what comes goes to a tail of each
+        continuation.  `max_tail` reserves room for that many tokens each."""
+        from ..attention.shared_attention import SharedPrompt
+        if not self.is_initialized:
+            raise ValueError("the layer holds no prompt yet")
+        if self.shared is not None:
+            raise ValueError("the layer's prompts are shared already: use batch_repeat_interleave")
+        self.indexer.wait_pending_update()
+        if self.indexer.state.values is None:
+            raise ValueError("the index stores no values")
+        self.indexer.state.active_parents = self.indexer.active_parents
+        kv = S.export(self.indexer.state, self.indexed_len)
+        kv = [t.view(self.B, self.H_kv, *t.shape[1:]) for t in kv]
+        if self.queued_len:
+            kv = [torch.cat([t, q], dim=2) for t, q in zip(kv, (self.queued_keys, self.queued_values))]
+        self.shared = SharedPrompt(*kv, branches, max_tail=max_tail)
+        self.indexed_len += self.queued_len
+        self.indexer = self._queue_k = self._queue_v = None
+        self.queued_keys, self.queued_values, self.queued_len = self.shared.tail_keys, self.shared.tail_values, 0
+        self.B = self.shared.batch
+
+    def reorder_cache(self, beam_idx):
+        """In place: sequence b goes on from what sequence beam_idx[b] was."""
+        if not self.is_initialized:
+            return
+        if self.shared is not None:
+            self.shared.reorder(beam_idx)
+            return
+        idx = S.check_picks(beam_idx, self.B, self._queue_k.device)
+        self.indexer.reorder(idx)
+        if self.queued_len:
+            S.gather_rows([(self._queue_k, self._queue_k), (self._queue_v, self._queue_v)], idx, self.queued_len)
+
+    def batch_select_indices(self, indices):
+        """Keeps the picked sequences, in their order; one that is picked several times is forked."""
+        if not self.is_initialized:
+            return
+        if self.shared is not None:
+            self.shared = self.shared.select(indices)
+            self.queued_keys, self.queued_values, self.B = self.shared.tail_keys, self.shared.tail_values, self.shared.batch
+            return
+        idx = S.check_picks(indices, self.B, self._queue_k.device)
+        self.indexer = self.indexer.select(idx)
+        old, self.B, n = (self._queue_k, self._queue_v), idx.numel(), self.queued_len
+        self._queue_k, self._queue_v = (torch.empty((self.B, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in old)
+        if n:
+            S.gather_rows(list(zip(old, (self._queue_k, self._queue_v))), idx, n)
+        self.queued_keys, self.queued_values = self._queue_k[:, :, :n], self._queue_v[:, :, :n]
+
+    def batch_repeat_interleave(self, repeats: int):
+        """Forks every sequence into `repeats` that lie one behind another."""
+        if self.is_initialized:
+            self.batch_select_indices(torch.arange(self.B).repeat_interleave(repeats))
+
     def get_mask_sizes(self, cache_position):
         """Accepts the query length as an int (current transformers) or a cache_position
         tensor (the signature the reference was written against, cache/hira_cache.py:155-159)."""
@@ -149,7 +218,9 @@ class HiraCacheLayer(CacheLayerMixin):
     def reset(self):
         if self.is_initialized:
             self.indexer = self.indexer_cls(**self.indexer_kwargs)
-            self._reset_queue()
+            if self.shared is None:
+                self._reset_queue()
+            self.shared = None
             self.is_initialized = False
         if hasattr(self, "cumulative_length"):
             self.cumulative_length = 0
@@ -185,3 +256,21 @@ class HiraCache(Cache):
                cache_kwargs: dict[str, Any] | None = None, *args, **kwargs):
         cache_output, _ = self.layers[layer_idx].update(key_states, value_states, cache_kwargs)
         return cache_output, None
+
+    def share_prompt(self, branches: int, max_tail: int = 0):
+        """`HiraCacheLayer.share_prompt` for every layer: call it after the prompts' forward pass, and go on with
+        `branches` times as many sequences."""
+        for layer in self.layers:
+            layer.share_prompt(branches, max_tail)
+
+    def reorder_cache(self, beam_idx):
+        for layer in self.layers:
+            layer.reorder_cache(beam_idx)
+
+    def batch_select_indices(self, indices):
+        for layer in self.layers:
+            layer.batch_select_indices(indices)
+
+    def batch_repeat_interleave(self, repeats: int):
+        for layer in self.layers:
+            layer.batch_repeat_interleave(repeats)

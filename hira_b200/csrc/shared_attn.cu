@@ -1,0 +1,353 @@
+// Decode attention of a batch whose sequences ("branches") share their prompts.
+//
+//   out[b, hq, t] = softmax(sm_scale * q[b, hq, t] . K) V  over the keys K = prefix[prompt(b)] ++ tail[b]
+//
+// The prefix of a prompt serves all its branches: its keys and values are read once for all query rows of a kv head
+// (branches x group x tokens) instead of once a branch.  A tail is a branch's own; its last n_q keys are those of the
+// query tokens, so token t sees the first tail_len - (n_q - 1 - t) of them.
+//
+// Prefix and tails give softmax partials (m, l, o) per output row, which the merge joins:
+//   M = max m_i,  out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,  and 0 for a row that saw no key.
+#include "shared_attn.cuh"
+#include <math_constants.h>
+
+namespace hira {
+
+constexpr int SA_THREADS = 128;
+constexpr int SA_KEYS = 64;       // keys a tile
+constexpr int SA_PAD = 4;         // floats behind each row in shared memory: rows 4 banks apart
+
+// ---------------------------------------------------------------------------
+// CUDA-core kernel for what the tensor cores do not serve: fp32, and rows wider than 128.
+//
+// One block takes ROWS = 8 * RPT query rows of one item against a run of the item's keys, in tiles of 64 held as fp32
+// in shared memory.  16 lanes share RPT rows: for the products of a tile a lane has RPT rows x 4 keys in registers
+// (RPT + 4 16-byte loads for 16 RPT FMAs), for the weighted sums RPT rows x V / 16 channels.  A row's softmax
+// statistics stay with its 16 lanes, so the blocks only meet to exchange tiles.  fp32 products and sums throughout.
+// ---------------------------------------------------------------------------
+template <typename T, int RPT, int NV, bool TAIL>
+__global__ void __launch_bounds__(SA_THREADS)
+shared_simt_kernel(const SharedAttn P) {
+    constexpr int ROWS = 8 * RPT;
+    extern __shared__ __align__(16) float sa_smem[];
+    const int ldk = P.dim + SA_PAD, ldv = P.vdim + SA_PAD;
+    float* s_q = sa_smem;                       // [ROWS][ldk]
+    float* s_k = s_q + ROWS * ldk;              // [SA_KEYS][ldk]
+    float* s_v = s_k + SA_KEYS * ldk;           // [SA_KEYS][ldv]
+    float* s_p = s_v + SA_KEYS * ldv;           // [SA_KEYS][ROWS + SA_PAD]
+    constexpr int LDP = ROWS + SA_PAD;
+
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int row0 = blockIdx.x * ROWS, split = blockIdx.y;
+    const int item = blockIdx.z, h = item % P.n_kv, owner = item / P.n_kv;      // prompt, or branch of a tail
+    const int per = P.group * P.n_q;
+    const int n_rows = TAIL ? per : P.n_branches * per;
+    const int n_splits = TAIL ? P.tail_parts : P.prefix_parts;
+    const int len = TAIL ? shared_tail_len(P, owner) : shared_prefix_len(P, owner);
+    const T* gk = reinterpret_cast<const T*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
+    const T* gv = reinterpret_cast<const T*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
+    const long long ks = TAIL ? P.tks[2] : P.pks[2], vs = TAIL ? P.tvs[2] : P.pvs[2];
+    auto out_row = [&](int r) {
+        return TAIL ? (owner * P.n_kv + h) * per + r : shared_row(P, owner, h, r);
+    };
+
+    const int kc = P.dim / 8, vc = P.vdim / 8;
+    for (int i = tid; i < ROWS * kc; i += SA_THREADS) {
+        const int r = i / kc, c = i - r * kc;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (row0 + r < n_rows)
+            to_float(load_chunk<T>(reinterpret_cast<const T*>(P.q) + shared_row_offset(P, out_row(row0 + r), P.qs), c), f);
+        float4* d = reinterpret_cast<float4*>(s_q + r * ldk + c * 8);
+        d[0] = make_float4(f[0], f[1], f[2], f[3]);
+        d[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    // keys this row sees
+    int seen[RPT];
+    float m[RPT], l[RPT], o[RPT][NV][4];
+#pragma unroll
+    for (int a = 0; a < RPT; ++a) {
+        const int r = row0 + ty * RPT + a;
+        seen[a] = TAIL ? len - (P.n_q - 1 - r % P.n_q) : len;
+        m[a] = -CUDART_INF_F;
+        l[a] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[a][c][e] = 0.f;
+    }
+    // equal runs of tiles for the splits
+    const int tiles = (len + SA_KEYS - 1) / SA_KEYS;
+    const int t0 = (int)((long long)split * tiles / n_splits), t1 = (int)((long long)(split + 1) * tiles / n_splits);
+    for (int t = t0; t < t1; ++t) {
+        const int k0 = t * SA_KEYS;
+        __syncthreads();      // the tile before is used up (and the queries are in place)
+        for (int i = tid; i < SA_KEYS * kc; i += SA_THREADS) {
+            const int r = i / kc, c = i - r * kc;
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (k0 + r < len) to_float(load_chunk<T>(gk + (k0 + r) * ks, c), f);
+            float4* d = reinterpret_cast<float4*>(s_k + r * ldk + c * 8);
+            d[0] = make_float4(f[0], f[1], f[2], f[3]);
+            d[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
+        for (int i = tid; i < SA_KEYS * vc; i += SA_THREADS) {
+            const int r = i / vc, c = i - r * vc;
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};      // past the last key: nothing there is read
+            if (k0 + r < len) to_float(load_chunk<T>(gv + (k0 + r) * vs, c), f);
+            float4* d = reinterpret_cast<float4*>(s_v + r * ldv + c * 8);
+            d[0] = make_float4(f[0], f[1], f[2], f[3]);
+            d[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
+        __syncthreads();
+        float s[RPT][4];
+#pragma unroll
+        for (int a = 0; a < RPT; ++a)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[a][j] = 0.f;
+        const float* qrow = s_q + ty * RPT * ldk;
+        const float* krow = s_k + tx * ldk;
+#pragma unroll 2
+        for (int d = 0; d < P.dim; d += 4) {
+            float4 kk[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const float4*>(krow + 16 * j * ldk + d);
+#pragma unroll
+            for (int a = 0; a < RPT; ++a) {
+                const float4 qq = *reinterpret_cast<const float4*>(qrow + a * ldk + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[a][j] = __fmaf_rn(qq.x, kk[j].x, s[a][j]);
+                    s[a][j] = __fmaf_rn(qq.y, kk[j].y, s[a][j]);
+                    s[a][j] = __fmaf_rn(qq.z, kk[j].z, s[a][j]);
+                    s[a][j] = __fmaf_rn(qq.w, kk[j].w, s[a][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < RPT; ++a) {
+            float mx = -CUDART_INF_F;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[a][j] = k0 + tx + 16 * j < seen[a] ? s[a][j] * P.scale_log2 : -CUDART_INF_F;
+                mx = fmaxf(mx, s[a][j]);
+            }
+#pragma unroll
+            for (int w = 8; w >= 1; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+            const float nm = fmaxf(m[a], mx), base = nm > -CUDART_INF_F ? nm : 0.f;
+            const float alpha = exp2_approx(m[a] - base);
+            m[a] = nm;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[a][j] = exp2_approx(s[a][j] - base);
+                sum += s[a][j];
+            }
+#pragma unroll
+            for (int w = 8; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            l[a] = __fmaf_rn(l[a], alpha, sum);
+#pragma unroll
+            for (int c = 0; c < NV; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[a][c][e] *= alpha;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s_p[(tx + 16 * j) * LDP + ty * RPT + a] = s[a][j];
+        }
+        __syncwarp();         // a row's weights pass between its 16 lanes only
+#pragma unroll 2
+        for (int k = 0; k < SA_KEYS; ++k) {
+            float p[RPT];
+#pragma unroll
+            for (int a = 0; a < RPT; ++a) p[a] = s_p[k * LDP + ty * RPT + a];
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int ch = tx * 4 + 64 * c;
+                if (ch < P.vdim) {
+                    const float4 v = *reinterpret_cast<const float4*>(s_v + k * ldv + ch);
+#pragma unroll
+                    for (int a = 0; a < RPT; ++a) {
+                        o[a][c][0] = __fmaf_rn(p[a], v.x, o[a][c][0]);
+                        o[a][c][1] = __fmaf_rn(p[a], v.y, o[a][c][1]);
+                        o[a][c][2] = __fmaf_rn(p[a], v.z, o[a][c][2]);
+                        o[a][c][3] = __fmaf_rn(p[a], v.w, o[a][c][3]);
+                    }
+                }
+            }
+        }
+    }
+    const int part = (TAIL ? P.prefix_parts : 0) + split;
+#pragma unroll
+    for (int a = 0; a < RPT; ++a) {
+        const int r = row0 + ty * RPT + a;
+        if (r >= n_rows) continue;
+        const size_t at = (size_t)part * P.n_rows + out_row(r);
+        if (tx == 0) P.part_ml[at] = make_float2(m[a], l[a]);
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int ch = tx * 4 + 64 * c;
+            if (ch < P.vdim) *reinterpret_cast<float4*>(P.part_o + at * P.vdim + ch) = make_float4(o[a][c][0], o[a][c][1], o[a][c][2], o[a][c][3]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The partials of an output row joined, by one warp.
+// ---------------------------------------------------------------------------
+constexpr int SA_MERGE_WARPS = 4;
+template <typename T>
+__global__ void __launch_bounds__(32 * SA_MERGE_WARPS)
+shared_merge_kernel(const SharedAttn P) {
+    const int R = blockIdx.x * SA_MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (R >= P.n_rows) return;
+    const int n = P.prefix_parts + P.tail_parts;
+    float M = -CUDART_INF_F;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, P.part_ml[(size_t)i * P.n_rows + R].x);
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+    const float base = M > -CUDART_INF_F ? M : 0.f;
+    float L = 0.f, acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    const bool mine = lane * 8 < P.vdim;
+    for (int i = 0; i < n; ++i) {
+        const size_t at = (size_t)i * P.n_rows + R;
+        const float2 ml = P.part_ml[at];
+        const float w = exp2_approx(ml.x - base);
+        L = __fmaf_rn(w, ml.y, L);
+        if (mine) {
+            const float4* po = reinterpret_cast<const float4*>(P.part_o + at * P.vdim + lane * 8);
+            const float4 a = po[0], b = po[1];
+            acc[0] = __fmaf_rn(w, a.x, acc[0]); acc[1] = __fmaf_rn(w, a.y, acc[1]);
+            acc[2] = __fmaf_rn(w, a.z, acc[2]); acc[3] = __fmaf_rn(w, a.w, acc[3]);
+            acc[4] = __fmaf_rn(w, b.x, acc[4]); acc[5] = __fmaf_rn(w, b.y, acc[5]);
+            acc[6] = __fmaf_rn(w, b.z, acc[6]); acc[7] = __fmaf_rn(w, b.w, acc[7]);
+        }
+    }
+    if (!mine) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = L == 0.f ? 0.f : acc[e] / L;      // no key seen: 0 (a NaN stays one)
+    store_chunk(reinterpret_cast<T*>(P.out) + shared_row_offset(P, R, P.os), lane, acc);
+}
+
+template <typename T, int RPT, int NV, bool TAIL>
+static int launch_simt(const SharedAttn& P, cudaStream_t s) {
+    auto kern = shared_simt_kernel<T, RPT, NV, TAIL>;
+    const int per = P.group * P.n_q, rows = TAIL ? per : P.n_branches * per;
+    const size_t smem = sizeof(float) * ((size_t)(8 * RPT + SA_KEYS) * (P.dim + SA_PAD) + (size_t)SA_KEYS * (P.vdim + SA_PAD) +
+                                         (size_t)SA_KEYS * (8 * RPT + SA_PAD));
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+        set_error("hira_shared_attn: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));
+        return HIRA_ERR_CUDA;
+    }
+    const dim3 grid((unsigned)((rows + 8 * RPT - 1) / (8 * RPT)), (unsigned)(TAIL ? P.tail_parts : P.prefix_parts),
+                    (unsigned)((TAIL ? P.n_prompts * P.n_branches : P.n_prompts) * P.n_kv));
+    kern<<<grid, SA_THREADS, smem, s>>>(P);
+    HIRA_CHECK_LAUNCH("hira_shared_attn launch");
+    return HIRA_OK;
+}
+
+// rows a block takes: no more than there are, so that a few rows do not pay for the products of many
+static int simt_rows(int rows, int vdim) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 || vdim > 128 ? 32 : 64; }
+
+template <typename T, bool TAIL>
+static int launch_simt_rows(const SharedAttn& P, cudaStream_t s) {
+    const int per = P.group * P.n_q, rows = simt_rows(TAIL ? per : P.n_branches * per, P.vdim);
+    if (P.vdim > 128) {
+        if (rows == 8) return launch_simt<T, 1, 4, TAIL>(P, s);
+        if (rows == 16) return launch_simt<T, 2, 4, TAIL>(P, s);
+        return launch_simt<T, 4, 4, TAIL>(P, s);
+    }
+    if (rows == 8) return launch_simt<T, 1, 2, TAIL>(P, s);
+    if (rows == 16) return launch_simt<T, 2, 2, TAIL>(P, s);
+    if (rows == 32) return launch_simt<T, 4, 2, TAIL>(P, s);
+    return launch_simt<T, 8, 2, TAIL>(P, s);
+}
+
+// Splits of the keys: enough blocks for two an SM, none with fewer than two tiles of its own.
+static int simt_splits(int rows, int items, int len, int vdim) {
+    if (len <= 0) return 0;
+    const int block_rows = simt_rows(rows, vdim), tiles = (len + SA_KEYS - 1) / SA_KEYS;
+    const long long blocks = (long long)((rows + block_rows - 1) / block_rows) * items;
+    long long splits = (2 * SM_COUNT + blocks - 1) / blocks;
+    if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
+    if (splits > 64) splits = 64;
+    return splits < 1 ? 1 : (int)splits;
+}
+
+static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
+    HIRA_CHECK_ARG(a != nullptr, HIRA_ERR_ARG, "hira_shared_attn: arguments are NULL");
+    HIRA_CHECK_ARG(a->dtype == HIRA_F32 || a->dtype == HIRA_BF16, HIRA_ERR_DTYPE,
+                   "hira_shared_attn: dtype %d is neither HIRA_F32 nor HIRA_BF16", a->dtype);
+    HIRA_CHECK_ARG(a->n_prompts >= 1 && a->n_branches >= 1 && a->n_kv >= 1 && a->group >= 1 && a->n_q >= 1, HIRA_ERR_SHAPE,
+                   "hira_shared_attn: n_prompts=%d n_branches=%d n_kv=%d group=%d n_q=%d must be >= 1", a->n_prompts,
+                   a->n_branches, a->n_kv, a->group, a->n_q);
+    HIRA_CHECK_ARG(a->dim >= 8 && a->dim <= 256 && a->dim % 8 == 0 && a->vdim >= 8 && a->vdim <= 256 && a->vdim % 8 == 0,
+                   HIRA_ERR_SHAPE, "hira_shared_attn: dim=%d and vdim=%d must be multiples of 8 in 8..256", a->dim, a->vdim);
+    HIRA_CHECK_ARG(a->prefix_len >= 0 && a->tail_len >= 0 && a->prefix_len < (1 << 30) && a->tail_len < (1 << 30), HIRA_ERR_SHAPE,
+                   "hira_shared_attn: prefix_len=%d tail_len=%d outside 0..2^30", a->prefix_len, a->tail_len);
+    const long long rows = (long long)a->n_prompts * a->n_branches * a->n_kv * a->group * a->n_q;
+    HIRA_CHECK_ARG(rows < (1ll << 30) && (long long)a->n_prompts * a->n_branches * a->n_kv <= 65535, HIRA_ERR_SHAPE,
+                   "hira_shared_attn: %lld query rows, or %lld (branch, kv head) pairs, exceed 2^30 or 65535", rows,
+                   (long long)a->n_prompts * a->n_branches * a->n_kv);
+    HIRA_CHECK_ARG(a->q && a->out, HIRA_ERR_ARG, "hira_shared_attn: q and out must not be NULL");
+    HIRA_CHECK_ARG(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), HIRA_ERR_ARG, "hira_shared_attn: prefix_k / prefix_v is NULL");
+    HIRA_CHECK_ARG(a->tail_len == 0 || (a->tail_k && a->tail_v), HIRA_ERR_ARG, "hira_shared_attn: tail_k / tail_v is NULL");
+    const int es = (int)elem_size(a->dtype);
+    uintptr_t mis = (uintptr_t)a->q | (uintptr_t)a->out;
+    const void* kv[4] = {a->prefix_k, a->prefix_v, a->tail_k, a->tail_v};
+    const int64_t* st[6] = {a->prefix_k_stride, a->prefix_v_stride, a->tail_k_stride, a->tail_v_stride, a->q_stride, a->out_stride};
+    for (int i = 0; i < 4; ++i)
+        if (i < 2 ? a->prefix_len : a->tail_len) mis |= (uintptr_t)kv[i] | (uintptr_t)((st[i][0] | st[i][1] | st[i][2]) * es);
+    for (int i = 4; i < 6; ++i) mis |= (uintptr_t)((st[i][0] | st[i][1] | st[i][2]) * es);
+    HIRA_CHECK_ARG((mis & 15) == 0, HIRA_ERR_ARG, "hira_shared_attn: every row must start on a 16-byte boundary");
+    P = SharedAttn{};
+    P.q = a->q; P.out = a->out;
+    P.pk = a->prefix_k; P.pv = a->prefix_v; P.tk = a->tail_k; P.tv = a->tail_v;
+    P.prefix_lens = a->prefix_lens; P.tail_lens = a->tail_lens;
+    P.n_prompts = a->n_prompts; P.n_branches = a->n_branches; P.n_kv = a->n_kv; P.group = a->group; P.n_q = a->n_q;
+    P.dim = a->dim; P.vdim = a->vdim; P.prefix_len = a->prefix_len; P.tail_len = a->tail_len;
+    P.n_rows = (int)rows;
+    P.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634074);     // log2(e)
+    for (int i = 0; i < 3; ++i) {
+        P.pks[i] = st[0][i]; P.pvs[i] = st[1][i]; P.tks[i] = st[2][i]; P.tvs[i] = st[3][i]; P.qs[i] = st[4][i]; P.os[i] = st[5][i];
+    }
+    const int per = a->group * a->n_q;
+    P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
+    P.tail_parts = simt_splits(per, a->n_prompts * a->n_branches * a->n_kv, a->tail_len, a->vdim);
+    return HIRA_OK;
+}
+static size_t shared_parts_bytes(const SharedAttn& P) {
+    return (size_t)(P.prefix_parts + P.tail_parts) * P.n_rows * (P.vdim + 2) * sizeof(float);
+}
+
+template <typename T>
+static int run_shared(const SharedAttn& P, cudaStream_t s) {
+    int rc = HIRA_OK;
+    if (P.prefix_parts > 0) rc = launch_simt_rows<T, false>(P, s);
+    if (rc == HIRA_OK && P.tail_parts > 0) rc = launch_simt_rows<T, true>(P, s);
+    if (rc != HIRA_OK) return rc;
+    shared_merge_kernel<T><<<(unsigned)((P.n_rows + SA_MERGE_WARPS - 1) / SA_MERGE_WARPS), 32 * SA_MERGE_WARPS, 0, s>>>(P);
+    HIRA_CHECK_LAUNCH("hira_shared_attn merge launch");
+    return HIRA_OK;
+}
+
+}  // namespace hira
+
+using namespace hira;
+
+extern "C" size_t hira_shared_attn_workspace_bytes(const hira_shared_attn_t* a) {
+    SharedAttn P;
+    return shared_plan(a, P) == HIRA_OK ? shared_parts_bytes(P) : 0;
+}
+
+extern "C" int hira_shared_attn(const hira_shared_attn_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+    SharedAttn P;
+    const int rc = shared_plan(a, P);
+    if (rc != HIRA_OK) return rc;
+    const size_t need = shared_parts_bytes(P);
+    HIRA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), HIRA_ERR_CAPACITY,
+                   "hira_shared_attn: a 16-byte aligned workspace of %zu bytes is needed, %zu given", need, workspace_bytes);
+    P.part_o = reinterpret_cast<float*>(workspace);
+    P.part_ml = reinterpret_cast<float2*>(P.part_o + (size_t)(P.prefix_parts + P.tail_parts) * P.n_rows * P.vdim);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return a->dtype == HIRA_BF16 ? run_shared<__nv_bfloat16>(P, s) : run_shared<float>(P, s);
+}

@@ -590,6 +590,123 @@ def assign(points: torch.Tensor, cents: torch.Tensor, use_tensor_cores: bool = F
     return idx, d2
 
 
+# ---- several continuations of one prompt ----------------------------------------------------------------
+def row_strides(t: torch.Tensor) -> Optional[tuple]:
+    """Element strides of a 4-d tensor's first three dimensions where its rows are contiguous and all start on
+    16-byte boundaries, else None.  A stride along a dimension of one says nothing and counts as 0."""
+    a, b, c, d = t.shape
+    s = t.stride()
+    if (s[3] != 1 and d > 1) or t.data_ptr() % 16:
+        return None
+    st = (s[0] if a > 1 else 0, s[1] if b > 1 else 0, s[2] if c > 1 else 0)
+    return None if (st[0] | st[1] | st[2]) * t.element_size() % 16 else st
+
+
+def writable_rows(t: torch.Tensor) -> bool:
+    """Whether rows can be written to `t`: as `row_strides`, and no two of them the same."""
+    return row_strides(t) is not None and all(s for n, s in zip(t.shape, t.stride()) if n > 1)
+
+
+def with_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a dense copy of it where `row_strides` does not accept it."""
+    return t if row_strides(t) is not None else aligned(t.contiguous())
+
+
+def shared_attn(q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, sm_scale: float, out):
+    """hira_shared_attn on tensors that `row_strides` accepts (tails and lengths may be None)."""
+    lib = L.load()
+    b, hq, n_q, d = q.shape
+    p, h, n, vdim = prefix_v.shape
+    a = L.HiraSharedAttnStruct()
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.prefix_k, a.prefix_v, a.prefix_lens, a.tail_lens = L.ptr(prefix_k), L.ptr(prefix_v), L.ptr(prefix_lens), L.ptr(tail_lens)
+    a.q_stride[:], a.out_stride[:] = row_strides(q), row_strides(out)
+    a.prefix_k_stride[:], a.prefix_v_stride[:] = row_strides(prefix_k), row_strides(prefix_v)
+    a.prefix_len = n
+    if tail_k is not None:
+        a.tail_k, a.tail_v, a.tail_len = L.ptr(tail_k), L.ptr(tail_v), tail_k.shape[2]
+        a.tail_k_stride[:], a.tail_v_stride[:] = row_strides(tail_k), row_strides(tail_v)
+    a.dtype, a.n_prompts, a.n_branches, a.n_kv, a.group = L.dtype_code(q.dtype), p, b // p, h, hq // h
+    a.n_q, a.dim, a.vdim, a.sm_scale = n_q, d, vdim, float(sm_scale)
+    with torch.cuda.device(q.device):
+        nbytes = int(lib.hira_shared_attn_workspace_bytes(C.byref(a)))
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
+        L.check(lib.hira_shared_attn(C.byref(a), L.ptr(ws), nbytes, L.current_stream(q.device)), "hira_shared_attn")
+    return out
+
+
+def check_picks(indices, n: int, device) -> torch.Tensor:
+    """Indices of sequences as a contiguous int64 tensor on `device`.  What is on the host is checked here
+    (the kernels check what is on the device); a mask becomes the indices it keeps."""
+    t = torch.as_tensor(indices)
+    if t.ndim != 1:
+        raise ValueError(f"indices must be one-dimensional, got {tuple(t.shape)}")
+    if t.dtype == torch.bool:
+        if t.numel() != n:
+            raise ValueError(f"a mask of {t.numel()} does not fit {n} sequences")
+        t = t.nonzero().flatten()
+    elif t.dtype.is_floating_point or t.dtype.is_complex:
+        if t.numel():
+            raise ValueError(f"indices must be whole numbers, got {t.dtype}")
+        t = t.to(torch.int64)
+    if not t.is_cuda and t.numel() and not (0 <= int(t.min()) and int(t.max()) < n):
+        raise ValueError(f"indices outside 0..{n - 1}: {t.tolist()}")
+    return t.to(device=device, dtype=torch.int64).contiguous()
+
+
+def gather_rows(pairs, index: torch.Tensor, used_rows: int, status: Optional[torch.Tensor] = None):
+    """hira_gather of the first `used_rows` rows of (source, destination) tensors (B, H, rows, D) whose rows are
+    contiguous; source and destination the same tensor: in place."""
+    lib = L.load()
+    items = (L.HiraGatherItemStruct * len(pairs))()
+    for it, (src, dst) in zip(items, pairs):
+        e = src.element_size()
+        it.src, it.dst, it.n_seg = src.data_ptr(), dst.data_ptr(), src.shape[1]
+        it.src_seq_stride, it.src_seg_stride = src.stride(0) * e, src.stride(1) * e
+        it.dst_seq_stride, it.dst_seg_stride = dst.stride(0) * e, dst.stride(1) * e
+        it.bytes = it.bytes_filled = used_rows * src.shape[3] * e
+    src, dst = pairs[0]
+    with torch.cuda.device(src.device):
+        L.check(lib.hira_gather(items, len(pairs), L.ptr(index), src.shape[0], index.numel(), 1 if src is dst else 0, L.ptr(status),
+                                L.current_stream(src.device)), "hira_gather")
+
+
+def _with_q8(st: IndexState) -> L.HiraIndexStruct:
+    """The struct of `st` with its int8 side copy, also when enable_int8_copy has left that out of the view."""
+    s = L.HiraIndexStruct.from_buffer_copy(st._struct)
+    for name in st.Q8_ARRAYS:
+        setattr(s, name, L.ptr(getattr(st, name)))
+    return s
+
+
+def gather_index(src: IndexState, dst: IndexState, index: torch.Tensor, n_src: int, samples: Optional[torch.Tensor] = None):
+    """hira_gather_index: sequences `index` of `src` (of `n_src`, heads folded) into `dst`, which may be `src`."""
+    lib = L.load()
+    a, b = _with_q8(src), _with_q8(dst)
+    nbytes = 0 if samples is None else samples[0].numel() * samples.element_size()
+    with torch.cuda.device(src.device):
+        L.check(lib.hira_gather_index(C.byref(a), C.byref(b), n_src, index.numel(), L.ptr(index), L.ptr(samples), nbytes,
+                                      L.ptr(dst.status), L.current_stream(src.device)), "hira_gather_index")
+
+
+def qk_norm_rope(q, k, cos, sin, q_weight, k_weight, eps: float, interleaved: bool, out_q, out_k):
+    """hira_qk_norm_rope on tensors that `row_strides` accepts; cos / sin (B or 1, n, R) with contiguous rows."""
+    lib = L.load()
+    b, hq, n, d = q.shape
+    a = L.HiraRopeStruct()
+    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr()
+    a.q_weight, a.k_weight, a.cos, a.sin = L.ptr(q_weight), L.ptr(k_weight), L.ptr(cos), L.ptr(sin)
+    a.q_stride[:], a.k_stride[:] = row_strides(q), row_strides(k)
+    a.q_out_stride[:], a.k_out_stride[:] = row_strides(out_q), row_strides(out_k)
+    a.cos_stride[:] = (cos.stride(0) if cos.shape[0] > 1 else 0, cos.stride(1))
+    a.sin_stride[:] = (sin.stride(0) if sin.shape[0] > 1 else 0, sin.stride(1))
+    a.dtype, a.table_dtype, a.batch, a.n_tokens, a.q_heads, a.k_heads = L.dtype_code(q.dtype), L.dtype_code(cos.dtype), b, n, hq, k.shape[1]
+    a.dim, a.rotary, a.interleaved, a.eps = d, cos.shape[2], int(bool(interleaved)), float(eps)
+    with torch.cuda.device(q.device):
+        L.check(lib.hira_qk_norm_rope(C.byref(a), L.current_stream(q.device)), "hira_qk_norm_rope")
+    return out_q, out_k
+
+
 class DecodeStep:
     """Device scratch and events of `hira_decode_step` for one index: the whole decode step of a
     layer (query copy, threshold, search, sparse attention, output copy and, beside them on a

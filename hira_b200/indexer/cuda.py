@@ -20,6 +20,7 @@ Differences by design:
 """
 from __future__ import annotations
 
+import copy
 from enum import Enum
 from typing import Optional
 
@@ -73,6 +74,7 @@ class CUDAIndexer(BaseIndexer):
         self._appended = 0        # keys appended since the build
         self._n_keys = 0
         self._built_keys = 0      # keys of the latest build: every head holds at least as many
+        self.batch = 1            # sequences folded into the heads
 
     # ---- reference attribute names as views ---------------------------------
     @property
@@ -168,7 +170,9 @@ class CUDAIndexer(BaseIndexer):
     @torch.no_grad()
     def build(self, keys: torch.Tensor, values: Optional[torch.Tensor] = None):
         """keys (B, H, L, D); values optional (B, H, L, V)."""
-        return self._build(keys, values, reuse=None)
+        self._build(keys, values, reuse=None)
+        self.batch = max(1, int(keys.shape[0]))
+        return self
 
     def _build(self, keys, values, reuse: Optional[S.IndexState]):
         """`reuse`: a state of this indexer whose arrays are taken over when they are large enough
@@ -410,6 +414,8 @@ class CUDAIndexer(BaseIndexer):
         """Raises if an append ran out of pre-allocated slots (reads one word from the device)."""
         self.wait_pending_update() if self.state is not None else None
         code = int(self.state.status.item())
+        if code & 8:
+            raise RuntimeError("a sequence that does not exist was picked (status bit HIRA_STATUS_BAD_INDEX)")
         if code & 4:
             raise RuntimeError("the tensor-core assignment of the build gave up on a bounded wait for some points "
                                "(status bit HIRA_STATUS_ASSIGN_FAILED); rebuild with use_tensor_cores=False")
@@ -429,11 +435,59 @@ class CUDAIndexer(BaseIndexer):
         self._build(keys.unsqueeze(0), None if values is None else values.unsqueeze(0), reuse=st)
         return self
 
+    # ---- sequences forked, reordered, compacted ------------------------------
+    @torch.no_grad()
+    def reorder(self, indices):
+        """In place: sequence b (of the B that were built) becomes what sequence indices[b] was; any may be picked many
+        times.  Sequences that pick themselves are not touched, and nothing is allocated.  `indices` (B,): on the host it
+        is checked, on the device an index out of range leaves its sequence as it was and is reported by `check_status`."""
+        st = self._settled()
+        idx = S.check_picks(indices, self.batch, st.device)
+        if idx.numel() != self.batch:
+            raise ValueError(f"{idx.numel()} indices for {self.batch} sequences")
+        if self._scan_pending:
+            self._scan_slots.fill_(-1)    # that scan was of other sequences
+            self._scan_pending = False
+        drawn = getattr(self, "_tau_samples", None)
+        S.gather_index(st, st, idx, self.batch, drawn[1] if drawn is not None and drawn[0] is st else None)
+        return self
+
+    @torch.no_grad()
+    def select(self, indices) -> "CUDAIndexer":
+        """A new index of the picked sequences: forked where an index repeats, compacted where some are left out.  This
+        one stays as it is.  An index on the device that is out of range leaves an empty sequence and is reported by
+        `check_status`."""
+        st = self._settled()
+        idx = S.check_picks(indices, self.batch, st.device)
+        n = idx.numel()
+        if n == 0:
+            raise ValueError("no sequence picked")
+        heads = self.num_heads // self.batch
+        new = copy.copy(self)
+        new.state = S.IndexState(n_heads=n * heads, dim=st.dim, vdim=st.vdim, bf=st.bf, depth=st.depth, cap_parents=st.cap_parents,
+                                 dtype=st.dtype, vdtype=st.vdtype, device=st.device, with_values=st.values is not None,
+                                 int8_copy=st.int8_copy, cleared=False)
+        new.state.status.copy_(st.status)
+        new.num_heads, new.batch = n * heads, n
+        new._snapshot = new._scan_slots = new._searched = new._pending_append = new._pinned = new._tau_samples = None
+        new._scan_pending = new._searched_fresh = False
+        S.gather_index(st, new.state, idx, self.batch)
+        return new
+
+    def _settled(self) -> S.IndexState:
+        """The state, with no update running and its bound on the slots in use set."""
+        if self.state is None:
+            raise ValueError("Indexer is not built")
+        self.wait_pending_update()
+        self.state.active_parents = self.active_parents
+        return self.state
+
     # ---- checkpoint ---------------------------------------------------------
     def state_dict(self) -> dict:
         self.wait_pending_update() if self.state is not None else None
         d = self.state.state_dict()
-        d["meta"].update(n_keys=self._n_keys, parents_bound=self._parents_bound, gp_bound=self._gp_bound)
+        d["meta"].update(n_keys=self._n_keys, parents_bound=self._parents_bound, gp_bound=self._gp_bound,
+                         batch=self.batch)
         return d
 
     @classmethod
@@ -449,4 +503,5 @@ class CUDAIndexer(BaseIndexer):
         self._n_keys = m.get("n_keys", 0)
         self._parents_bound = m.get("parents_bound", st.cap_parents)
         self._gp_bound = m.get("gp_bound", st.cap_gp)
+        self.batch = m.get("batch", 1)
         return self

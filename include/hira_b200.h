@@ -52,6 +52,7 @@ extern "C" {
                                        wait for some points (their hira_assign index is -1); the
                                        build placed them under centre 0, so the index is valid but
                                        of poor quality: rebuild with use_tensor_cores = 0 */
+#define HIRA_STATUS_BAD_INDEX 8    /* hira_gather, hira_gather_index: a picked sequence does not exist */
 
 /* search flags */
 #define HIRA_GATE_GT 0x0          /* keep node iff q.c + r >  tau (reference Triton kernels, kernels/triton_search_kernels.py:49,114,131) */
@@ -512,6 +513,84 @@ int hira_assign(const void* points, const void* cents, int32_t dtype,
                 int32_t n_heads, int32_t n, int32_t k, int32_t dim,
                 int32_t use_tensor_cores, float* csq_scratch, int32_t* out_idx,
                 float* out_dist2, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Several continuations of one prompt.
+ *
+ * Decode attention of a batch whose sequences ("branches") share their prompts: sequence b = prompt * n_branches + j
+ * attends to the keys of its prompt, kept once for all its branches, and to a tail of its own,
+ *   out[b][hq][t] = softmax(sm_scale q[b][hq][t] . K) V,   K = prefix[prompt][hq / group][0 .. prefix_len)
+ *                                                           ++ tail[b][hq / group][0 .. tail_len - (n_q - 1 - t)).
+ * The last n_q keys of a tail are those of the query tokens, so token t does not see the ones behind it.  A row that
+ * sees no key is 0.  Softmax and sums in fp32, the output rounded once to `dtype`; with bf16 rows of up to 128 the
+ * softmax weights enter the tensor cores as bf16, each off by at most 2^-8 of itself, as the output's own rounding.
+ * What lies behind a length is never used, whatever it holds.
+ * All rows start on 16-byte boundaries with their elements one behind another; strides are in elements: (prompt or
+ * branch, head, row or token).  Any of them may be 0 or negative on the tails, the queries and the CUDA-core path.
+ * `workspace` belongs to the call until it is done; hira_shared_attn_workspace_bytes gives its size (16-byte aligned). */
+typedef struct hira_shared_attn {
+    const void* q;              /* [n_prompts * n_branches][n_kv * group][n_q][dim]   */
+    const void* prefix_k;       /* [n_prompts][n_kv][prefix_len][dim]                 */
+    const void* prefix_v;       /* [n_prompts][n_kv][prefix_len][vdim]                */
+    const void* tail_k;         /* [n_prompts * n_branches][n_kv][tail_len][dim]      */
+    const void* tail_v;         /* [n_prompts * n_branches][n_kv][tail_len][vdim]     */
+    void* out;                  /* [n_prompts * n_branches][n_kv * group][n_q][vdim]  */
+    const int32_t* prefix_lens; /* [n_prompts] keys a prefix really holds, cut to 0..prefix_len; NULL: all      */
+    const int32_t* tail_lens;   /* [n_prompts * n_branches] the same of the tails; NULL: all                    */
+    int64_t q_stride[3], prefix_k_stride[3], prefix_v_stride[3], tail_k_stride[3], tail_v_stride[3], out_stride[3];
+    int32_t dtype, n_prompts, n_branches, n_kv, group, n_q, dim, vdim, prefix_len, tail_len;
+    float sm_scale;
+} hira_shared_attn_t;
+size_t hira_shared_attn_workspace_bytes(const hira_shared_attn_t* args);
+int hira_shared_attn(const hira_shared_attn_t* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sequences of a cache forked, reordered or compacted: out[j] = in[index[j]] for j in 0..n_dst, all arrays in one
+ * launch.  index [n_dst] on the device.  Into other memory (in_place = 0) every array of every sequence is written whole:
+ * the bytes in use copied, the rest filled.  In place (n_src == n_dst, src == dst) sequences that pick themselves are
+ * not touched, and of the others only the bytes in use are replaced, as if all had been read before the first was
+ * written.  An index outside 0..n_src sets HIRA_STATUS_BAD_INDEX in *status (may be NULL) and leaves that sequence
+ * empty (in place: as it was).  At most 24 arrays, 2048 sequences. */
+typedef struct hira_gather_item {
+    const void* src;
+    void* dst;
+    int64_t src_seq_stride, dst_seq_stride;   /* bytes between sequences                                    */
+    int64_t src_seg_stride, dst_seg_stride;   /* bytes between the parts (heads) of a sequence              */
+    int64_t bytes;                            /* in use at the start of each part (multiple of 4)           */
+    int64_t bytes_filled;                     /* bytes of a part of dst that are written (>= bytes)         */
+    int32_t n_seg;                            /* parts of a sequence                                        */
+    uint32_t fill;                            /* word behind the bytes in use                               */
+} hira_gather_item_t;
+int hira_gather(const hira_gather_item_t* items, int32_t n_items, const int64_t* index, int32_t n_src, int32_t n_dst,
+                int32_t in_place, int32_t* status, void* stream);
+
+/* hira_gather over the arrays of an index (heads folded as sequence * heads + head, `from` and `to` of one capacity;
+ * from == to: in place), the int8 side copy with them.  Visits the parent slots below from->active_parents (0 = all).
+ * samples: optional [heads of all sequences][sample_bytes] of rows drawn from the index (threshold finder), which
+ * follow their sequences; in place only. */
+int hira_gather_index(const hira_index_t* from, const hira_index_t* to, int32_t n_src, int32_t n_dst, const int64_t* index,
+                      void* samples, int64_t sample_bytes, int32_t* status, void* stream);
+
+/* Norms of the query and key heads and the rotation by position in one pass, from q, k to q_out, k_out (which may be
+ * q, k themselves):
+ *   x^ = x * rsqrt(mean(x^2) + eps) * weight    (weight NULL: x^ = x)
+ *   y_i = x^_i cos_i - x^_p sin_i,  y_p = x^_p cos_p + x^_i sin_p
+ * for the channel pairs (i, p) = (i, i + rotary/2), or (2i, 2i + 1) when interleaved, below `rotary`; the channels
+ * behind pass through.  fp32, rounded once.  Tables [batch][n_tokens][rotary], strides in elements (0: one for all
+ * sequences).  Strides of the heads' rows: (sequence, head, token). */
+typedef struct hira_rope {
+    const void* q;         /* [batch][q_heads][n_tokens][dim]  */
+    const void* k;         /* [batch][k_heads][n_tokens][dim]  */
+    void* q_out;
+    void* k_out;
+    const void* q_weight;  /* [dim] in `dtype`, or NULL        */
+    const void* k_weight;
+    const void* cos;
+    const void* sin;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3], cos_stride[2], sin_stride[2];
+    int32_t dtype, table_dtype, batch, n_tokens, q_heads, k_heads, dim, rotary, interleaved;
+    float eps;
+} hira_rope_t;
+int hira_qk_norm_rope(const hira_rope_t* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,166 @@
+"""What the operators for several continuations refuse, and what the host decides, on the CPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from hira_b200 import CUDAIndexer, SharedPrompt, hira_qk_norm_rope, hira_shared_attention, patch_attention
+from hira_b200 import _lib as L
+from hira_b200 import index_state as S
+
+
+def _t(*shape, dtype=torch.bfloat16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+GOOD = dict(query=(6, 4, 1, 64), prefix_keys=(2, 2, 9, 64), prefix_values=(2, 2, 9, 64), tail_keys=(6, 2, 3, 64), tail_values=(6, 2, 3, 64))
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(query=(6, 4, 64)), "4 dimensions"), (dict(prefix_keys=(2, 2, 8, 64)), "fit neither"), (dict(prefix_keys=(2, 2, 9, 72)), "fit neither"),
+    (dict(query=(5, 4, 1, 64), tail_keys=(5, 2, 3, 64), tail_values=(5, 2, 3, 64)), "no multiple"), (dict(query=(6, 3, 1, 64)), "no multiple"),
+    (dict(tail_keys=(6, 2, 4, 64)), "do not fit"), (dict(tail_values=(6, 2, 3, 72)), "do not fit"), (dict(tail_keys=(3, 2, 3, 64)), "do not fit"),
+    (dict(query=(6, 4, 1, 60), prefix_keys=(2, 2, 9, 60), tail_keys=(6, 2, 3, 60)), "multiple of 8"),
+    (dict(prefix_values=(2, 2, 9, 264), tail_values=(6, 2, 3, 264)), "multiple of 8"), (dict(tail_keys=None), "together"), ({}, "CUDA"),
+])
+def test_shared_attention_refuses(change, match):
+    shapes = {**GOOD, **change}
+    with pytest.raises(ValueError, match=match):
+        hira_shared_attention(**{k: None if s is None else _t(*s) for k, s in shapes.items()})
+
+
+def test_shared_attention_refuses_types_lengths_and_gradients():
+    a = {k: _t(*s) for k, s in GOOD.items()}
+    with pytest.raises(ValueError, match="query is"):
+        hira_shared_attention(**{**a, "tail_keys": a["tail_keys"].float()})
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        hira_shared_attention(**{k: t.half() for k, t in a.items()})
+    for kw, match in ((dict(prefix_lens=[9, 10]), "outside"), (dict(prefix_lens=[-1, 1]), "outside"), (dict(prefix_lens=[1]), "whole numbers"),
+                      (dict(tail_lens=[1.0] * 6), "whole numbers"), (dict(tail_lens=[4] * 6), "outside")):
+        with pytest.raises(ValueError, match=match):
+            hira_shared_attention(**a, **kw)
+    with pytest.raises(ValueError, match="without tails"):
+        hira_shared_attention(a["query"], a["prefix_keys"], a["prefix_values"], tail_lens=[0] * 6)
+    with pytest.raises(ValueError, match="no backward"):
+        hira_shared_attention(**{**a, "query": a["query"].float().requires_grad_().bfloat16()})
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(key=(2, 2, 5, 64)), "does not go"), (dict(key=(2, 2, 4, 72)), "does not go"), (dict(cos=(3, 4, 64)), "must be"), (dict(cos=(2, 5, 64)), "must be"),
+    (dict(cos=(2, 4, 32)), "differ"), (dict(cos=(2, 4, 7), sin=(2, 4, 7)), "even"), (dict(cos=(2, 4, 66), sin=(2, 4, 66)), "at most"),
+    (dict(q_weight=(32,)), "q_weight"), (dict(query=(2, 4, 4, 60), key=(2, 2, 4, 60)), "multiple of 8"), ({}, "CUDA"),
+])
+def test_rotation_refuses(kw, match):
+    shapes = {**dict(query=(2, 4, 4, 64), key=(2, 2, 4, 64), cos=(2, 4, 64), sin=(2, 4, 64)), **kw}
+    with pytest.raises(ValueError, match=match):
+        hira_qk_norm_rope(**{k: _t(*s) for k, s in shapes.items()})
+
+
+def test_rotation_refuses_types_and_outputs():
+    q, k, c = _t(2, 4, 4, 64), _t(2, 2, 4, 64), _t(2, 4, 64)
+    for kw, match in ((dict(q_weight=torch.ones(64)), "q_weight"), (dict(out_q=q.float()), "out_q"), (dict(out_k=k[:, :1].expand(2, 2, 4, 64)), "out_k"),
+                      (dict(out_q=q.transpose(1, 2).contiguous().transpose(1, 2)[..., :32]), "out_q"), (dict(out_q=q.flip(0).view(2, 4, 4, 64)), "CUDA")):
+        with pytest.raises(ValueError, match=match):
+            hira_qk_norm_rope(q, k, c, c, **kw)
+    buf = _t(2, 6, 5, 64)
+    with pytest.raises(ValueError, match="apart"):       # one row off: rows would be overwritten before they are read
+        hira_qk_norm_rope(buf[:, :4, :4], buf[:, 4:, :4], c, c, out_q=buf[:, :4, 1:])
+    with pytest.raises(ValueError, match="query is"):
+        hira_qk_norm_rope(q, k.float(), c, c)
+    with pytest.raises(ValueError, match="no backward"):
+        hira_qk_norm_rope(q.float().requires_grad_(), k.float(), c, c)
+    with pytest.raises(ValueError, match="no attention layer"):
+        patch_attention(torch.nn.Linear(2, 2))
+
+
+@pytest.mark.parametrize("picks,match", [([0, 3], "outside"), ([-1], "outside"), ([[0]], "one-dimensional"), ([0.5], "whole"), ([True, False], "mask")])
+def test_picks_are_checked_on_the_host(picks, match):
+    with pytest.raises(ValueError, match=match):
+        S.check_picks(picks, 3, "cpu")
+    assert S.check_picks([True, False, True], 3, "cpu").tolist() == [0, 2]
+    assert S.check_picks(torch.tensor([2, 0], dtype=torch.int32), 3, "cpu").dtype == torch.int64
+
+
+def test_shared_prompt_refuses():
+    k = _t(2, 2, 9, 64)
+    for args, match in (((k, k, 0), "branches"), ((k, _t(2, 2, 8, 64), 2), "agree"), ((k, k.float(), 2), "agree"), ((k.half(), k.half(), 2), "unsupported"),
+                        ((k[0], k, 2), "4 dimensions")):
+        with pytest.raises(ValueError, match=match):
+            SharedPrompt(*args)
+    p = SharedPrompt(k, k, 3, max_tail=2)
+    for shape in ((6, 2, 1, 72), (5, 2, 1, 64), (6, 1, 1, 64)):
+        with pytest.raises(ValueError, match="do not continue"):
+            p.append(_t(*shape), _t(*shape))
+    with pytest.raises(ValueError, match="do not continue"):
+        p.append(_t(6, 2, 1, 64), _t(6, 2, 2, 64))
+    for n in (1, 1, 5, 20):
+        p.append(torch.full((6, 2, n, 64), float(n)).bfloat16(), _t(6, 2, n, 64))
+    assert p.tail_len == 27 and p.tail_keys[0, 0, :, 0].tolist() == [1.0] * 2 + [5.0] * 5 + [20.0] * 20
+    for picks, match in (([0, 1, 2, 3, 4], "apart"), ([0, 1, 2], "apart"), ([3, 4, 5, 0, 1, 2], "apart"), ([], "picked")):
+        with pytest.raises(ValueError, match=match):
+            p.select(picks)
+    with pytest.raises(ValueError, match="indices for"):
+        p.reorder([0, 3])
+
+
+def test_an_index_that_is_not_built_cannot_be_picked_from():
+    for f in (CUDAIndexer(3, 1, 8).reorder, CUDAIndexer(3, 1, 8).select):
+        with pytest.raises(ValueError, match="not built"):
+            f([0])
+
+
+def _args(**kw):
+    a = L.HiraSharedAttnStruct()
+    for n in ("q", "prefix_k", "prefix_v", "tail_k", "tail_v", "out"):
+        setattr(a, n, 1 << 20)
+    for n, v in dict(dtype=L.HIRA_BF16, n_prompts=1, n_branches=2, n_kv=2, group=2, n_q=1, dim=64, vdim=64, prefix_len=10, tail_len=3).items():
+        setattr(a, n, v)
+    for n, v in kw.items():
+        if isinstance(v, tuple):
+            getattr(a, n)[:] = v
+        else:
+            setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=7), L.HIRA_ERR_DTYPE), (dict(n_kv=0), L.HIRA_ERR_SHAPE), (dict(dim=60), L.HIRA_ERR_SHAPE), (dict(vdim=264), L.HIRA_ERR_SHAPE),
+    (dict(prefix_len=-1), L.HIRA_ERR_SHAPE), (dict(n_branches=1 << 20), L.HIRA_ERR_SHAPE), (dict(q=None), L.HIRA_ERR_ARG),
+    (dict(prefix_v=None), L.HIRA_ERR_ARG), (dict(tail_k=None), L.HIRA_ERR_ARG), (dict(q=(1 << 20) + 8), L.HIRA_ERR_ARG),
+    (dict(tail_v_stride=(0, 4, 64)), L.HIRA_ERR_ARG), ({}, L.HIRA_ERR_CAPACITY),
+])
+def test_library_refuses_before_any_launch(kw, code):
+    lib, a = L.load(), _args(**kw)
+    need = lib.hira_shared_attn_workspace_bytes(C.byref(a))
+    assert (need > 0) == (code == L.HIRA_ERR_CAPACITY)
+    assert lib.hira_shared_attn(C.byref(a), None, 0, None) == code and lib.hira_last_error()
+    assert lib.hira_shared_attn(None, None, 0, None) == L.HIRA_ERR_ARG
+
+
+def test_library_refuses_gathers_that_do_not_fit():
+    lib, item = L.load(), L.HiraGatherItemStruct
+    one = lambda **kw: (item * 1)(item(**{**dict(src=4096, dst=8192, n_seg=1, bytes=16, bytes_filled=16), **kw}))
+    for items, n, src, dst, place, code in (
+            (one(), 1, 2, 3, 1, L.HIRA_ERR_SHAPE), (one(), 1, 0, 1, 0, L.HIRA_ERR_SHAPE), (one(), 1, 2049, 1, 0, L.HIRA_ERR_SHAPE),
+            (one(), 25, 1, 1, 0, L.HIRA_ERR_SHAPE), (one(bytes=32), 1, 1, 1, 0, L.HIRA_ERR_SHAPE), (one(), 1, 1, 1, 1, L.HIRA_ERR_ARG),
+            (one(dst=4096), 1, 1, 1, 0, L.HIRA_ERR_ARG), (one(bytes=14), 1, 1, 1, 0, L.HIRA_ERR_ARG), (one(src=None), 1, 1, 1, 0, L.HIRA_ERR_ARG)):
+        assert lib.hira_gather(items, n, 4096, src, dst, place, None, None) == code and lib.hira_last_error()
+    assert lib.hira_gather(None, 1, 4096, 1, 1, 0, None, None) == L.HIRA_ERR_ARG
+    assert lib.hira_gather(one(n_seg=0), 1, 4096, 1, 1, 0, None, None) == L.HIRA_OK      # nothing to move
+    a = S.IndexState(n_heads=4, dim=64, vdim=64, bf=8, depth=2, cap_parents=16, dtype=torch.float32, vdtype=torch.float32, device="cpu")
+    b = S.IndexState(n_heads=6, dim=64, vdim=64, bf=8, depth=2, cap_parents=17, dtype=torch.float32, vdtype=torch.float32, device="cpu")
+    assert lib.hira_gather_index(a.struct, b.struct, 2, 3, 4096, None, 0, None, None) == L.HIRA_ERR_SHAPE
+    assert lib.hira_gather_index(a.struct, a.struct, 3, 3, 4096, None, 0, None, None) == L.HIRA_ERR_SHAPE
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=5), L.HIRA_ERR_DTYPE), (dict(table_dtype=5), L.HIRA_ERR_DTYPE), (dict(dim=12), L.HIRA_ERR_SHAPE), (dict(rotary=65), L.HIRA_ERR_SHAPE),
+    (dict(rotary=72), L.HIRA_ERR_SHAPE), (dict(batch=65536), L.HIRA_ERR_SHAPE), (dict(k=None), L.HIRA_ERR_ARG), (dict(sin=None), L.HIRA_ERR_ARG),
+    (dict(q_out=4100), L.HIRA_ERR_ARG), (dict(batch=0), L.HIRA_OK), (dict(n_tokens=0), L.HIRA_OK),
+])
+def test_library_refuses_rotations_that_do_not_fit(kw, code):
+    a = L.HiraRopeStruct(q=4096, k=8192, q_out=4096, k_out=8192, cos=512, sin=1024, dtype=0, table_dtype=0, batch=1, n_tokens=1, q_heads=1,
+                         k_heads=1, dim=64, rotary=64, eps=1e-6)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    assert L.load().hira_qk_norm_rope(C.byref(a), None) == code
