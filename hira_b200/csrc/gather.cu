@@ -173,7 +173,7 @@ extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, con
     const long long* idx = reinterpret_cast<const long long*>(index);
     if (in_place) {
         const size_t smem = (size_t)cols * n_dst * 16;
-        if (smem > 32 * 1024) {      // beside 16 KB of lists
+        if (smem > 24 * 1024) {      // beside 16 KB of lists: more than the 48 KB a launch may take unasked
             const cudaError_t e = cudaFuncSetAttribute(permute_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) {
                 set_error("hira_gather: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));

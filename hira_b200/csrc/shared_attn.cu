@@ -197,9 +197,18 @@ __global__ void __launch_bounds__(32 * SA_MERGE_WARPS)
 shared_merge_kernel(const SharedAttn P) {
     const int R = blockIdx.x * SA_MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (R >= P.n_rows) return;
-    const int n = P.prefix_parts + P.tail_parts;
+    const int bh = R / P.n_q, heads = P.n_kv * P.group;
+    const int item = bh / heads / P.n_branches * P.n_kv + bh % heads / P.group;
+    // the partials there are: the item's own, then (from prefix_parts on) the tail's
+    const int np = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0, n = np + P.tail_parts;
+    auto part = [&](int i) { return (size_t)(i < np ? i : i - np + P.prefix_parts) * P.n_rows + R; };
     float M = -CUDART_INF_F;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, P.part_ml[(size_t)i * P.n_rows + R].x);
+    bool bad = false;
+    for (int i = lane; i < n; i += 32) {
+        const float m = P.part_ml[part(i)].x;
+        bad |= m != m;
+        M = fmaxf(M, m);
+    }
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
     const float base = M > -CUDART_INF_F ? M : 0.f;
@@ -207,9 +216,11 @@ shared_merge_kernel(const SharedAttn P) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
     const bool mine = lane * 8 < P.vdim;
+    if (__any_sync(0xffffffffu, bad)) L = CUDART_NAN_F;
     for (int i = 0; i < n; ++i) {
-        const size_t at = (size_t)i * P.n_rows + R;
+        const size_t at = part(i);
         const float2 ml = P.part_ml[at];
+        if (!(ml.x > -CUDART_INF_F)) continue;      // a part without keys has no sums either
         const float w = exp2_approx(ml.x - base);
         L = __fmaf_rn(w, ml.y, L);
         if (mine) {
@@ -311,7 +322,8 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
         P.pks[i] = st[0][i]; P.pvs[i] = st[1][i]; P.tks[i] = st[2][i]; P.tvs[i] = st[3][i]; P.qs[i] = st[4][i]; P.os[i] = st[5][i];
     }
     const int per = a->group * a->n_q;
-    P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
+    if (shared_tc_supported(P, a->dtype)) shared_tc_plan(P);
+    else P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
     P.tail_parts = simt_splits(per, a->n_prompts * a->n_branches * a->n_kv, a->tail_len, a->vdim);
     return HIRA_OK;
 }
@@ -322,7 +334,8 @@ static size_t shared_parts_bytes(const SharedAttn& P) {
 template <typename T>
 static int run_shared(const SharedAttn& P, cudaStream_t s) {
     int rc = HIRA_OK;
-    if (P.prefix_parts > 0) rc = launch_simt_rows<T, false>(P, s);
+    if (P.shares > 0) rc = shared_tc_launch(P, s);
+    else if (P.prefix_parts > 0) rc = launch_simt_rows<T, false>(P, s);
     if (rc == HIRA_OK && P.tail_parts > 0) rc = launch_simt_rows<T, true>(P, s);
     if (rc != HIRA_OK) return rc;
     shared_merge_kernel<T><<<(unsigned)((P.n_rows + SA_MERGE_WARPS - 1) / SA_MERGE_WARPS), 32 * SA_MERGE_WARPS, 0, s>>>(P);

@@ -51,10 +51,24 @@ __device__ __forceinline__ long long shared_row_offset(const SharedAttn& P, int 
     const int heads = P.n_kv * P.group, t = R % P.n_q, bh = R / P.n_q;
     return (long long)(bh / heads) * s[0] + (long long)(bh % heads) * s[1] + (long long)t * s[2];
 }
+// the run of tiles that an item begins in (run s is tiles s * total / shares .. (s + 1) * total / shares), and its partials
+__device__ __forceinline__ int shared_share_of(const SharedAttn& P, long long tile) {
+    const long long total = (long long)P.n_prompts * P.n_kv * P.item_tiles;
+    return (int)(((tile + 1) * P.shares - 1) / total);
+}
+__device__ __forceinline__ int shared_first_share(const SharedAttn& P, int item) { return shared_share_of(P, (long long)item * P.item_tiles); }
+__device__ __forceinline__ int shared_item_parts(const SharedAttn& P, int item) {
+    if (P.shares == 0) return P.prefix_parts;
+    return (shared_share_of(P, (long long)(item + 1) * P.item_tiles - 1) - shared_first_share(P, item) + 1) * P.parts_per_share;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+bool shared_tc_supported(const SharedAttn& P, int dtype);
+void shared_tc_plan(SharedAttn& P);
+int shared_tc_launch(const SharedAttn& P, cudaStream_t s);
 
 }  // namespace hira

@@ -1,0 +1,531 @@
+// The prefix of hira_shared_attn on the tensor cores (bf16, rows of up to 128).
+//
+// A block takes the query rows of one (prompt, kv head) -- 128, or 256 where there are more -- through a run of key
+// tiles of 128.  One warp streams the tiles in by TMA, one thread issues the products
+//   S = Q K^T  (tcgen05.mma, operands in shared memory, fp32 accumulator in TMEM)
+//   O += P V   (P = 2^(S - m) as bf16 in TMEM, where S was; V in shared memory as it lies in memory)
+// and two groups of four warps turn S into P, each thread one row: no exchange between threads for maximum and sum.
+// The two groups are two independent chains, so that one group's exponentials run under the other's products:
+//   256 rows: a group has 128 rows of its own, both see every tile;
+//   128 rows: the groups take the tiles alternately, and each leaves a partial of its own (two partials a block).
+// The reference maximum of a row moves only when a tile exceeds it by 2^8: until then O and the sum stay as they are
+// (weights up to 256 lose nothing in floating point), and O in TMEM is rescaled in rare tiles instead of each.
+//
+// The tiles of all items are dealt out in equal runs, one to each SM, whatever the items' number: a run may end
+// inside an item and go on in the next one.  Every wait is bounded; a block whose wait ran out leaves NaN.
+#include "shared_attn.cuh"
+#include "tc_common.cuh"
+
+#include <cuda.h>
+#include <math_constants.h>
+
+namespace hira {
+
+constexpr int ST_KEYS = 128;                 // keys a tile
+constexpr int ST_ROWS = 128;                 // query rows of a group
+constexpr int ST_WG = 128;                   // threads of a softmax group
+constexpr int ST_THREADS = 3 * ST_WG;        // the third group: the TMA warp, the MMA warp, two that idle
+constexpr int ST_MAX_STAGES = 12;
+constexpr int ST_SMEM = 227 * 1024;
+// Registers: 384 threads start with 168 each; the softmax groups hold a row of 128 scores and take what the others leave
+// (2 x 208 + 88 = 3 x 168).
+constexpr float ST_SLACK = 8.0f;             // log2 of how far a row may rise above its reference maximum
+
+template <int HD>
+struct StLayout {
+    static constexpr int BOXES = HD / 64;                       // 128-byte swizzled boxes of 64 channels
+    static constexpr int BOX_BYTES = ST_KEYS * 128;
+    static constexpr int TILE_BYTES = BOXES * BOX_BYTES;        // 128 rows of keys, values or queries
+};
+template <int HD, int NT>
+constexpr int st_stages() {
+    const int n = (ST_SMEM - 2048 - NT * StLayout<HD>::TILE_BYTES) / StLayout<HD>::TILE_BYTES;
+    return n > ST_MAX_STAGES ? ST_MAX_STAGES : n;
+}
+
+__device__ __forceinline__ void st_tma_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void st_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void st_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Values as the B operand: channels one behind another in memory (N), a key a row (K).  128-byte swizzle; 64 channels a
+// box, the next 64 a box further; 8 keys are 1024 bytes.
+template <int HD>
+__device__ __forceinline__ uint64_t st_desc_v(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3ffff) >> 4);
+    d |= (uint64_t)(StLayout<HD>::BOX_BYTES >> 4) << 16;     // to the next 64 channels
+    d |= (uint64_t)(1024 >> 4) << 32;                        // to the next 8 keys
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// fp32 accumulator, bf16 operands, 128 x n
+constexpr uint32_t st_idesc(int n, bool b_transposed) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_transposed ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(ST_ROWS >> 4) << 24);
+}
+__device__ __forceinline__ void st_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+// the registers of a st_ld32 are valid behind this; they are its operands, so that no use moves ahead of it
+__device__ __forceinline__ void st_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
+__device__ __forceinline__ void st_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+           "r"(taddr) : "memory");
+}
+// load and wait
+__device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// One segment: a block's run of tiles inside one item.  All roles walk the same segments.
+struct StSegment {
+    int item, first, n;       // n tiles from `first` on that hold keys (0: none)
+    int part;                 // index among the item's runs
+    int len;                  // keys of the prompt
+};
+struct StWalk {
+    long long at, end;
+    __device__ __forceinline__ StWalk(const SharedAttn& P, int share) {
+        const long long total = (long long)P.n_prompts * P.n_kv * P.item_tiles;
+        at = share * total / P.shares;
+        end = (share + 1) * total / P.shares;
+    }
+    __device__ __forceinline__ bool next(const SharedAttn& P, int share, StSegment& s) {
+        if (at >= end) return false;
+        s.item = (int)(at / P.item_tiles);
+        const long long base = (long long)s.item * P.item_tiles;
+        s.first = (int)(at - base);
+        const int stop = (int)min(end - base, (long long)P.item_tiles);
+        s.len = shared_prefix_len(P, s.item / P.n_kv);
+        s.n = max(0, min(stop, (s.len + ST_KEYS - 1) / ST_KEYS) - s.first);
+        s.part = share - shared_first_share(P, s.item);
+        at = base + stop;
+        return true;
+    }
+};
+
+// where keys tile j and values tile j of a segment of n tiles lie in the order of their loads: K0 K1 V0 K2 V1 ... V(n-1),
+// which is the order of their products
+__device__ __forceinline__ int st_pos_k(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int st_pos_v(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(ST_THREADS, 1)
+shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int row_blocks) {
+    using Lay = StLayout<HD>;
+    constexpr int STAGES = st_stages<HD, NT>();
+    extern __shared__ unsigned char st_smem_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(st_smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t s_q = smem_u32(sm), s_ring = s_q + NT * Lay::TILE_BYTES;
+    __shared__ __align__(8) unsigned long long s_bar[2 * ST_MAX_STAGES + 9];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_fail;
+    const uint32_t bars = smem_u32(s_bar);
+    const uint32_t bar_full = bars, bar_empty = bars + 8 * ST_MAX_STAGES;      // [STAGES] tile landed, tile used up
+    const uint32_t bar_q = bars + 16 * ST_MAX_STAGES;                            // the segment's queries are in place
+    const uint32_t bar_done = bar_q + 8;                                         // all products of the segment are complete
+    const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48;   // [2] S written, P written, O complete
+    const uint32_t bar_exit = bar_q + 64;
+
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int rb = blockIdx.x % row_blocks, share = blockIdx.x / row_blocks;
+    if (tid == 0) {
+        s_fail = 0;
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(bar_full + 8 * i, 1);
+            mbar_init(bar_empty + 8 * i, 1);
+        }
+        mbar_init(bar_q, 2 * ST_WG);
+        mbar_init(bar_done, 1);
+        mbar_init(bar_exit, 1);
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(bar_s + 8 * w, 1);
+            mbar_init(bar_p + 8 * w, ST_WG);
+            mbar_init(bar_o + 8 * w, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
+    volatile int* fail = &s_fail;
+    const uint32_t tm_s = tmem, tm_o = tmem + 2 * ST_KEYS;      // S and P of the chains, then O of the chains
+    grid_trigger();      // what follows on the stream reads nothing of this before it waits
+
+    StWalk walk(P, share);
+    StSegment seg;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // ---- tiles in, in the order of their products ---------------------------------------------------
+            if ((tid & 31) == 0) {
+                uint32_t pos = 0;
+                auto load = [&](const CUtensorMap* map, int tile, const StSegment& s) {
+                    const uint32_t stage = pos % STAGES, round = pos / STAGES;
+                    if (round > 0 && (*fail || !mbar_wait(bar_empty + 8 * stage, (round - 1) & 1))) return false;
+                    const uint32_t bar = bar_full + 8 * stage, dst = s_ring + stage * Lay::TILE_BYTES;
+                    mbar_expect_tx(bar, Lay::TILE_BYTES);
+    #pragma unroll
+                    for (int b = 0; b < Lay::BOXES; ++b)
+                        st_tma_load(dst + b * Lay::BOX_BYTES, map, b * 64, tile * ST_KEYS, s.item % P.n_kv, s.item / P.n_kv, bar);
+                    ++pos;
+                    return true;
+                };
+                bool ok = true;
+                while (ok && walk.next(P, share, seg)) {
+                    if (seg.n == 0) continue;
+                    ok = load(&map_k, seg.first, seg);
+                    for (int j = 0; ok && j < seg.n; ++j) {
+                        if (j + 1 < seg.n) ok = load(&map_k, seg.first + j + 1, seg);
+                        ok = ok && load(&map_v, seg.first + j, seg);
+                    }
+                }
+                if (!ok) *fail = 1;
+                // no copy may be in flight when the shared memory is given back: the products waited for each, unless one failed
+                if (*fail)
+                    for (uint32_t p = pos > STAGES ? pos - STAGES : 0; p < pos; ++p) mbar_wait(bar_full + 8 * (p % STAGES), (p / STAGES) & 1);
+            }
+        } else if (warp == 9) {
+            // ---- products --------------------------------------------------------------------------------------
+            if ((tid & 31) == 0) {
+                uint32_t base = 0, segs = 0, n_p[2] = {0, 0};      // loads, segments and P tiles so far
+                bool ok = true;
+                while (ok && walk.next(P, share, seg)) {
+                    const int n = seg.n;
+                    if (n == 0) continue;
+                    ok = mbar_wait(bar_q, segs & 1) && !*fail;
+                    const int count[2] = {NT == 2 ? n : (n + 1) / 2, NT == 2 ? n : n / 2};
+                    auto tile_of = [&](int w, int i) { return NT == 2 ? i : 2 * i + w; };
+                    auto qk = [&](int w, int i) {
+                        const uint32_t pos = base + st_pos_k(tile_of(w, i)), stage = pos % STAGES;
+                        if (!mbar_wait(bar_full + 8 * stage, (pos / STAGES) & 1)) return false;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t a0 = s_q + (NT == 2 ? w : 0) * Lay::TILE_BYTES, b0 = s_ring + stage * Lay::TILE_BYTES;
+    #pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint32_t off = (k >> 2) * Lay::BOX_BYTES + (k & 3) * 32;
+                            st_mma_ss(tm_s + w * ST_KEYS, umma_desc(a0 + off), umma_desc(b0 + off), st_idesc(ST_KEYS, false), k > 0);
+                        }
+                        umma_commit(bar_s + 8 * w);
+                        if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
+                        return true;
+                    };
+                    auto pv = [&](int w, int i) {
+                        const uint32_t pos = base + st_pos_v(tile_of(w, i), n), stage = pos % STAGES;
+                        if (!mbar_wait(bar_p + 8 * w, n_p[w] & 1) || *fail || !mbar_wait(bar_full + 8 * stage, (pos / STAGES) & 1)) return false;
+                        ++n_p[w];
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t b0 = s_ring + stage * Lay::TILE_BYTES;
+    #pragma unroll
+                        for (int k = 0; k < ST_KEYS / 16; ++k)
+                            st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
+                        if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
+                        if (i == count[w] - 1) umma_commit(bar_o + 8 * w);
+                        return true;
+                    };
+                    for (int w = 0; w < 2; ++w)
+                        if (count[w] > 0) ok = ok && qk(w, 0);
+                    for (int i = 0; ok && i < count[0]; ++i)
+                        for (int w = 0; w < 2; ++w) {
+                            if (i < count[w]) ok = ok && pv(w, i);
+                            // behind that product in the pipe, so that it may write where P was
+                            if (i + 1 < count[w]) ok = ok && qk(w, i + 1);
+                        }
+                    if (ok) umma_commit(bar_done);
+                    base += 2 * n;
+                    ++segs;
+                }
+                // nothing of the tensor cores may be under way when shared memory and TMEM are given back
+                if (!ok) {
+                    *fail = 1;
+                    umma_commit(bar_exit);
+                    mbar_wait(bar_exit, 0);
+                } else if (segs > 0) {
+                    mbar_wait(bar_done, (segs - 1) & 1);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ---- softmax: thread t of group w has row t of its chain (TMEM lane t) -----------------------------
+        const int w = warp >> 2, t = tid & (ST_WG - 1);
+        const int per = P.group * P.n_q, n_rows = P.n_branches * per;
+        const int row0 = (rb * NT + (NT == 2 ? w : 0)) * ST_ROWS;       // first row of the chain
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t my_s = tm_s + w * ST_KEYS + lanes, my_o = tm_o + w * HD + lanes;
+        const bool warp_used = row0 + (warp & 3) * 32 < n_rows;          // rows behind the last: nothing to compute
+        const int row = row0 + t;
+        const float scale = fabsf(P.scale_log2);
+        const uint32_t flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;     // a negative scale turns the queries round
+        uint32_t base = 0, segs = 0, n_s = 0, n_o = 0;
+        bool ok = true;
+        // the same answer for the whole warp: what follows is done by warps
+        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity) && !*fail) != 0; };
+        while (walk.next(P, share, seg)) {
+            const int prompt = seg.item / P.n_kv, h = seg.item % P.n_kv, n = seg.n;
+            const int count = NT == 2 ? n : (n + 1 - w) / 2;
+            float m = -CUDART_INF_F, l = 0.f;
+            if (n > 0 && ok) {
+                // queries into the swizzled layout of the products; the products of the segment before have read theirs
+                if (segs > 0) ok = wait(bar_done, (segs - 1) & 1);
+                const int first = NT == 2 ? t : tid, step = NT == 2 ? ST_WG : 2 * ST_WG;
+                for (int i = first; i < ST_ROWS * (HD / 8); i += step) {
+                    const int r = i / (HD / 8), c = i % (HD / 8);
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (row0 + r < n_rows && c * 8 < P.dim) {
+                        x = *(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) +
+                                                             shared_row_offset(P, shared_row(P, prompt, h, row0 + r), P.qs)) + c);
+                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                    }
+                    *reinterpret_cast<uint4*>(sm + (NT == 2 ? w : 0) * Lay::TILE_BYTES + (c >> 3) * Lay::BOX_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bar_q);
+                for (int i = 0; i < count && ok; ++i) {
+                    const int j = NT == 2 ? i : 2 * i + w, k0 = (seg.first + j) * ST_KEYS;
+                    ok = wait(bar_s + 8 * w, n_s & 1);
+                    if (!ok) break;
+                    ++n_s;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const int valid = min(seg.len - k0, ST_KEYS);
+                    if (warp_used) {
+                        uint32_t s[4][32];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) st_ld32(my_s + q * 32, s[q]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) st_ld_wait(s[q]);
+                        if (valid < ST_KEYS) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (q * 32 + e >= valid) s[q][e] = 0xff800000u;      // -inf
+                        }
+                        float mx[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            mx[q] = __uint_as_float(s[q][0]);
+#pragma unroll
+                            for (int e = 1; e < 31; e += 2) mx[q] = max3f(mx[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
+                            mx[q] = fmaxf(mx[q], __uint_as_float(s[q][31]));
+                        }
+                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                        const bool rise = top > m + ST_SLACK;      // from -inf on: always, unless the tile is -inf too
+                        if (__any_sync(0xffffffffu, rise)) {
+                            const float to = rise ? top : m;
+                            const float f = rise ? exp2_approx(m - top) : 1.f;      // 0 from -inf on
+                            m = to;
+                            l *= f;
+                            if (i > 0) {
+                                // the product before last is complete: S of this tile was committed behind it
+                                uint32_t o[16];
+#pragma unroll 1
+                                for (int c = 0; c < HD; c += 16) {
+                                    st_ld16(my_o + c, o);
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                    st_st16(my_o + c, o);
+                                }
+                            }
+                        }
+                        const float nm = m > -CUDART_INF_F ? -m : 0.f;
+                        const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(nm, nm);
+                        float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t p[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float2 y = __ffma2_rn(make_float2(__uint_as_float(s[q][2 * e]), __uint_as_float(s[q][2 * e + 1])), sc2, nm2);
+                                const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                                sum2 = __fadd2_rn(sum2, z);
+                                p[e] = pack_bf16(z.x, z.y);
+                            }
+                            st_st16(my_s + q * 16, p);
+                        }
+                        l += sum2.x + sum2.y;
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                    if (k0 + valid < min(P.prefix_len, k0 + ST_KEYS)) {
+                        // rows of the value tile behind the prompt's keys, whatever they hold: 0, as what TMA fills in
+                        // behind the array (0 x NaN would be NaN)
+                        const uint32_t pos = base + st_pos_v(j, n), stage = pos % STAGES;
+                        ok = wait(bar_full + 8 * stage, (pos / STAGES) & 1);
+                        unsigned char* v = sm + (NT + stage) * Lay::TILE_BYTES;
+                        for (int q = valid * 8 + t; q < ST_KEYS * 8; q += ST_WG)
+#pragma unroll
+                            for (int b = 0; b < Lay::BOXES; ++b) *reinterpret_cast<uint4*>(v + b * Lay::BOX_BYTES + q * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    mbar_arrive(bar_p + 8 * w);
+                }
+                if (count > 0 && ok) {
+                    ok = wait(bar_o + 8 * w, n_o & 1);
+                    ++n_o;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
+                base += 2 * n;
+                ++segs;
+            }
+            if (!ok) *fail = 1;
+            const int part = NT == 2 ? seg.part : 2 * seg.part + w;
+            if (warp_used) {
+                const bool mine = row < n_rows;
+                const size_t at = (size_t)part * P.n_rows + (mine ? shared_row(P, prompt, h, row) : 0);
+                if (mine) P.part_ml[at] = ok ? make_float2(m, l) : make_float2(CUDART_NAN_F, CUDART_NAN_F);
+                if (count > 0 && ok) {
+                    uint32_t o[16];
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        st_ld16(my_o + c, o);
+                        if (mine)
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4)
+                                if (c + e < P.vdim)
+                                    *reinterpret_cast<float4*>(P.part_o + at * P.vdim + c + e) =
+                                        make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 9) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+typedef CUresult (*StEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static StEncodeFn st_encode_fn() {
+    static const StEncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<StEncodeFn>(p) : nullptr;
+    }();
+    return fn;
+}
+// (prompts, heads, rows, width) bf16 with the given strides; boxes of 64 channels x 128 rows
+static bool st_make_map(CUtensorMap* map, const void* base, int width, const SharedAttn& P, const long long (&s)[3]) {
+    const StEncodeFn fn = st_encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)P.prefix_len, (cuuint64_t)P.n_kv, (cuuint64_t)P.n_prompts};
+    // a stride along a dimension of one is not used, but has to be one that the encoder takes
+    const cuuint64_t row = (cuuint64_t)(P.prefix_len > 1 ? s[2] : width) * 2;
+    const cuuint64_t strides[3] = {row, P.n_kv > 1 ? (cuuint64_t)s[1] * 2 : row, P.n_prompts > 1 ? (cuuint64_t)s[0] * 2 : row};
+    const cuuint32_t box[4] = {64, (cuuint32_t)ST_KEYS, 1, 1}, one[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Strides that a tensor map takes: forward, and below 2^40 bytes.
+bool shared_tc_supported(const SharedAttn& P, int dtype) {
+    if (dtype != HIRA_BF16 || P.prefix_len == 0 || P.dim > 128 || P.vdim > 128 || (P.dim > 64) != (P.vdim > 64)) return false;
+    const int n[3] = {P.n_prompts, P.n_kv, P.prefix_len};
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (P.pks[i] < 1 || P.pvs[i] < 1 || P.pks[i] >= (1ll << 39) || P.pvs[i] >= (1ll << 39))) return false;
+    return true;
+}
+
+void shared_tc_plan(SharedAttn& P) {
+    const int rows = P.n_branches * P.group * P.n_q, nt = rows > ST_ROWS ? 2 : 1, row_blocks = (rows + nt * ST_ROWS - 1) / (nt * ST_ROWS);
+    P.item_tiles = (P.prefix_len + ST_KEYS - 1) / ST_KEYS;
+    const long long total = (long long)P.n_prompts * P.n_kv * P.item_tiles;
+    long long shares = SM_COUNT / row_blocks;
+    if (shares > total) shares = total;
+    P.shares = shares < 1 ? 1 : (int)shares;
+    P.parts_per_share = nt == 2 ? 1 : 2;
+    // an item of T tiles spans at most this many runs of total / shares tiles
+    const long long run = total / P.shares;
+    long long runs = (P.item_tiles + run - 1) / run + 1;
+    if (runs > P.shares) runs = P.shares;
+    P.prefix_parts = (int)runs * P.parts_per_share;
+}
+
+template <int HD, int NT>
+static int st_launch(const SharedAttn& P, int row_blocks, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
+    auto kern = shared_tc_kernel<HD, NT>;
+    const size_t smem = (size_t)(NT + st_stages<HD, NT>()) * StLayout<HD>::TILE_BYTES + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+        set_error("hira_shared_attn: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));
+        return HIRA_ERR_CUDA;
+    }
+    kern<<<(unsigned)(P.shares * row_blocks), ST_THREADS, smem, s>>>(P, mk, mv, row_blocks);
+    HIRA_CHECK_LAUNCH("hira_shared_attn launch");
+    return HIRA_OK;
+}
+
+int shared_tc_launch(const SharedAttn& P, cudaStream_t s) {
+    CUtensorMap mk, mv;
+    if (!st_make_map(&mk, P.pk, P.dim, P, P.pks) || !st_make_map(&mv, P.pv, P.vdim, P, P.pvs)) {
+        set_error("hira_shared_attn: cuTensorMapEncodeTiled failed or is unavailable");
+        return HIRA_ERR_CUDA;
+    }
+    const int rows = P.n_branches * P.group * P.n_q, nt = rows > ST_ROWS ? 2 : 1, row_blocks = (rows + nt * ST_ROWS - 1) / (nt * ST_ROWS);
+    const bool wide = P.dim > 64;
+    if (nt == 1) return wide ? st_launch<128, 1>(P, row_blocks, mk, mv, s) : st_launch<64, 1>(P, row_blocks, mk, mv, s);
+    return wide ? st_launch<128, 2>(P, row_blocks, mk, mv, s) : st_launch<64, 2>(P, row_blocks, mk, mv, s);
+}
+
+}  // namespace hira

@@ -234,7 +234,7 @@ def test_rows_gathered_into_other_memory_and_in_place(picks, rows, dim, dtype):
     assert torch.equal(src, want)
 
 
-@pytest.mark.parametrize("n", [2, 17, 100, 769, 2048])
+@pytest.mark.parametrize("n", [2, 8, 12, 17, 32, 100, 769, 2048])
 def test_many_sequences_permuted_in_place(n):
     gen = torch.Generator().manual_seed(n)
     src = torch.randn((n, 2, 9, 8), generator=gen).cuda()
