@@ -233,3 +233,12 @@ def dtype_code(dt: torch.dtype) -> int:
 
 def current_stream(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(index: int, call, *args):
+    """`call(*args, stream)` with the device `index` current and its current stream; the device is switched only where
+    it is not current already."""
+    if torch.cuda.current_device() == index:
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))

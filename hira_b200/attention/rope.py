@@ -16,6 +16,19 @@ from .. import index_state as S
 from .shared_attention import refuse_grad
 
 _TYPES = (torch.float32, torch.bfloat16)
+_plans = {}
+
+
+def _layout(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _check_apart(o: torch.Tensor, x: torch.Tensor, other: torch.Tensor, name: str):
+    if o.data_ptr() == x.data_ptr() and o.stride() == x.stride():
+        return
+    own = o.untyped_storage().data_ptr()
+    if own == x.untyped_storage().data_ptr() or own == other.untyped_storage().data_ptr():
+        raise ValueError(f"{name} must be its own input or memory apart from both inputs")
 
 
 def _table(t: torch.Tensor, b: int, n: int, name: str) -> torch.Tensor:
@@ -41,7 +54,20 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     fp32 or bf16; D a multiple of 8 up to 256.  Any strides with contiguous, 16-byte aligned rows (a projection's
     transposed view as it is); others are copied.  `out_q` / `out_k`: where to write, with such rows: the input itself,
     or memory apart from both inputs (part of a cache, say).  No backward pass."""
-    refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
+    if torch.is_grad_enabled():
+        refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
+    # calls of a layout that has been checked before go straight to the library
+    layout = (_layout(query), _layout(key), _layout(cos), _layout(sin), _layout(q_weight), _layout(k_weight), _layout(out_q), _layout(out_k),
+              eps, interleaved)
+    plan = _plans.get(layout)
+    if plan is not None:
+        if out_q is not None:
+            _check_apart(out_q, query, key, "out_q")
+        if out_k is not None:
+            _check_apart(out_k, key, query, "out_k")
+        done = plan(query, key, cos, sin, q_weight, k_weight, out_q, out_k)
+        if done is not None:
+            return done
     if query.ndim != 4 or key.ndim != 4:
         raise ValueError(f"query and key must be (B, H, L, D), got {tuple(query.shape)} and {tuple(key.shape)}")
     b, hq, n, d = query.shape
@@ -58,6 +84,7 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and (w.shape != (d,) or w.dtype != query.dtype):
             raise ValueError(f"{name} must be ({d},) {query.dtype}, got {tuple(w.shape)} {w.dtype}")
+    given = cos, sin
     cos, sin = _table(cos, b, n, "cos"), _table(sin, b, n, "sin")
     if cos.shape[2] != sin.shape[2] or cos.dtype != sin.dtype:
         raise ValueError(f"cos {tuple(cos.shape)} {cos.dtype} and sin {tuple(sin.shape)} {sin.dtype} differ")
@@ -69,18 +96,17 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
             continue
         if o.shape != x.shape or o.dtype != x.dtype or not S.writable_rows(o):
             raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype} with aligned contiguous rows")
-        if not (o.data_ptr() == x.data_ptr() and o.stride() == x.stride()):
-            own = o.untyped_storage().data_ptr()
-            if own in (query.untyped_storage().data_ptr(), key.untyped_storage().data_ptr()):
-                raise ValueError(f"{name} must be its own input or memory apart from both inputs")
+        _check_apart(o, x, key if x is query else query, name)
     if not query.is_cuda:
         raise ValueError("hira_qk_norm_rope needs CUDA tensors (there is no CPU fallback)")
-    if out_q is None:
-        out_q = torch.empty((b, hq, n, d), dtype=query.dtype, device=query.device)
-    if out_k is None:
-        out_k = torch.empty(key.shape, dtype=key.dtype, device=key.device)
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    return S.qk_norm_rope(S.with_rows(query), S.with_rows(key), cos, sin, q_weight, k_weight, eps, interleaved, out_q, out_k)
+    args = (S.with_rows(query), S.with_rows(key), cos, sin, *(None if w is None else S.aligned(w.contiguous()) for w in (q_weight, k_weight)))
+    as_given = all(a is b for a, b in zip(args, (query, key, *given, q_weight, k_weight)))
+    oq = torch.empty((b, hq, n, d), dtype=query.dtype, device=query.device) if out_q is None else out_q
+    ok = torch.empty(tuple(key.shape), dtype=key.dtype, device=key.device) if out_k is None else out_k
+    plan = S.RopePlan(*args[:4], eps, interleaved, oq, ok)
+    if as_given:
+        S.remember(_plans, layout, plan)
+    return plan(*args, oq, ok)
 
 
 def hira_attention_forward(module, hidden_states: torch.Tensor, position_embeddings, attention_mask: Optional[torch.Tensor] = None,

@@ -15,6 +15,19 @@ import torch
 from .. import index_state as S
 
 _TYPES = (torch.float32, torch.bfloat16)
+_plans = {}
+
+
+def _layout(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _tail_layout(t: Optional[torch.Tensor]):
+    """All but the length, which grows from call to call."""
+    if t is None or t.ndim != 4:
+        return t if t is None else ()
+    b, h, n, d = t.shape
+    return b, h, d, min(n, 2), t.stride(), t.dtype, t.get_device()      # the strides of one row need not fit two
 
 
 def refuse_grad(what: str, *tensors):
@@ -52,7 +65,20 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     fp32 or bf16, all of one type; D and V multiples of 8 up to 256.  fp32 is computed in fp32; bf16 with fp32
     sums and statistics.  Rows have to be contiguous and 16-byte aligned: what is not is copied first.  `out` has
     to be so.  No backward pass.  A key hidden from one query token but not from another has to be finite."""
-    refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
+    if torch.is_grad_enabled():
+        refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
+    # calls of a layout that has been checked before go straight to the library
+    layout = None
+    if out is None and (tail_keys is None or tail_values is not None and tail_keys.shape[:-1] == tail_values.shape[:-1]) \
+            and (prefix_lens is None or torch.is_tensor(prefix_lens) and prefix_lens.is_cuda) \
+            and (tail_lens is None or torch.is_tensor(tail_lens) and tail_lens.is_cuda):
+        layout = (_layout(query), _layout(prefix_keys), _layout(prefix_values), _tail_layout(tail_keys), _tail_layout(tail_values),
+                  _layout(prefix_lens), _layout(tail_lens), scaling)
+        plan = _plans.get(layout)
+        if plan is not None:
+            done = plan(query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
+            if done is not None:
+                return done
     if (tail_keys is None) != (tail_values is None):
         raise ValueError("tail_keys and tail_values are given together or not at all")
     named = [("query", query), ("prefix_keys", prefix_keys), ("prefix_values", prefix_values)]
@@ -83,6 +109,7 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     for name, w in (("D", d), ("V", v)):
         if w % 8 or not 8 <= w <= 256:
             raise ValueError(f"{name}={w} must be a multiple of 8 in 8..256")
+    given = (query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
     prefix_lens = _lengths(prefix_lens, p, n, query.device, "prefix_lens")
     if tail_keys is not None:
         tail_lens = _lengths(tail_lens, b, tail_keys.shape[2], query.device, "tail_lens")
@@ -94,10 +121,11 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
         raise ValueError(f"out must be ({b}, {hq}, {n_q}, {v}) {query.dtype} on {query.device} with aligned contiguous rows")
     if out.numel() == 0:
         return out
-    if tail_keys is not None:
-        tail_keys, tail_values = S.with_rows(tail_keys), S.with_rows(tail_values)
-    return S.shared_attn(S.with_rows(query), S.with_rows(prefix_keys), S.with_rows(prefix_values), tail_keys, tail_values,
-                         prefix_lens, tail_lens, d ** -0.5 if scaling is None else scaling, out)
+    args = tuple(None if t is None else S.with_rows(t) for t in given[:5]) + (prefix_lens, tail_lens)
+    plan = S.SharedAttnPlan(*args[:5], d ** -0.5 if scaling is None else scaling, out)
+    if layout is not None and all(a is b for a, b in zip(args, given)):
+        S.remember(_plans, layout, plan)
+    return plan(*args, out)
 
 
 class SharedPrompt:

@@ -14,7 +14,7 @@ namespace hira {
 
 constexpr int GA_THREADS = 256;
 constexpr int GA_ITEMS = 24;              // arrays a launch takes
-constexpr int GA_STAGE_BYTES = 48 * 1024; // staged strips of a block, up to 768 sequences; 64 bytes a sequence beyond
+constexpr int GA_STAGE_BYTES = 48 * 1024; // staged strips of a block; 64 bytes a sequence where that is more
 constexpr int GA_MAX_SEQ = 2048;
 
 struct GatherItems {
@@ -76,63 +76,123 @@ gather_kernel(const __grid_constant__ GatherItems items, const long long* __rest
     }
 }
 
-// in place: `cols` columns of every sequence that changes
-template <typename W>
+// In place, `cols` columns of the m sequences that change.
+//   staged: all read before the first is written;
+//   direct (no changed sequence is another's source): copied right away, a source that follows itself read once.
+template <typename W, bool STAGED>
 __device__ __forceinline__ void permute_strip(const hira_gather_item_t& g, long long strip, const int* s_dst, const int* s_src, int moved,
                                               int cols, W* s_stage) {
-    const long long strips = (g.bytes / (long long)sizeof(W) + cols - 1) / cols;
-    const long long seg = strip / strips, col0 = (strip - seg * strips) * cols, used = g.bytes / sizeof(W);
+    const long long used = g.bytes / sizeof(W), strips = (used + cols - 1) / cols;
+    const long long seg = strip / strips, col0 = (strip - seg * strips) * cols;
     char* base = reinterpret_cast<char*>(g.dst) + seg * g.dst_seg_stride;
-    const int n = moved * cols;
+    if (STAGED) {
+        const int n = moved * cols;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += GA_THREADS) {
-        const int k = i / cols;
-        const long long col = col0 + (i - k * cols);
-        if (col < used) s_stage[i] = reinterpret_cast<const W*>(base + s_src[k] * g.dst_seq_stride)[col];
-    }
-    __syncthreads();
+        for (int i = threadIdx.x; i < n; i += GA_THREADS) {
+            const int k = i / cols;
+            const long long col = col0 + (i - k * cols);
+            if (col < used) s_stage[i] = reinterpret_cast<const W*>(base + s_src[k] * g.dst_seq_stride)[col];
+        }
+        __syncthreads();
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += GA_THREADS) {
-        const int k = i / cols;
-        const long long col = col0 + (i - k * cols);
-        if (col < used) reinterpret_cast<W*>(base + s_dst[k] * g.dst_seq_stride)[col] = s_stage[i];
+        for (int i = threadIdx.x; i < n; i += GA_THREADS) {
+            const int k = i / cols;
+            const long long col = col0 + (i - k * cols);
+            if (col < used) reinterpret_cast<W*>(base + s_dst[k] * g.dst_seq_stride)[col] = s_stage[i];
+        }
+        __syncthreads();
+    } else {
+        W v[GA_COLS];
+        int have = -1;
+        for (int k = 0; k < moved; ++k) {
+            if (s_src[k] != have) {
+                have = s_src[k];
+#pragma unroll
+                for (int c = 0; c < GA_COLS; ++c) {
+                    const long long col = col0 + threadIdx.x + c * GA_THREADS;
+                    if (col < used) v[c] = reinterpret_cast<const W*>(base + have * g.dst_seq_stride)[col];
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < GA_COLS; ++c) {
+                const long long col = col0 + threadIdx.x + c * GA_THREADS;
+                if (col < used) reinterpret_cast<W*>(base + s_dst[k] * g.dst_seq_stride)[col] = v[c];
+            }
+        }
     }
-    __syncthreads();
 }
 
+// The strips' width follows from how many sequences change, which only the device knows; so the strips are counted here.
 __global__ void __launch_bounds__(GA_THREADS)
-permute_kernel(const __grid_constant__ GatherItems items, const long long* __restrict__ index, int n_seq, int cols, int32_t* status) {
+permute_kernel(const __grid_constant__ GatherItems items, const long long* __restrict__ index, int n_seq, int stage_bytes, int32_t* status) {
     extern __shared__ __align__(16) unsigned char ga_stage[];
     __shared__ int s_dst[GA_MAX_SEQ], s_src[GA_MAX_SEQ];
-    __shared__ int s_n;
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < n_seq; j += GA_THREADS) {
+    __shared__ unsigned char s_moves[GA_MAX_SEQ];
+    __shared__ long long s_first[GA_ITEMS + 1];
+    __shared__ int s_n, s_hazard;
+    const int tid = threadIdx.x;
+    if (tid == 0) s_n = s_hazard = 0;
+    for (int j = tid; j < n_seq; j += GA_THREADS) {
         const long long i = index[j];
         const bool ok = i >= 0 && i < n_seq;
         if (!ok && status && blockIdx.x == 0) atomicOr(status, HIRA_STATUS_BAD_INDEX);      // left as it was
-        if (ok && i != j) {
-            const int k = atomicAdd(&s_n, 1);       // the order of the list changes nothing that is stored
-            s_dst[k] = j;
-            s_src[k] = (int)i;
+        s_src[j] = ok ? (int)i : j;
+        s_moves[j] = ok && i != j;
+    }
+    __syncthreads();
+    // the list of those that change, packed by the first warp in their order
+    for (int j = tid; j < n_seq; j += GA_THREADS)
+        if (s_moves[j] && s_moves[s_src[j]]) s_hazard = 1;
+    __syncthreads();
+    if (tid < 32) {
+        int n = 0;
+        for (int j0 = 0; j0 < n_seq; j0 += 32) {
+            const int j = j0 + tid, src = j < n_seq ? s_src[j] : 0;
+            const unsigned m = __ballot_sync(0xffffffffu, j < n_seq && s_moves[j]);
+            __syncwarp();
+            if (m >> tid & 1) {       // never ahead of what is still to be read: n + rank <= j
+                const int k = n + __popc(m & ((1u << tid) - 1));
+                s_dst[k] = j;
+                s_src[k] = src;
+            }
+            n += __popc(m);
+            __syncwarp();
         }
+        if (tid == 0) s_n = n;
     }
     __syncthreads();
     const int moved = s_n;
     if (moved == 0) return;
-    for (long long strip = blockIdx.x; strip < items.first[items.n]; strip += gridDim.x) {
-        int a = 0;
-        while (strip >= items.first[a + 1]) ++a;
-        if (items.wide[a]) permute_strip<uint4>(items.it[a], strip - items.first[a], s_dst, s_src, moved, cols, reinterpret_cast<uint4*>(ga_stage));
-        else permute_strip<uint32_t>(items.it[a], strip - items.first[a], s_dst, s_src, moved, cols, reinterpret_cast<uint32_t*>(ga_stage));
+    const bool staged = s_hazard != 0;
+    int cols = GA_THREADS * GA_COLS;
+    if (staged) {
+        cols = stage_bytes / 16 / moved;
+        if (cols > GA_THREADS) cols = cols / GA_THREADS * GA_THREADS;
     }
-}
-
-// columns of 16 bytes a block stages for each of n sequences
-static int permute_cols(int n_seq) {
-    int cols = GA_THREADS;
-    while (cols > 4 && (long long)cols * n_seq * 16 > GA_STAGE_BYTES) cols /= 2;
-    return cols;
+    if (tid == 0) {
+        long long n = 0;
+        for (int a = 0; a < items.n; ++a) {
+            s_first[a] = n;
+            const long long words = items.it[a].bytes / (items.wide[a] ? 16 : 4);
+            n += (words + cols - 1) / cols * items.it[a].n_seg;
+        }
+        s_first[items.n] = n;
+    }
+    __syncthreads();
+    for (long long strip = blockIdx.x; strip < s_first[items.n]; strip += gridDim.x) {
+        int a = 0;
+        while (strip >= s_first[a + 1]) ++a;
+        const long long at = strip - s_first[a];
+        uint4* s16 = reinterpret_cast<uint4*>(ga_stage);
+        uint32_t* s4 = reinterpret_cast<uint32_t*>(ga_stage);
+        if (items.wide[a]) {
+            if (staged) permute_strip<uint4, true>(items.it[a], at, s_dst, s_src, moved, cols, s16);
+            else permute_strip<uint4, false>(items.it[a], at, s_dst, s_src, moved, cols, s16);
+        } else {
+            if (staged) permute_strip<uint32_t, true>(items.it[a], at, s_dst, s_src, moved, cols, s4);
+            else permute_strip<uint32_t, false>(items.it[a], at, s_dst, s_src, moved, cols, s4);
+        }
+    }
 }
 
 }  // namespace hira
@@ -147,7 +207,6 @@ extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, con
                    "hira_gather: %d sequences picked from %d, 1..%d are served", n_dst, n_src, GA_MAX_SEQ);
     HIRA_CHECK_ARG(!in_place || n_src == n_dst, HIRA_ERR_SHAPE, "hira_gather: in place %d sequences cannot become %d", n_src, n_dst);
     GatherItems G = {};
-    const int cols = permute_cols(n_dst);
     for (int i = 0; i < n_items; ++i) {
         const hira_gather_item_t& g = items[i];
         HIRA_CHECK_ARG(g.n_seg >= 0 && g.bytes >= 0 && g.bytes_filled >= g.bytes, HIRA_ERR_SHAPE,
@@ -163,7 +222,7 @@ extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, con
         HIRA_CHECK_ARG((mix & 3) == 0, HIRA_ERR_ARG, "hira_gather: array %d is not made of 4-byte words", i);
         G.it[G.n] = g;
         G.wide[G.n] = (mix & 15) == 0;
-        const long long word = G.wide[G.n] ? 16 : 4, strip = in_place ? word * cols : word * GA_THREADS * GA_COLS;
+        const long long word = G.wide[G.n] ? 16 : 4, strip = word * GA_THREADS * GA_COLS;
         G.first[G.n + 1] = G.first[G.n] + (span + strip - 1) / strip * g.n_seg;
         ++G.n;
     }
@@ -172,16 +231,15 @@ extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, con
     const long long strips = G.first[G.n];
     const long long* idx = reinterpret_cast<const long long*>(index);
     if (in_place) {
-        const size_t smem = (size_t)cols * n_dst * 16;
-        if (smem > 24 * 1024) {      // beside 16 KB of lists: more than the 48 KB a launch may take unasked
-            const cudaError_t e = cudaFuncSetAttribute(permute_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) {
-                set_error("hira_gather: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));
-                return HIRA_ERR_CUDA;
-            }
+        const int smem = n_dst * 64 > GA_STAGE_BYTES ? n_dst * 64 : GA_STAGE_BYTES;
+        const cudaError_t e = cudaFuncSetAttribute(permute_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) {
+            set_error("hira_gather: cudaFuncSetAttribute(%d B smem): %s", smem, cudaGetErrorString(e));
+            return HIRA_ERR_CUDA;
         }
-        const long long blocks = strips < 4 * SM_COUNT ? strips : 4 * SM_COUNT;
-        permute_kernel<<<(unsigned)blocks, GA_THREADS, smem, s>>>(G, idx, n_dst, cols, status);
+        // strips of the direct copy; staged ones are more
+        const long long blocks = strips < 3 * SM_COUNT ? strips : 3 * SM_COUNT;
+        permute_kernel<<<(unsigned)blocks, GA_THREADS, smem, s>>>(G, idx, n_dst, smem, status);
     } else {
         const long long blocks = strips < 8 * SM_COUNT ? strips : 8 * SM_COUNT;
         gather_kernel<<<(unsigned)blocks, GA_THREADS, 0, s>>>(G, idx, n_src, n_dst, status);
@@ -210,15 +268,16 @@ extern "C" int hira_gather_index(const hira_index_t* from, const hira_index_t* t
     hira_gather_item_t it[GA_ITEMS];
     int n = 0;
     // the parents in use, and what belongs to them, lie before `p` in every head; behind is nothing
-    auto add = [&](const void* src, void* dst, long long row, long long rows, long long cap, uint32_t fill) {
+    auto add = [&](const void* src, void* dst, long long row, long long rows, long long cap, uint32_t fill, bool clear = true) {
         if (!src || !dst) return;
-        it[n++] = hira_gather_item_t{src, dst, heads * cap * row, heads * cap * row, cap * row, cap * row, rows * row, cap * row, heads, fill};
+        it[n++] = hira_gather_item_t{src, dst, heads * cap * row, heads * cap * row, cap * row, cap * row, rows * row,
+                                     (clear ? cap : rows) * row, heads, fill};
     };
     add(from->children, to->children, from->dim * es, p * bf, cp * bf, 0);
     add(from->values, to->values, from->vdim * ves, p * bf, cp * bf, 0);
-    add(from->children_q8, to->children_q8, 128, p * bf, cp * bf, 0);
+    add(from->children_q8, to->children_q8, 128, p * bf, cp * bf, 0, false);      // of free slots nothing is kept there
     add(from->slot2token, to->slot2token, 4, p * bf, cp * bf, 0xffffffffu);
-    add(from->children_q8_meta, to->children_q8_meta, 4, p * bf, cp * bf, 0);
+    add(from->children_q8_meta, to->children_q8_meta, 4, p * bf, cp * bf, 0, false);
     add(from->parents, to->parents, from->dim * es, p, cp, 0);
     add(from->parent_radii, to->parent_radii, 4, p, cp, 0);
     add(from->parent_sqnorm, to->parent_sqnorm, 4, p, cp, 0);

@@ -612,33 +612,65 @@ def with_rows(t: torch.Tensor) -> torch.Tensor:
     return t if row_strides(t) is not None else aligned(t.contiguous())
 
 
-def shared_attn(q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, sm_scale: float, out):
-    """hira_shared_attn on tensors that `row_strides` accepts (tails and lengths may be None)."""
-    lib = L.load()
-    b, hq, n_q, d = q.shape
-    p, h, n, vdim = prefix_v.shape
-    a = L.HiraSharedAttnStruct()
-    a.q, a.out = q.data_ptr(), out.data_ptr()
-    a.prefix_k, a.prefix_v, a.prefix_lens, a.tail_lens = L.ptr(prefix_k), L.ptr(prefix_v), L.ptr(prefix_lens), L.ptr(tail_lens)
-    a.q_stride[:], a.out_stride[:] = row_strides(q), row_strides(out)
-    a.prefix_k_stride[:], a.prefix_v_stride[:] = row_strides(prefix_k), row_strides(prefix_v)
-    a.prefix_len = n
-    if tail_k is not None:
-        a.tail_k, a.tail_v, a.tail_len = L.ptr(tail_k), L.ptr(tail_v), tail_k.shape[2]
-        a.tail_k_stride[:], a.tail_v_stride[:] = row_strides(tail_k), row_strides(tail_v)
-    a.dtype, a.n_prompts, a.n_branches, a.n_kv, a.group = L.dtype_code(q.dtype), p, b // p, h, hq // h
-    a.n_q, a.dim, a.vdim, a.sm_scale = n_q, d, vdim, float(sm_scale)
-    with torch.cuda.device(q.device):
-        nbytes = int(lib.hira_shared_attn_workspace_bytes(C.byref(a)))
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
-        L.check(lib.hira_shared_attn(C.byref(a), L.ptr(ws), nbytes, L.current_stream(q.device)), "hira_shared_attn")
-    return out
+def remember(plans: dict, key, plan):
+    """Keeps what follows from the layout of a call's arguments (never their addresses or contents), boundedly many."""
+    if len(plans) >= 512:
+        plans.clear()
+    plans[key] = plan
+    return plan
+
+
+class SharedAttnPlan:
+    """hira_shared_attn for tensors of one layout (all that `row_strides` accepts); the tails' length may change from call
+    to call."""
+
+    def __init__(self, q, prefix_k, prefix_v, tail_k, tail_v, sm_scale: float, out):
+        b, hq, n_q, d = q.shape
+        p, h, n, vdim = prefix_v.shape
+        a = self.args = L.HiraSharedAttnStruct()
+        a.q_stride[:], a.out_stride[:] = row_strides(q), row_strides(out)
+        a.prefix_k_stride[:], a.prefix_v_stride[:] = row_strides(prefix_k), row_strides(prefix_v)
+        a.prefix_len = n
+        if tail_k is not None:
+            a.tail_k_stride[:], a.tail_v_stride[:] = row_strides(tail_k), row_strides(tail_v)
+        a.dtype, a.n_prompts, a.n_branches, a.n_kv, a.group = L.dtype_code(q.dtype), p, b // p, h, hq // h
+        a.n_q, a.dim, a.vdim, a.sm_scale = n_q, d, vdim, float(sm_scale)
+        self.out_shape, self.device, self.index = (b, hq, n_q, vdim), q.device, q.get_device()
+
+    def __call__(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out=None):
+        """None where a tensor does not start on a 16-byte boundary."""
+        lib = L.load()
+        if out is None:
+            out = q.new_empty(self.out_shape)
+        a = L.HiraSharedAttnStruct.from_buffer_copy(self.args)      # one of its own for every call
+        pq, pk, pv, po = q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), out.data_ptr()
+        every = pq | pk | pv | po
+        a.q, a.prefix_k, a.prefix_v, a.out = pq, pk, pv, po
+        if tail_k is not None:
+            tk, tv = tail_k.data_ptr(), tail_v.data_ptr()
+            every |= tk | tv
+            a.tail_k, a.tail_v, a.tail_len = tk, tv, tail_k.shape[2]
+        if every & 15:
+            return None
+        if prefix_lens is not None:
+            a.prefix_lens = prefix_lens.data_ptr()
+        if tail_lens is not None:
+            a.tail_lens = tail_lens.data_ptr()
+        ref = C.byref(a)
+        nbytes = lib.hira_shared_attn_workspace_bytes(ref)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device) if nbytes else None
+        rc = L.on_device(self.index, lib.hira_shared_attn, ref, None if ws is None else ws.data_ptr(), nbytes)
+        if rc:
+            L.check(rc, "hira_shared_attn")
+        return out
 
 
 def check_picks(indices, n: int, device) -> torch.Tensor:
     """Indices of sequences as a contiguous int64 tensor on `device`.  What is on the host is checked here
     (the kernels check what is on the device); a mask becomes the indices it keeps."""
     t = torch.as_tensor(indices)
+    if t.dtype == torch.int64 and t.ndim == 1 and t.is_cuda and t.device == device and t.is_contiguous():
+        return t
     if t.ndim != 1:
         raise ValueError(f"indices must be one-dimensional, got {tuple(t.shape)}")
     if t.dtype == torch.bool:
@@ -666,9 +698,8 @@ def gather_rows(pairs, index: torch.Tensor, used_rows: int, status: Optional[tor
         it.dst_seq_stride, it.dst_seg_stride = dst.stride(0) * e, dst.stride(1) * e
         it.bytes = it.bytes_filled = used_rows * src.shape[3] * e
     src, dst = pairs[0]
-    with torch.cuda.device(src.device):
-        L.check(lib.hira_gather(items, len(pairs), L.ptr(index), src.shape[0], index.numel(), 1 if src is dst else 0, L.ptr(status),
-                                L.current_stream(src.device)), "hira_gather")
+    L.check(L.on_device(src.get_device(), lib.hira_gather, items, len(pairs), L.ptr(index), src.shape[0], index.numel(),
+                        1 if src is dst else 0, L.ptr(status)), "hira_gather")
 
 
 def _with_q8(st: IndexState) -> L.HiraIndexStruct:
@@ -684,27 +715,46 @@ def gather_index(src: IndexState, dst: IndexState, index: torch.Tensor, n_src: i
     lib = L.load()
     a, b = _with_q8(src), _with_q8(dst)
     nbytes = 0 if samples is None else samples[0].numel() * samples.element_size()
-    with torch.cuda.device(src.device):
-        L.check(lib.hira_gather_index(C.byref(a), C.byref(b), n_src, index.numel(), L.ptr(index), L.ptr(samples), nbytes,
-                                      L.ptr(dst.status), L.current_stream(src.device)), "hira_gather_index")
+    L.check(L.on_device(src.arrays_device.index, lib.hira_gather_index, C.byref(a), C.byref(b), n_src, index.numel(), L.ptr(index),
+                        L.ptr(samples), nbytes, L.ptr(dst.status)), "hira_gather_index")
 
 
-def qk_norm_rope(q, k, cos, sin, q_weight, k_weight, eps: float, interleaved: bool, out_q, out_k):
-    """hira_qk_norm_rope on tensors that `row_strides` accepts; cos / sin (B or 1, n, R) with contiguous rows."""
-    lib = L.load()
-    b, hq, n, d = q.shape
-    a = L.HiraRopeStruct()
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr()
-    a.q_weight, a.k_weight, a.cos, a.sin = L.ptr(q_weight), L.ptr(k_weight), L.ptr(cos), L.ptr(sin)
-    a.q_stride[:], a.k_stride[:] = row_strides(q), row_strides(k)
-    a.q_out_stride[:], a.k_out_stride[:] = row_strides(out_q), row_strides(out_k)
-    a.cos_stride[:] = (cos.stride(0) if cos.shape[0] > 1 else 0, cos.stride(1))
-    a.sin_stride[:] = (sin.stride(0) if sin.shape[0] > 1 else 0, sin.stride(1))
-    a.dtype, a.table_dtype, a.batch, a.n_tokens, a.q_heads, a.k_heads = L.dtype_code(q.dtype), L.dtype_code(cos.dtype), b, n, hq, k.shape[1]
-    a.dim, a.rotary, a.interleaved, a.eps = d, cos.shape[2], int(bool(interleaved)), float(eps)
-    with torch.cuda.device(q.device):
-        L.check(lib.hira_qk_norm_rope(C.byref(a), L.current_stream(q.device)), "hira_qk_norm_rope")
-    return out_q, out_k
+class RopePlan:
+    """hira_qk_norm_rope for tensors of one layout: heads that `row_strides` accepts, tables (B or 1, n, R)."""
+
+    def __init__(self, q, k, cos, sin, eps: float, interleaved: bool, out_q, out_k):
+        b, hq, n, d = q.shape
+        a = self.args = L.HiraRopeStruct()
+        a.q_stride[:], a.k_stride[:] = row_strides(q), row_strides(k)
+        a.q_out_stride[:], a.k_out_stride[:] = row_strides(out_q), row_strides(out_k)
+        a.cos_stride[:] = (cos.stride(0) if cos.shape[0] > 1 else 0, cos.stride(1) if n > 1 else 0)
+        a.sin_stride[:] = (sin.stride(0) if sin.shape[0] > 1 else 0, sin.stride(1) if n > 1 else 0)
+        a.dtype, a.table_dtype, a.batch, a.n_tokens = L.dtype_code(q.dtype), L.dtype_code(cos.dtype), b, n
+        a.q_heads, a.k_heads, a.dim, a.rotary, a.interleaved, a.eps = hq, k.shape[1], d, cos.shape[2], int(bool(interleaved)), float(eps)
+        self.index = q.get_device()
+
+    def __call__(self, q, k, cos, sin, q_weight, k_weight, out_q=None, out_k=None):
+        """None where a tensor does not start on a 16-byte boundary."""
+        if out_q is None:
+            out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if out_k is None:
+            out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
+        a = L.HiraRopeStruct.from_buffer_copy(self.args)            # one of its own for every call
+        pq, pk, oq, ok = q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr()
+        every = pq | pk | oq | ok
+        a.q, a.k, a.q_out, a.k_out, a.cos, a.sin = pq, pk, oq, ok, cos.data_ptr(), sin.data_ptr()
+        if q_weight is not None:
+            w = a.q_weight = q_weight.data_ptr()
+            every |= w
+        if k_weight is not None:
+            w = a.k_weight = k_weight.data_ptr()
+            every |= w
+        if every & 15:
+            return None
+        rc = L.on_device(self.index, L.load().hira_qk_norm_rope, C.byref(a))
+        if rc:
+            L.check(rc, "hira_qk_norm_rope")
+        return out_q, out_k
 
 
 class DecodeStep:
