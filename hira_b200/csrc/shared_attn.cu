@@ -186,16 +186,19 @@ shared_simt_kernel(const SharedAttn P) {
             if (ch < P.vdim) *reinterpret_cast<float4*>(P.part_o + at * P.vdim + ch) = make_float4(o[a][c][0], o[a][c][1], o[a][c][2], o[a][c][3]);
         }
     }
+    if (TAIL) grid_wait();      // so that who waits for this waits for the prefix too
 }
 
 // ---------------------------------------------------------------------------
 // The partials of an output row joined, by one warp.
 // ---------------------------------------------------------------------------
 constexpr int SA_MERGE_WARPS = 4;
+constexpr int SA_FLIGHT = 8;      // parts of a row on their way at once
 template <typename T>
 __global__ void __launch_bounds__(32 * SA_MERGE_WARPS)
 shared_merge_kernel(const SharedAttn P) {
     const int R = blockIdx.x * SA_MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    grid_wait();
     if (R >= P.n_rows) return;
     const int bh = R / P.n_q, heads = P.n_kv * P.group;
     const int item = bh / heads / P.n_branches * P.n_kv + bh % heads / P.group;
@@ -205,9 +208,9 @@ shared_merge_kernel(const SharedAttn P) {
     float M = -CUDART_INF_F;
     bool bad = false;
     for (int i = lane; i < n; i += 32) {
-        const float m = P.part_ml[part(i)].x;
-        bad |= m != m;
-        M = fmaxf(M, m);
+        const float2 ml = P.part_ml[part(i)];
+        bad |= ml.x != ml.x || ml.y != ml.y;       // a NaN among the logits, which a maximum passes over
+        M = fmaxf(M, ml.x);
     }
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
@@ -215,21 +218,40 @@ shared_merge_kernel(const SharedAttn P) {
     float L = 0.f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    const bool mine = lane * 8 < P.vdim;
     if (__any_sync(0xffffffffu, bad)) L = CUDART_NAN_F;
-    for (int i = 0; i < n; ++i) {
-        const size_t at = part(i);
-        const float2 ml = P.part_ml[at];
-        if (!(ml.x > -CUDART_INF_F)) continue;      // a part without keys has no sums either
-        const float w = exp2_approx(ml.x - base);
-        L = __fmaf_rn(w, ml.y, L);
-        if (mine) {
-            const float4* po = reinterpret_cast<const float4*>(P.part_o + at * P.vdim + lane * 8);
-            const float4 a = po[0], b = po[1];
-            acc[0] = __fmaf_rn(w, a.x, acc[0]); acc[1] = __fmaf_rn(w, a.y, acc[1]);
-            acc[2] = __fmaf_rn(w, a.z, acc[2]); acc[3] = __fmaf_rn(w, a.w, acc[3]);
-            acc[4] = __fmaf_rn(w, b.x, acc[4]); acc[5] = __fmaf_rn(w, b.y, acc[5]);
-            acc[6] = __fmaf_rn(w, b.z, acc[6]); acc[7] = __fmaf_rn(w, b.w, acc[7]);
+    // 32 parts at a time: each lane weighs one of them, then the rows come in, SA_FLIGHT at once
+    const bool mine = lane * 8 < P.vdim;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const size_t at = part(min(i0 + lane, n - 1));
+        const float2 ml = i0 + lane < n ? P.part_ml[at] : make_float2(-CUDART_INF_F, 0.f);
+        const float w = ml.x > -CUDART_INF_F ? exp2_approx(ml.x - base) : 0.f;      // a part without keys has no sums either
+        float wl = w > 0.f ? w * ml.y : 0.f;
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, s);
+        L += wl;
+        const int count = min(n - i0, 32);
+        for (int j0 = 0; j0 < count; j0 += SA_FLIGHT) {
+            float4 x[SA_FLIGHT][2];
+            float ws[SA_FLIGHT];
+#pragma unroll
+            for (int j = 0; j < SA_FLIGHT; ++j) {
+                ws[j] = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
+                if (j0 + j >= count) ws[j] = 0.f;
+                if (mine && ws[j] != 0.f) {      // (a NaN is read)
+                    const float4* po = reinterpret_cast<const float4*>(P.part_o + part(i0 + j0 + j) * P.vdim + lane * 8);
+                    x[j][0] = po[0];
+                    x[j][1] = po[1];
+                } else {
+                    x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < SA_FLIGHT; ++j) {
+                acc[0] = __fmaf_rn(ws[j], x[j][0].x, acc[0]); acc[1] = __fmaf_rn(ws[j], x[j][0].y, acc[1]);
+                acc[2] = __fmaf_rn(ws[j], x[j][0].z, acc[2]); acc[3] = __fmaf_rn(ws[j], x[j][0].w, acc[3]);
+                acc[4] = __fmaf_rn(ws[j], x[j][1].x, acc[4]); acc[5] = __fmaf_rn(ws[j], x[j][1].y, acc[5]);
+                acc[6] = __fmaf_rn(ws[j], x[j][1].z, acc[6]); acc[7] = __fmaf_rn(ws[j], x[j][1].w, acc[7]);
+            }
         }
     }
     if (!mine) return;
@@ -239,20 +261,28 @@ shared_merge_kernel(const SharedAttn P) {
 }
 
 template <typename T, int RPT, int NV, bool TAIL>
-static int launch_simt(const SharedAttn& P, cudaStream_t s) {
+static int launch_simt(const SharedAttn& P, bool chained, cudaStream_t s) {
     auto kern = shared_simt_kernel<T, RPT, NV, TAIL>;
     const int per = P.group * P.n_q, rows = TAIL ? per : P.n_branches * per;
     const size_t smem = sizeof(float) * ((size_t)(8 * RPT + SA_KEYS) * (P.dim + SA_PAD) + (size_t)SA_KEYS * (P.vdim + SA_PAD) +
                                          (size_t)SA_KEYS * (8 * RPT + SA_PAD));
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) {
         set_error("hira_shared_attn: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));
         return HIRA_ERR_CUDA;
     }
     const dim3 grid((unsigned)((rows + 8 * RPT - 1) / (8 * RPT)), (unsigned)(TAIL ? P.tail_parts : P.prefix_parts),
                     (unsigned)((TAIL ? P.n_prompts * P.n_branches : P.n_prompts) * P.n_kv));
-    kern<<<grid, SA_THREADS, smem, s>>>(P);
-    HIRA_CHECK_LAUNCH("hira_shared_attn launch");
+    if (chained) {
+        e = launch_chained(kern, grid, dim3(SA_THREADS), smem, s, P);
+    } else {
+        kern<<<grid, SA_THREADS, smem, s>>>(P);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) {
+        set_error("hira_shared_attn launch: %s", cudaGetErrorString(e));
+        return HIRA_ERR_CUDA;
+    }
     return HIRA_OK;
 }
 
@@ -260,17 +290,17 @@ static int launch_simt(const SharedAttn& P, cudaStream_t s) {
 static int simt_rows(int rows, int vdim) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 || vdim > 128 ? 32 : 64; }
 
 template <typename T, bool TAIL>
-static int launch_simt_rows(const SharedAttn& P, cudaStream_t s) {
+static int launch_simt_rows(const SharedAttn& P, bool chained, cudaStream_t s) {
     const int per = P.group * P.n_q, rows = simt_rows(TAIL ? per : P.n_branches * per, P.vdim);
     if (P.vdim > 128) {
-        if (rows == 8) return launch_simt<T, 1, 4, TAIL>(P, s);
-        if (rows == 16) return launch_simt<T, 2, 4, TAIL>(P, s);
-        return launch_simt<T, 4, 4, TAIL>(P, s);
+        if (rows == 8) return launch_simt<T, 1, 4, TAIL>(P, chained, s);
+        if (rows == 16) return launch_simt<T, 2, 4, TAIL>(P, chained, s);
+        return launch_simt<T, 4, 4, TAIL>(P, chained, s);
     }
-    if (rows == 8) return launch_simt<T, 1, 2, TAIL>(P, s);
-    if (rows == 16) return launch_simt<T, 2, 2, TAIL>(P, s);
-    if (rows == 32) return launch_simt<T, 4, 2, TAIL>(P, s);
-    return launch_simt<T, 8, 2, TAIL>(P, s);
+    if (rows == 8) return launch_simt<T, 1, 2, TAIL>(P, chained, s);
+    if (rows == 16) return launch_simt<T, 2, 2, TAIL>(P, chained, s);
+    if (rows == 32) return launch_simt<T, 4, 2, TAIL>(P, chained, s);
+    return launch_simt<T, 8, 2, TAIL>(P, chained, s);
 }
 
 // Splits of the keys: enough blocks for two an SM, none with fewer than two tiles of its own.
@@ -324,7 +354,8 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
     const int per = a->group * a->n_q;
     if (shared_tc_supported(P, a->dtype)) shared_tc_plan(P);
     else P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
-    P.tail_parts = simt_splits(per, a->n_prompts * a->n_branches * a->n_kv, a->tail_len, a->vdim);
+    P.tail_parts = shared_tail_supported(P, a->dtype) ? shared_tail_splits(P)
+                                                      : simt_splits(per, a->n_prompts * a->n_branches * a->n_kv, a->tail_len, a->vdim);
     return HIRA_OK;
 }
 static size_t shared_parts_bytes(const SharedAttn& P) {
@@ -333,13 +364,28 @@ static size_t shared_parts_bytes(const SharedAttn& P) {
 
 template <typename T>
 static int run_shared(const SharedAttn& P, cudaStream_t s) {
+    // The first kernel starts when all before it on the stream is done; the ones behind it may start beside it, so each
+    // waits for the one before it by its end (the merge: at its start).
     int rc = HIRA_OK;
     if (P.shares > 0) rc = shared_tc_launch(P, s);
-    else if (P.prefix_parts > 0) rc = launch_simt_rows<T, false>(P, s);
-    if (rc == HIRA_OK && P.tail_parts > 0) rc = launch_simt_rows<T, true>(P, s);
+    else if (P.prefix_parts > 0) rc = launch_simt_rows<T, false>(P, false, s);
     if (rc != HIRA_OK) return rc;
-    shared_merge_kernel<T><<<(unsigned)((P.n_rows + SA_MERGE_WARPS - 1) / SA_MERGE_WARPS), 32 * SA_MERGE_WARPS, 0, s>>>(P);
-    HIRA_CHECK_LAUNCH("hira_shared_attn merge launch");
+    if (P.tail_parts > 0)
+        rc = shared_tail_supported(P, sizeof(T) == 2 ? HIRA_BF16 : HIRA_F32) ? shared_tail_launch(P, P.prefix_parts > 0, s)
+                                                                            : launch_simt_rows<T, true>(P, P.prefix_parts > 0, s);
+    if (rc != HIRA_OK) return rc;
+    const dim3 grid((unsigned)((P.n_rows + SA_MERGE_WARPS - 1) / SA_MERGE_WARPS));
+    cudaError_t e;
+    if (P.prefix_parts + P.tail_parts > 0) {
+        e = launch_chained(shared_merge_kernel<T>, grid, dim3(32 * SA_MERGE_WARPS), 0, s, P);
+    } else {
+        shared_merge_kernel<T><<<grid, 32 * SA_MERGE_WARPS, 0, s>>>(P);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) {
+        set_error("hira_shared_attn merge launch: %s", cudaGetErrorString(e));
+        return HIRA_ERR_CUDA;
+    }
     return HIRA_OK;
 }
 

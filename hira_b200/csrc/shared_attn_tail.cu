@@ -1,0 +1,261 @@
+// The tails of hira_shared_attn for bf16 rows of up to 128: few query rows (group x tokens) against keys of their own.
+//
+// Bound by the tails' bytes: 16 query rows cost 16-bit matrix products that hide behind the loads.  A block of four
+// warps takes 16 rows of one (branch, kv head) against a run of its keys; each warp takes 16 keys of every 64, through
+// a ring of its own (cp.async, no barrier between warps), with softmax statistics of its own, and the four join once, at
+// the end.  Products by mma.sync m16n8k16: the rows are too few for a tcgen05 tile, which would be 7/8 empty.
+// 64 branches x 8 heads x 256 keys (134 MB): see the launch below for what it measured.
+#include "shared_attn.cuh"
+#include "tc_common.cuh"
+#include <math_constants.h>
+
+namespace hira {
+
+constexpr int TL_WARPS = 4;
+constexpr int TL_ROWS = 16;
+constexpr int TL_KEYS = 16;                     // keys a warp takes a step
+constexpr int TL_STEP = TL_WARPS * TL_KEYS;
+constexpr int TL_STAGES = 3;
+
+template <int HD>
+struct TlLayout {
+    static constexpr int ROW = HD * 2;                              // bytes
+    static constexpr int STAGE = 2 * TL_KEYS * ROW;                 // keys, then values, of one warp
+    static constexpr int BYTES = TL_WARPS * TL_STAGES * STAGE;      // the joined sums (16 x HD floats a warp) fit too
+};
+
+__device__ __forceinline__ void tl_cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void tl_ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tl_ldm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tl_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tl_pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(32 * TL_WARPS, 2)
+shared_tail_kernel(const SharedAttn P) {
+    using Lay = TlLayout<HD>;
+    extern __shared__ __align__(128) unsigned char tl_smem[];
+    __shared__ float s_m[TL_WARPS][TL_ROWS], s_l[TL_WARPS][TL_ROWS];
+    grid_trigger();      // the merge waits before it reads
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
+    const int row0 = blockIdx.x * TL_ROWS, split = blockIdx.y;
+    const int b = blockIdx.z / P.n_kv, h = blockIdx.z % P.n_kv, per = P.group * P.n_q;
+    const int len = shared_tail_len(P, b);
+    const __nv_bfloat16* gk = reinterpret_cast<const __nv_bfloat16*>(P.tk) + b * P.tks[0] + h * P.tks[1];
+    const __nv_bfloat16* gv = reinterpret_cast<const __nv_bfloat16*>(P.tv) + b * P.tvs[0] + h * P.tvs[1];
+    const int out_row0 = (b * P.n_kv + h) * per;
+
+    // this warp's steps: 16 keys of every 64
+    const int steps_all = (len + TL_STEP - 1) / TL_STEP;
+    const int t0 = (int)((long long)split * steps_all / P.tail_parts), t1 = (int)((long long)(split + 1) * steps_all / P.tail_parts);
+    const uint32_t ring = smem_u32(tl_smem) + warp * TL_STAGES * Lay::STAGE;
+    auto load = [&](int t, int stage) {
+        const int k0 = t * TL_STEP + warp * TL_KEYS;
+        if (t < t1 && k0 < len) {
+            constexpr int CH = HD / 8;
+#pragma unroll
+            for (int i = lane; i < TL_KEYS * CH; i += 32) {
+                const int r = i / CH, c = i % CH;
+                const uint32_t dst = ring + stage * Lay::STAGE + r * Lay::ROW + ((c ^ (r & 7)) << 4);
+                const bool row = k0 + r < len;       // behind the last key, and behind the row's channels: 0
+                tl_cp16(dst, row && c * 8 < P.dim ? gk + (k0 + r) * P.tks[2] + c * 8 : gk, row && c * 8 < P.dim);
+                tl_cp16(dst + TL_KEYS * Lay::ROW, row && c * 8 < P.vdim ? gv + (k0 + r) * P.tvs[2] + c * 8 : gv, row && c * 8 < P.vdim);
+            }
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < TL_STAGES - 1; ++i) load(t0 + i, i);
+
+    // queries as the products want them: rows g and g + 8, two channels a register
+    uint32_t q[HD / 16][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int r = row0 + g + 8 * j;
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(P.q) + (r < per ? shared_row_offset(P, out_row0 + r, P.qs) : 0);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int ch = k * 16 + u * 8 + tig * 2;
+                q[k][j + 2 * u] = r < per && ch < P.dim ? *reinterpret_cast<const uint32_t*>(src + ch) : 0u;
+            }
+    }
+    int seen[2];
+    float m[2], l[2], o[HD / 8][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        seen[j] = len - (P.n_q - 1 - (row0 + g + 8 * j) % P.n_q);
+        m[j] = -CUDART_INF_F;
+        l[j] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
+    for (int t = t0; t < t1; ++t) {
+        const int stage = (t - t0) % TL_STAGES;
+        load(t + TL_STAGES - 1, (t - t0 + TL_STAGES - 1) % TL_STAGES);
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(TL_STAGES - 1) : "memory");
+        __syncwarp();
+        const int k0 = t * TL_STEP + warp * TL_KEYS;
+        if (k0 < len) {          // the same for the warp
+            const uint32_t sk = ring + stage * Lay::STAGE, sv = sk + TL_KEYS * Lay::ROW;
+            float s[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) {
+                    uint32_t kk[4];
+                    const int r = n * 8 + (lane & 7), c = k * 4 + (lane >> 3);
+                    tl_ldm4(kk, sk + r * Lay::ROW + ((c ^ (r & 7)) << 4));
+                    tl_mma(s[n], q[2 * k], kk[0], kk[1]);
+                    tl_mma(s[n], q[2 * k + 1], kk[2], kk[3]);
+                }
+            float f[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float mx = -CUDART_INF_F;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& x = s[n][2 * j + e];
+                        x = k0 + n * 8 + tig * 2 + e < seen[j] ? x * P.scale_log2 : -CUDART_INF_F;
+                        mx = fmaxf(mx, x);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float nm = fmaxf(m[j], mx), base = nm > -CUDART_INF_F ? nm : 0.f;
+                f[j] = exp2_approx(m[j] - base);
+                m[j] = nm;
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& x = s[n][2 * j + e];
+                        x = exp2_approx(x - base);
+                        sum += x;
+                    }
+                l[j] = __fmaf_rn(l[j], f[j], sum);      // this lane's keys; the four lanes of a row are added at the end
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f))
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n) {
+                    o[n][0] *= f[0]; o[n][1] *= f[0];
+                    o[n][2] *= f[1]; o[n][3] *= f[1];
+                }
+            const uint32_t p[4] = {tl_pack(s[0][0], s[0][1]), tl_pack(s[0][2], s[0][3]), tl_pack(s[1][0], s[1][1]), tl_pack(s[1][2], s[1][3])};
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+                uint32_t vv[4];
+                const int r = ((lane >> 3) & 1) * 8 + (lane & 7), c = n * 2 + (lane >> 4);
+                tl_ldm4t(vv, sv + r * Lay::ROW + ((c ^ (r & 7)) << 4));
+                tl_mma(o[2 * n], p, vv[0], vv[1]);
+                tl_mma(o[2 * n + 1], p, vv[2], vv[3]);
+            }
+        }
+        __syncwarp();            // the stage is read before it is filled again
+    }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
+        if (tig == 0) {
+            s_m[warp][g + 8 * j] = m[j];
+            s_l[warp][g + 8 * j] = l[j];
+        }
+    }
+    __syncthreads();             // statistics of all warps; and no ring is in use any more
+    float* s_o = reinterpret_cast<float*>(tl_smem);      // [warp][row][HD]
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < TL_WARPS; ++w) top = fmaxf(top, s_m[w][g + 8 * j]);
+        const float w = top > -CUDART_INF_F ? exp2_approx(m[j] - top) : 0.f;
+        float* dst = s_o + (warp * TL_ROWS + g + 8 * j) * HD + tig * 2;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * j] * w, o[n][2 * j + 1] * w);
+    }
+    __syncthreads();
+    const size_t part = (size_t)(P.prefix_parts + split) * P.n_rows;
+    for (int i = tid; i < TL_ROWS * (HD / 4); i += 32 * TL_WARPS) {
+        const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+        if (row0 + r >= per || c >= P.vdim) continue;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < TL_WARPS; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * TL_ROWS + r) * HD + c);
+            a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        }
+        const size_t at = part + out_row0 + row0 + r;
+        *reinterpret_cast<float4*>(P.part_o + at * P.vdim + c) = a;
+        if (c == 0) {
+            float top = -CUDART_INF_F, sum = 0.f;
+            for (int w = 0; w < TL_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+            for (int w = 0; w < TL_WARPS; ++w) sum += s_m[w][r] > -CUDART_INF_F ? s_l[w][r] * exp2_approx(s_m[w][r] - top) : s_l[w][r];
+            P.part_ml[at] = make_float2(top, sum);
+        }
+    }
+    grid_wait();                 // so that who waits for this waits for the prefix too
+}
+
+bool shared_tail_supported(const SharedAttn& P, int dtype) { return dtype == HIRA_BF16 && P.dim <= 128 && P.vdim <= 128; }
+
+// Splits of a tail: two blocks an SM, none with less than two steps of its own.
+int shared_tail_splits(const SharedAttn& P) {
+    if (P.tail_len <= 0) return 0;
+    const long long blocks = (long long)((P.group * P.n_q + TL_ROWS - 1) / TL_ROWS) * P.n_prompts * P.n_branches * P.n_kv;
+    const int steps = (P.tail_len + TL_STEP - 1) / TL_STEP;
+    long long s = 2 * SM_COUNT / blocks;
+    if (s > steps / 2) s = steps / 2;
+    if (s > 32) s = 32;
+    return s < 1 ? 1 : (int)s;
+}
+
+template <int HD>
+static int tl_launch(const SharedAttn& P, bool chained, cudaStream_t s) {
+    auto kern = shared_tail_kernel<HD>;
+    const int smem = TlLayout<HD>::BYTES;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) {
+        const dim3 grid((unsigned)((P.group * P.n_q + TL_ROWS - 1) / TL_ROWS), (unsigned)P.tail_parts, (unsigned)(P.n_prompts * P.n_branches * P.n_kv));
+        if (chained) {
+            e = launch_chained(kern, grid, dim3(32 * TL_WARPS), smem, s, P);
+        } else {
+            kern<<<grid, 32 * TL_WARPS, smem, s>>>(P);
+            e = cudaGetLastError();
+        }
+    }
+    if (e != cudaSuccess) {
+        set_error("hira_shared_attn tail launch: %s", cudaGetErrorString(e));
+        return HIRA_ERR_CUDA;
+    }
+    return HIRA_OK;
+}
+int shared_tail_launch(const SharedAttn& P, bool chained, cudaStream_t s) {
+    return P.dim > 64 || P.vdim > 64 ? tl_launch<128>(P, chained, s) : tl_launch<64>(P, chained, s);
+}
+
+}  // namespace hira

@@ -170,6 +170,24 @@ def test_large_logits_of_either_sign():
         _check(hira_shared_attention(q, pk2, pv, tk, tv), _exact(q, pk2, pv, tk, tv))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_nan_in_sight_reaches_the_rows_that_see_it_and_no_other(dtype):
+    for where in ("query", "prefix", "tail"):
+        q, pk, pv, tk, tv = _qkv(2, 3, 2, 2, 1, 128, 128, 300, 40, dtype, seed=12)
+        good = hira_shared_attention(q, pk, pv, tk, tv)
+        hit = torch.zeros(6, 4, dtype=torch.bool, device="cuda")
+        if where == "query":
+            q[4, 1, 0, 5], hit[4, 1] = float("nan"), True
+        elif where == "prefix":
+            pk[1, 0, 200, 3], hit[3:, :2] = float("nan"), True
+        else:
+            tk[2, 1, 39, 3], hit[2, 2:] = float("nan"), True
+        got = hira_shared_attention(q, pk, pv, tk, tv)
+        assert bool(torch.isnan(got[hit]).all()) and bool((got[~hit] == good[~hit]).all()), where
+    q, pk, pv, tk, tv = _qkv(1, 2, 1, 2, 1, 64, 64, 300, 40, dtype, seed=13)
+    assert bool(torch.isnan(hira_shared_attention(q, pk * float("nan"), pv)).all())
+
+
 def test_prefix_beyond_two_gibi_elements():
     h, d, ctx = 1, 128, (1 << 24) + 77         # 2^31 elements and more: offsets beyond 32 bits
     k = torch.zeros((1, h, ctx, d), dtype=torch.bfloat16, device="cuda")
