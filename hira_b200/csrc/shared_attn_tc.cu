@@ -116,6 +116,15 @@ __device__ __forceinline__ void st_ld16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
+// A whole warp waits, and all lanes get the same answer.  The clock is looked at only where the phase is not complete yet:
+// a wait that need not wait lies on the path between two products.
+__device__ __forceinline__ bool st_wait(uint32_t bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const long long t0 = clock64();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+        if (__any_sync(0xffffffffu, (unsigned long long)(clock64() - t0) > TC_WAIT_CYCLES)) return false;
+    return true;
+}
 __device__ __forceinline__ float max3f(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -218,7 +227,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                 uint32_t pos = 0;
                 auto load = [&](const CUtensorMap* map, int tile, const StSegment& s) {
                     const uint32_t stage = pos % STAGES, round = pos / STAGES;
-                    if (round > 0 && (*fail || !mbar_wait(bar_empty + 8 * stage, (round - 1) & 1))) return false;
+                    if (round > 0 && (!mbar_wait(bar_empty + 8 * stage, (round - 1) & 1))) return false;
                     const uint32_t bar = bar_full + 8 * stage, dst = s_ring + stage * Lay::TILE_BYTES;
                     mbar_expect_tx(bar, Lay::TILE_BYTES);
     #pragma unroll
@@ -242,63 +251,74 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                     for (uint32_t p = pos > STAGES ? pos - STAGES : 0; p < pos; ++p) mbar_wait(bar_full + 8 * (p % STAGES), (p / STAGES) & 1);
             }
         } else if (warp == 9) {
-            // ---- products --------------------------------------------------------------------------------------
-            if ((tid & 31) == 0) {
-                uint32_t base = 0, segs = 0, n_p[2] = {0, 0};      // loads, segments and P tiles so far
-                bool ok = true;
-                while (ok && walk.next(P, share, seg)) {
-                    const int n = seg.n;
-                    if (n == 0) continue;
-                    ok = mbar_wait(bar_q, segs & 1) && !*fail;
-                    const int count[2] = {NT == 2 ? n : (n + 1) / 2, NT == 2 ? n : n / 2};
-                    auto tile_of = [&](int w, int i) { return NT == 2 ? i : 2 * i + w; };
-                    auto qk = [&](int w, int i) {
-                        const uint32_t pos = base + st_pos_k(tile_of(w, i)), stage = pos % STAGES;
-                        if (!mbar_wait(bar_full + 8 * stage, (pos / STAGES) & 1)) return false;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t a0 = s_q + (NT == 2 ? w : 0) * Lay::TILE_BYTES, b0 = s_ring + stage * Lay::TILE_BYTES;
-    #pragma unroll
+            // ---- products ------------------------------------------------------------------------------------
+            // The whole warp walks the loop, so that everything the instructions take is known to be the same in all
+            // lanes and lies in uniform registers; one lane issues.  (With one lane walking, each product waited some
+            // 120 cycles for its operands, twice the 64 that it takes.)
+            uint32_t leader;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+            uint32_t base = 0, segs = 0, n_p[2] = {0, 0};      // loads, segments and P tiles so far
+            bool ok = true;
+            while (ok && walk.next(P, share, seg)) {
+                const int n = seg.n;
+                if (n == 0) continue;
+                ok = st_wait(bar_q, segs & 1);
+                const int count[2] = {NT == 2 ? n : (n + 1) / 2, NT == 2 ? n : n / 2};
+                auto tile_of = [&](int w, int i) { return NT == 2 ? i : 2 * i + w; };
+                auto full = [&](uint32_t pos) { return st_wait(bar_full + 8 * (pos % STAGES), (pos / STAGES) & 1); };
+                auto qk = [&](int w, uint32_t pos) {
+                    const uint32_t stage = pos % STAGES, a0 = s_q + (NT == 2 ? w : 0) * Lay::TILE_BYTES, b0 = s_ring + stage * Lay::TILE_BYTES;
+                    if (leader) {
+#pragma unroll
                         for (int k = 0; k < HD / 16; ++k) {
                             const uint32_t off = (k >> 2) * Lay::BOX_BYTES + (k & 3) * 32;
                             st_mma_ss(tm_s + w * ST_KEYS, umma_desc(a0 + off), umma_desc(b0 + off), st_idesc(ST_KEYS, false), k > 0);
                         }
                         umma_commit(bar_s + 8 * w);
                         if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
-                        return true;
-                    };
-                    auto pv = [&](int w, int i) {
-                        const uint32_t pos = base + st_pos_v(tile_of(w, i), n), stage = pos % STAGES;
-                        if (!mbar_wait(bar_p + 8 * w, n_p[w] & 1) || *fail || !mbar_wait(bar_full + 8 * stage, (pos / STAGES) & 1)) return false;
+                    }
+                };
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                    if (ok && count[w] > 0) {
+                        const uint32_t pos = base + st_pos_k(tile_of(w, 0));
+                        ok = full(pos);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (ok) qk(w, pos);
+                    }
+                for (int i = 0; ok && i < count[0]; ++i)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        if (!ok || i >= count[w]) continue;
+                        // P V of tile i and Q K of the chain's next, back to back: the second is behind the first in the
+                        // pipe, so it may write S where P was.  The tiles are waited for first, P last.
+                        const bool more = i + 1 < count[w];
+                        const uint32_t pos_k = base + st_pos_k(tile_of(w, more ? i + 1 : i)), pos_v = base + st_pos_v(tile_of(w, i), n);
+                        ok = full(pos_v) && (!more || full(pos_k)) && st_wait(bar_p + 8 * w, n_p[w] & 1);
+                        if (!ok) continue;
                         ++n_p[w];
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t b0 = s_ring + stage * Lay::TILE_BYTES;
-    #pragma unroll
-                        for (int k = 0; k < ST_KEYS / 16; ++k)
-                            st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
-                        if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
-                        if (i == count[w] - 1) umma_commit(bar_o + 8 * w);
-                        return true;
-                    };
-                    for (int w = 0; w < 2; ++w)
-                        if (count[w] > 0) ok = ok && qk(w, 0);
-                    for (int i = 0; ok && i < count[0]; ++i)
-                        for (int w = 0; w < 2; ++w) {
-                            if (i < count[w]) ok = ok && pv(w, i);
-                            // behind that product in the pipe, so that it may write where P was
-                            if (i + 1 < count[w]) ok = ok && qk(w, i + 1);
+                        const uint32_t stage = pos_v % STAGES, b0 = s_ring + stage * Lay::TILE_BYTES;
+                        if (leader) {
+#pragma unroll
+                            for (int k = 0; k < ST_KEYS / 16; ++k)
+                                st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
+                            if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
+                            if (!more) umma_commit(bar_o + 8 * w);
                         }
-                    if (ok) umma_commit(bar_done);
-                    base += 2 * n;
-                    ++segs;
-                }
-                // nothing of the tensor cores may be under way when shared memory and TMEM are given back
-                if (!ok) {
-                    *fail = 1;
-                    umma_commit(bar_exit);
-                    mbar_wait(bar_exit, 0);
-                } else if (segs > 0) {
-                    mbar_wait(bar_done, (segs - 1) & 1);
-                }
+                        if (more) qk(w, pos_k);
+                    }
+                if (ok && leader) umma_commit(bar_done);
+                base += 2 * n;
+                ++segs;
+            }
+            // nothing of the tensor cores may be under way when shared memory and TMEM are given back
+            if (!ok) {
+                *fail = 1;
+                if (leader) umma_commit(bar_exit);
+                mbar_wait(bar_exit, 0);
+            } else if (segs > 0) {
+                mbar_wait(bar_done, (segs - 1) & 1);
             }
         }
     } else {
@@ -315,31 +335,31 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
         const uint32_t flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;     // a negative scale turns the queries round
         uint32_t base = 0, segs = 0, n_s = 0, n_o = 0;
         bool ok = true;
-        // the same answer for the whole warp: what follows is done by warps
-        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity) && !*fail) != 0; };
         while (walk.next(P, share, seg)) {
             const int prompt = seg.item / P.n_kv, h = seg.item % P.n_kv, n = seg.n;
             const int count = NT == 2 ? n : (n + 1 - w) / 2;
             float m = -CUDART_INF_F, l = 0.f;
             if (n > 0 && ok) {
                 // queries into the swizzled layout of the products; the products of the segment before have read theirs
-                if (segs > 0) ok = wait(bar_done, (segs - 1) & 1);
-                const int first = NT == 2 ? t : tid, step = NT == 2 ? ST_WG : 2 * ST_WG;
-                for (int i = first; i < ST_ROWS * (HD / 8); i += step) {
-                    const int r = i / (HD / 8), c = i % (HD / 8);
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (row0 + r < n_rows && c * 8 < P.dim) {
-                        x = *(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) +
-                                                             shared_row_offset(P, shared_row(P, prompt, h, row0 + r), P.qs)) + c);
-                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                    }
-                    *reinterpret_cast<uint4*>(sm + (NT == 2 ? w : 0) * Lay::TILE_BYTES + (c >> 3) * Lay::BOX_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
-                }
+                if (segs > 0) ok = st_wait(bar_done, (segs - 1) & 1);
+                // a thread takes a row (or half of one), all of it on its way at once
+                constexpr int CHUNKS = HD / 8 / (NT == 2 ? 1 : 2);
+                const int c0 = NT == 2 ? 0 : w * CHUNKS, have = row < n_rows ? P.dim / 8 : 0;
+                uint4 x[CHUNKS];
+                const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) +
+                                                                  (have ? shared_row_offset(P, shared_row(P, prompt, h, row), P.qs) : 0));
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) x[c] = c0 + c < have ? src[c0 + c] : make_uint4(0, 0, 0, 0);
+                unsigned char* dst = sm + (NT == 2 ? w : 0) * Lay::TILE_BYTES + t * 128;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+                    *reinterpret_cast<uint4*>(dst + ((c0 + c) >> 3) * Lay::BOX_BYTES + ((((c0 + c) & 7) ^ (t & 7)) << 4)) =
+                        make_uint4(x[c].x ^ flip, x[c].y ^ flip, x[c].z ^ flip, x[c].w ^ flip);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(bar_q);
                 for (int i = 0; i < count && ok; ++i) {
                     const int j = NT == 2 ? i : 2 * i + w, k0 = (seg.first + j) * ST_KEYS;
-                    ok = wait(bar_s + 8 * w, n_s & 1);
+                    ok = st_wait(bar_s + 8 * w, n_s & 1);
                     if (!ok) break;
                     ++n_s;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -406,7 +426,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                         // rows of the value tile behind the prompt's keys, whatever they hold: 0, as what TMA fills in
                         // behind the array (0 x NaN would be NaN)
                         const uint32_t pos = base + st_pos_v(j, n), stage = pos % STAGES;
-                        ok = wait(bar_full + 8 * stage, (pos / STAGES) & 1);
+                        ok = st_wait(bar_full + 8 * stage, (pos / STAGES) & 1);
                         unsigned char* v = sm + (NT + stage) * Lay::TILE_BYTES;
                         for (int q = valid * 8 + t; q < ST_KEYS * 8; q += ST_WG)
 #pragma unroll
@@ -417,7 +437,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                     mbar_arrive(bar_p + 8 * w);
                 }
                 if (count > 0 && ok) {
-                    ok = wait(bar_o + 8 * w, n_o & 1);
+                    ok = st_wait(bar_o + 8 * w, n_o & 1);
                     ++n_o;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
