@@ -176,7 +176,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
     extern __shared__ unsigned char st_smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(st_smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t s_q = smem_u32(sm), s_ring = s_q + NT * Lay::TILE_BYTES;
-    __shared__ __align__(8) unsigned long long s_bar[2 * ST_MAX_STAGES + 9];
+    __shared__ __align__(8) unsigned long long s_bar[2 * ST_MAX_STAGES + 11];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     const uint32_t bars = smem_u32(s_bar);
@@ -184,7 +184,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
     const uint32_t bar_q = bars + 16 * ST_MAX_STAGES;                            // the segment's queries are in place
     const uint32_t bar_done = bar_q + 8;                                         // all products of the segment are complete
     const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48;   // [2] S written, P written, O complete
-    const uint32_t bar_exit = bar_q + 64;
+    const uint32_t bar_pa = bar_q + 64, bar_exit = bar_q + 80;                   // [2] the first half of P written
 
     const int tid = threadIdx.x, warp = tid >> 5;
     const int rb = blockIdx.x % row_blocks, share = blockIdx.x / row_blocks;
@@ -200,6 +200,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
         for (int w = 0; w < 2; ++w) {
             mbar_init(bar_s + 8 * w, 1);
             mbar_init(bar_p + 8 * w, ST_WG);
+            mbar_init(bar_pa + 8 * w, ST_WG);
             mbar_init(bar_o + 8 * w, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -290,18 +291,27 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         if (!ok || i >= count[w]) continue;
-                        // P V of tile i and Q K of the chain's next, back to back: the second is behind the first in the
-                        // pipe, so it may write S where P was.  The tiles are waited for first, P last.
+                        // P V of tile i (its first half as soon as that half of P is there) and Q K of the chain's next, back
+                        // to back: the second is behind the first in the pipe, so it may write S where P was.  The tiles are
+                        // waited for first, P last.
                         const bool more = i + 1 < count[w];
                         const uint32_t pos_k = base + st_pos_k(tile_of(w, more ? i + 1 : i)), pos_v = base + st_pos_v(tile_of(w, i), n);
-                        ok = full(pos_v) && (!more || full(pos_k)) && st_wait(bar_p + 8 * w, n_p[w] & 1);
+                        const uint32_t stage = pos_v % STAGES, b0 = s_ring + stage * Lay::TILE_BYTES;
+                        ok = full(pos_v) && (!more || full(pos_k)) && st_wait(bar_pa + 8 * w, n_p[w] & 1);
+                        if (!ok) continue;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (leader) {
+#pragma unroll
+                            for (int k = 0; k < ST_KEYS / 32; ++k)
+                                st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
+                        }
+                        ok = st_wait(bar_p + 8 * w, n_p[w] & 1);
                         if (!ok) continue;
                         ++n_p[w];
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t stage = pos_v % STAGES, b0 = s_ring + stage * Lay::TILE_BYTES;
                         if (leader) {
 #pragma unroll
-                            for (int k = 0; k < ST_KEYS / 16; ++k)
+                            for (int k = ST_KEYS / 32; k < ST_KEYS / 16; ++k)
                                 st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
                             if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
                             if (!more) umma_commit(bar_o + 8 * w);
@@ -364,6 +374,17 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                     ++n_s;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const int valid = min(seg.len - k0, ST_KEYS);
+                    if (k0 + valid < min(P.prefix_len, k0 + ST_KEYS)) {
+                        // rows of the value tile behind the prompt's keys, whatever they hold: 0, as what TMA fills in
+                        // behind the array (0 x NaN would be NaN)
+                        const uint32_t pos = base + st_pos_v(j, n), stage = pos % STAGES;
+                        ok = st_wait(bar_full + 8 * stage, (pos / STAGES) & 1);
+                        unsigned char* v = sm + (NT + stage) * Lay::TILE_BYTES;
+                        for (int q = valid * 8 + t; q < ST_KEYS * 8; q += ST_WG)
+#pragma unroll
+                            for (int b = 0; b < Lay::BOXES; ++b) *reinterpret_cast<uint4*>(v + b * Lay::BOX_BYTES + q * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
                     if (warp_used) {
                         uint32_t s[4][32];
 #pragma unroll
@@ -418,20 +439,16 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                                 p[e] = pack_bf16(z.x, z.y);
                             }
                             st_st16(my_s + q * 16, p);
+                            if (q == 1) {
+                                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                mbar_arrive(bar_pa + 8 * w);
+                            }
                         }
                         l += sum2.x + sum2.y;
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    }
-                    if (k0 + valid < min(P.prefix_len, k0 + ST_KEYS)) {
-                        // rows of the value tile behind the prompt's keys, whatever they hold: 0, as what TMA fills in
-                        // behind the array (0 x NaN would be NaN)
-                        const uint32_t pos = base + st_pos_v(j, n), stage = pos % STAGES;
-                        ok = st_wait(bar_full + 8 * stage, (pos / STAGES) & 1);
-                        unsigned char* v = sm + (NT + stage) * Lay::TILE_BYTES;
-                        for (int q = valid * 8 + t; q < ST_KEYS * 8; q += ST_WG)
-#pragma unroll
-                            for (int b = 0; b < Lay::BOXES; ++b) *reinterpret_cast<uint4*>(v + b * Lay::BOX_BYTES + q * 16) = make_uint4(0, 0, 0, 0);
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    } else {
+                        mbar_arrive(bar_pa + 8 * w);
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     mbar_arrive(bar_p + 8 * w);
@@ -511,9 +528,18 @@ void shared_tc_plan(SharedAttn& P) {
     const int rows = P.n_branches * P.group * P.n_q, nt = rows > ST_ROWS ? 2 : 1, row_blocks = (rows + nt * ST_ROWS - 1) / (nt * ST_ROWS);
     P.item_tiles = (P.prefix_len + ST_KEYS - 1) / ST_KEYS;
     const long long total = (long long)P.n_prompts * P.n_kv * P.item_tiles;
+    const long long items = (long long)P.n_prompts * P.n_kv;
     long long shares = SM_COUNT / row_blocks;
+    if (shares < 1) shares = 1;
+    // A run that goes on in a second item pays for filling and draining the pipe again, about four tiles' time (64
+    // branches of 8 heads at 131,072 keys: such blocks ended 12 us behind the others' 128).  Runs that end with their
+    // items are taken where they cost no more than that.
+    if (items <= shares) {
+        const long long each = shares / items;
+        if ((P.item_tiles + each - 1) / each <= (total + shares - 1) / shares + 4) shares = each * items;
+    }
     if (shares > total) shares = total;
-    P.shares = shares < 1 ? 1 : (int)shares;
+    P.shares = (int)shares;
     P.parts_per_share = nt == 2 ? 1 : 2;
     // an item of T tiles spans at most this many runs of total / shares tiles
     const long long run = total / P.shares;

@@ -49,7 +49,8 @@ def _exact(q, pk, pv, tk, tv, plens=None, tlens=None, scaling=None):
                 logit = scaling * (x.abs() @ k.abs().T).amax(-1, keepdim=True)
                 off = 2 * (logit * (d + 8) * 2.0 ** -22 + 2.0 ** -21)
                 # sums over the keys in 32 bits; with bf16 each weight is rounded once more; the output once
-                off = off + 2.0 ** -23 * (64 + len(k) / 32) + (HALF[q.dtype] if q.dtype == torch.bfloat16 else 0)
+                # (and its exponential may be a polynomial's, 7.5e-5 off, in numerator and denominator)
+                off = off + 2.0 ** -23 * (64 + len(k) / 32) + (HALF[q.dtype] + 2 * 7.5e-5 if q.dtype == torch.bfloat16 else 0)
                 out[s, hh * g:(hh + 1) * g, t] = o
                 tol[s, hh * g:(hh + 1) * g, t] = off * mean + HALF[q.dtype] * o.abs() + 1e-30
     return out, tol
