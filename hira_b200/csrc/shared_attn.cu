@@ -25,6 +25,34 @@ constexpr int SA_PAD = 4;         // floats behind each row in shared memory: ro
 // (RPT + 4 16-byte loads for 16 RPT FMAs), for the weighted sums RPT rows x V / 16 channels.  A row's softmax
 // statistics stay with its 16 lanes, so the blocks only meet to exchange tiles.  fp32 products and sums throughout.
 // ---------------------------------------------------------------------------
+// rows k0 .. k0 + 63 of keys or values into shared memory as fp32; those from `len` on as 0, nothing of them is read
+__device__ __forceinline__ void sa_load_tile(float* dst, int ld, const float* src, long long stride, int k0, int len, int width) {
+    const uint32_t d0 = (uint32_t)__cvta_generic_to_shared(dst);
+    const int pieces = width / 4;
+    for (int i = threadIdx.x; i < SA_KEYS * pieces; i += SA_THREADS) {
+        const int r = i / pieces, c = i - r * pieces;
+        const bool there = k0 + r < len;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d0 + (uint32_t)(r * ld + c * 4) * 4),
+                     "l"(there ? src + (k0 + r) * stride + c * 4 : src), "r"(there ? 16 : 0) : "memory");
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+}
+__device__ __forceinline__ void sa_load_tile(float* dst, int ld, const __nv_bfloat16* src, long long stride, int k0, int len, int width) {
+    const int pieces = width / 8;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < SA_KEYS * pieces; i += SA_THREADS) {
+        const int r = i / pieces, c = i - r * pieces;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (k0 + r < len) to_float(load_chunk<__nv_bfloat16>(src + (k0 + r) * stride, c), f);
+        float4* d = reinterpret_cast<float4*>(dst + r * ld + c * 8);
+        d[0] = make_float4(f[0], f[1], f[2], f[3]);
+        d[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void sa_landed() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
 template <typename T, int RPT, int NV, bool TAIL>
 __global__ void __launch_bounds__(SA_THREADS)
 shared_simt_kernel(const SharedAttn P) {
@@ -51,7 +79,7 @@ shared_simt_kernel(const SharedAttn P) {
         return TAIL ? (owner * P.n_kv + h) * per + r : shared_row(P, owner, h, r);
     };
 
-    const int kc = P.dim / 8, vc = P.vdim / 8;
+    const int kc = P.dim / 8;
     for (int i = tid; i < ROWS * kc; i += SA_THREADS) {
         const int r = i / kc, c = i - r * kc;
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -78,26 +106,13 @@ shared_simt_kernel(const SharedAttn P) {
     // equal runs of tiles for the splits
     const int tiles = (len + SA_KEYS - 1) / SA_KEYS;
     const int t0 = (int)((long long)split * tiles / n_splits), t1 = (int)((long long)(split + 1) * tiles / n_splits);
+    // the values of a tile arrive while its products are formed, the next keys while its values are summed
+    if (t0 < t1) sa_load_tile(s_k, ldk, gk, ks, t0 * SA_KEYS, len, P.dim);
     for (int t = t0; t < t1; ++t) {
         const int k0 = t * SA_KEYS;
-        __syncthreads();      // the tile before is used up (and the queries are in place)
-        for (int i = tid; i < SA_KEYS * kc; i += SA_THREADS) {
-            const int r = i / kc, c = i - r * kc;
-            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (k0 + r < len) to_float(load_chunk<T>(gk + (k0 + r) * ks, c), f);
-            float4* d = reinterpret_cast<float4*>(s_k + r * ldk + c * 8);
-            d[0] = make_float4(f[0], f[1], f[2], f[3]);
-            d[1] = make_float4(f[4], f[5], f[6], f[7]);
-        }
-        for (int i = tid; i < SA_KEYS * vc; i += SA_THREADS) {
-            const int r = i / vc, c = i - r * vc;
-            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};      // past the last key: nothing there is read
-            if (k0 + r < len) to_float(load_chunk<T>(gv + (k0 + r) * vs, c), f);
-            float4* d = reinterpret_cast<float4*>(s_v + r * ldv + c * 8);
-            d[0] = make_float4(f[0], f[1], f[2], f[3]);
-            d[1] = make_float4(f[4], f[5], f[6], f[7]);
-        }
-        __syncthreads();
+        sa_load_tile(s_v, ldv, gv, vs, k0, len, P.vdim);
+        sa_landed<1>();
+        __syncthreads();      // the keys are there (and the queries)
         float s[RPT][4];
 #pragma unroll
         for (int a = 0; a < RPT; ++a)
@@ -121,6 +136,13 @@ shared_simt_kernel(const SharedAttn P) {
                     s[a][j] = __fmaf_rn(qq.w, kk[j].w, s[a][j]);
                 }
             }
+        }
+        __syncthreads();      // and used up
+        if (t + 1 < t1) {
+            sa_load_tile(s_k, ldk, gk, ks, k0 + SA_KEYS, len, P.dim);
+            sa_landed<1>();
+        } else {
+            sa_landed<0>();
         }
 #pragma unroll
         for (int a = 0; a < RPT; ++a) {
@@ -151,7 +173,7 @@ shared_simt_kernel(const SharedAttn P) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) s_p[(tx + 16 * j) * LDP + ty * RPT + a] = s[a][j];
         }
-        __syncwarp();         // a row's weights pass between its 16 lanes only
+        __syncthreads();      // the values are there; a row's weights pass between its 16 lanes only
 #pragma unroll 2
         for (int k = 0; k < SA_KEYS; ++k) {
             float p[RPT];
@@ -172,6 +194,7 @@ shared_simt_kernel(const SharedAttn P) {
                 }
             }
         }
+        __syncthreads();      // the values are used up
     }
     const int part = (TAIL ? P.prefix_parts : 0) + split;
 #pragma unroll
@@ -190,21 +213,28 @@ shared_simt_kernel(const SharedAttn P) {
 }
 
 // ---------------------------------------------------------------------------
-// The partials of an output row joined, by one warp.
+// The partials of an output row joined, by W warps: each weighs all parts (a lane a part), sums every W-th and the
+// first adds the sums up.  A few megabytes out of L2: bound by the round trips, so all loads of a round are issued at
+// once, and where a row has many parts four warps share them.
 // ---------------------------------------------------------------------------
 constexpr int SA_MERGE_WARPS = 4;
-constexpr int SA_FLIGHT = 8;      // parts of a row on their way at once
-template <typename T>
+constexpr int SA_FLIGHT = 8;      // parts of a row on their way at once, for each warp
+constexpr int SA_MAX_PARTS = 512;
+
+template <typename T, int W>
 __global__ void __launch_bounds__(32 * SA_MERGE_WARPS)
 shared_merge_kernel(const SharedAttn P) {
-    const int R = blockIdx.x * SA_MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    grid_wait();
-    if (R >= P.n_rows) return;
-    const int bh = R / P.n_q, heads = P.n_kv * P.group;
+    __shared__ float s_w[SA_MERGE_WARPS / W][SA_MAX_PARTS];
+    __shared__ float4 s_o[SA_MERGE_WARPS][64];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % W, slot = warp / W;
+    const int R = blockIdx.x * (SA_MERGE_WARPS / W) + slot;
+    const bool there = R < P.n_rows;
+    const int row = there ? R : P.n_rows - 1, bh = row / P.n_q, heads = P.n_kv * P.group;
     const int item = bh / heads / P.n_branches * P.n_kv + bh % heads / P.group;
     // the partials there are: the item's own, then (from prefix_parts on) the tail's
-    const int np = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0, n = np + P.tail_parts;
-    auto part = [&](int i) { return (size_t)(i < np ? i : i - np + P.prefix_parts) * P.n_rows + R; };
+    const int np = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0, n = np + P.tail_parts, gap = P.prefix_parts - np;
+    auto part = [&](int i) { return (size_t)(i < np ? i : i + gap) * P.n_rows + row; };
+    grid_wait();
     float M = -CUDART_INF_F;
     bool bad = false;
     for (int i = lane; i < n; i += 32) {
@@ -215,49 +245,66 @@ shared_merge_kernel(const SharedAttn P) {
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
     const float base = M > -CUDART_INF_F ? M : 0.f;
-    float L = 0.f, acc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    if (__any_sync(0xffffffffu, bad)) L = CUDART_NAN_F;
-    // 32 parts at a time: each lane weighs one of them, then the rows come in, SA_FLIGHT at once
-    const bool mine = lane * 8 < P.vdim;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const size_t at = part(min(i0 + lane, n - 1));
-        const float2 ml = i0 + lane < n ? P.part_ml[at] : make_float2(-CUDART_INF_F, 0.f);
+    float L = 0.f;
+    for (int i = lane; i < n; i += 32) {
+        const float2 ml = P.part_ml[part(i)];
         const float w = ml.x > -CUDART_INF_F ? exp2_approx(ml.x - base) : 0.f;      // a part without keys has no sums either
-        float wl = w > 0.f ? w * ml.y : 0.f;
+        L += w > 0.f ? w * ml.y : 0.f;
+        if (i % W == wi) s_w[slot][i] = w;         // the parts this warp sums
+    }
 #pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, s);
-        L += wl;
-        const int count = min(n - i0, 32);
-        for (int j0 = 0; j0 < count; j0 += SA_FLIGHT) {
-            float4 x[SA_FLIGHT][2];
-            float ws[SA_FLIGHT];
+    for (int w = 16; w >= 1; w >>= 1) L += __shfl_xor_sync(0xffffffffu, L, w);
+    if (__any_sync(0xffffffffu, bad)) L = CUDART_NAN_F;
+    __syncwarp();
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int ch = lane * 4 + c * 128;
+        if (c * 128 >= P.vdim) break;
+        const float* src = P.part_o + (ch < P.vdim ? ch : 0);
+        for (int i0 = wi; i0 < n; i0 += W * SA_FLIGHT) {
+            float4 x[SA_FLIGHT];
+#pragma unroll
+            for (int j = 0; j < SA_FLIGHT; ++j) x[j] = *reinterpret_cast<const float4*>(src + part(min(i0 + j * W, n - 1)) * P.vdim);
 #pragma unroll
             for (int j = 0; j < SA_FLIGHT; ++j) {
-                ws[j] = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
-                if (j0 + j >= count) ws[j] = 0.f;
-                if (mine && ws[j] != 0.f) {      // (a NaN is read)
-                    const float4* po = reinterpret_cast<const float4*>(P.part_o + part(i0 + j0 + j) * P.vdim + lane * 8);
-                    x[j][0] = po[0];
-                    x[j][1] = po[1];
-                } else {
-                    x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                const float w = i0 + j * W < n ? s_w[slot][i0 + j * W] : 0.f;
+                if (w != 0.f) {      // what a part without keys has there is not used, whatever it is
+                    acc[c].x = __fmaf_rn(w, x[j].x, acc[c].x); acc[c].y = __fmaf_rn(w, x[j].y, acc[c].y);
+                    acc[c].z = __fmaf_rn(w, x[j].z, acc[c].z); acc[c].w = __fmaf_rn(w, x[j].w, acc[c].w);
                 }
-            }
-#pragma unroll
-            for (int j = 0; j < SA_FLIGHT; ++j) {
-                acc[0] = __fmaf_rn(ws[j], x[j][0].x, acc[0]); acc[1] = __fmaf_rn(ws[j], x[j][0].y, acc[1]);
-                acc[2] = __fmaf_rn(ws[j], x[j][0].z, acc[2]); acc[3] = __fmaf_rn(ws[j], x[j][0].w, acc[3]);
-                acc[4] = __fmaf_rn(ws[j], x[j][1].x, acc[4]); acc[5] = __fmaf_rn(ws[j], x[j][1].y, acc[5]);
-                acc[6] = __fmaf_rn(ws[j], x[j][1].z, acc[6]); acc[7] = __fmaf_rn(ws[j], x[j][1].w, acc[7]);
             }
         }
     }
-    if (!mine) return;
+    if (W > 1) {
+        s_o[warp][lane] = acc[0];
+        s_o[warp][lane + 32] = acc[1];
+        __syncthreads();
+        if (wi != 0) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = L == 0.f ? 0.f : acc[e] / L;      // no key seen: 0 (a NaN stays one)
-    store_chunk(reinterpret_cast<T*>(P.out) + shared_row_offset(P, R, P.os), lane, acc);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int w = 1; w < W; ++w) {
+                const float4 x = s_o[warp + w][lane + 32 * c];
+                acc[c].x += x.x; acc[c].y += x.y; acc[c].z += x.z; acc[c].w += x.w;
+            }
+    }
+    if (!there) return;
+    T* out = reinterpret_cast<T*>(P.out) + shared_row_offset(P, R, P.os);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int ch = lane * 4 + c * 128;
+        if (ch >= P.vdim) continue;
+        float4 y;      // no key seen: 0 (a NaN stays one)
+        y.x = L == 0.f ? 0.f : acc[c].x / L; y.y = L == 0.f ? 0.f : acc[c].y / L;
+        y.z = L == 0.f ? 0.f : acc[c].z / L; y.w = L == 0.f ? 0.f : acc[c].w / L;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(out + ch) = y;
+        } else {
+            __nv_bfloat162 lo = __floats2bfloat162_rn(y.x, y.y), hi = __floats2bfloat162_rn(y.z, y.w);
+            *reinterpret_cast<uint2*>(out + ch) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+        }
+    }
 }
 
 template <typename T, int RPT, int NV, bool TAIL>
@@ -356,10 +403,11 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
     else P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
     P.tail_parts = shared_tail_supported(P, a->dtype) ? shared_tail_splits(P)
                                                       : simt_splits(per, a->n_prompts * a->n_branches * a->n_kv, a->tail_len, a->vdim);
+    P.fused = shared_tail_supported(P, a->dtype) && shared_tail_joins(P);
     return HIRA_OK;
 }
 static size_t shared_parts_bytes(const SharedAttn& P) {
-    return (size_t)(P.prefix_parts + P.tail_parts) * P.n_rows * (P.vdim + 2) * sizeof(float);
+    return (size_t)(P.prefix_parts + (P.fused ? 0 : P.tail_parts)) * P.n_rows * (P.vdim + 2) * sizeof(float);
 }
 
 template <typename T>
@@ -373,13 +421,17 @@ static int run_shared(const SharedAttn& P, cudaStream_t s) {
     if (P.tail_parts > 0)
         rc = shared_tail_supported(P, sizeof(T) == 2 ? HIRA_BF16 : HIRA_F32) ? shared_tail_launch(P, P.prefix_parts > 0, s)
                                                                             : launch_simt_rows<T, true>(P, P.prefix_parts > 0, s);
-    if (rc != HIRA_OK) return rc;
-    const dim3 grid((unsigned)((P.n_rows + SA_MERGE_WARPS - 1) / SA_MERGE_WARPS));
+    if (rc != HIRA_OK || P.fused) return rc;
+    const int parts = P.prefix_parts + P.tail_parts;
+    const bool many = parts > SA_FLIGHT;
+    const int rows = many ? 1 : SA_MERGE_WARPS;
+    const dim3 grid((unsigned)((P.n_rows + rows - 1) / rows));
+    auto merge = many ? shared_merge_kernel<T, SA_MERGE_WARPS> : shared_merge_kernel<T, 1>;
     cudaError_t e;
-    if (P.prefix_parts + P.tail_parts > 0) {
-        e = launch_chained(shared_merge_kernel<T>, grid, dim3(32 * SA_MERGE_WARPS), 0, s, P);
+    if (parts > 0) {
+        e = launch_chained(merge, grid, dim3(32 * SA_MERGE_WARPS), 0, s, P);
     } else {
-        shared_merge_kernel<T><<<grid, 32 * SA_MERGE_WARPS, 0, s>>>(P);
+        merge<<<grid, 32 * SA_MERGE_WARPS, 0, s>>>(P);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) {
@@ -406,7 +458,7 @@ extern "C" int hira_shared_attn(const hira_shared_attn_t* a, void* workspace, si
     HIRA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), HIRA_ERR_CAPACITY,
                    "hira_shared_attn: a 16-byte aligned workspace of %zu bytes is needed, %zu given", need, workspace_bytes);
     P.part_o = reinterpret_cast<float*>(workspace);
-    P.part_ml = reinterpret_cast<float2*>(P.part_o + (size_t)(P.prefix_parts + P.tail_parts) * P.n_rows * P.vdim);
+    P.part_ml = reinterpret_cast<float2*>(P.part_o + (size_t)(P.prefix_parts + (P.fused ? 0 : P.tail_parts)) * P.n_rows * P.vdim);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return a->dtype == HIRA_BF16 ? run_shared<__nv_bfloat16>(P, s) : run_shared<float>(P, s);
 }

@@ -23,6 +23,7 @@ struct SharedAttn {
     int prefix_len, tail_len;
     int prefix_parts;             // partials of the prefix (at most, see `shares`), then the tail's
     int tail_parts;
+    int fused;                    // the tail's kernel joins the parts itself
     int n_rows;                   // output rows
     float scale_log2;             // sm_scale * log2(e)
     long long qs[3], os[3];       // elements between branches, heads, tokens
@@ -30,7 +31,7 @@ struct SharedAttn {
     long long tks[3], tvs[3];     // branches, heads, rows
     // The tensor-core kernel deals the key tiles of all (prompt, kv head) items out in `shares` equal runs, so an item's
     // number of partials follows from its position (0: every item has prefix_parts of them).
-    int shares, item_tiles, parts_per_share;
+    int shares, item_tiles;
 };
 
 __device__ __forceinline__ int shared_prefix_len(const SharedAttn& P, int prompt) {
@@ -59,7 +60,7 @@ __device__ __forceinline__ int shared_share_of(const SharedAttn& P, long long ti
 __device__ __forceinline__ int shared_first_share(const SharedAttn& P, int item) { return shared_share_of(P, (long long)item * P.item_tiles); }
 __device__ __forceinline__ int shared_item_parts(const SharedAttn& P, int item) {
     if (P.shares == 0) return P.prefix_parts;
-    return (shared_share_of(P, (long long)(item + 1) * P.item_tiles - 1) - shared_first_share(P, item) + 1) * P.parts_per_share;
+    return shared_share_of(P, (long long)(item + 1) * P.item_tiles - 1) - shared_first_share(P, item) + 1;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -72,6 +73,7 @@ void shared_tc_plan(SharedAttn& P);
 int shared_tc_launch(const SharedAttn& P, cudaStream_t s);
 bool shared_tail_supported(const SharedAttn& P, int dtype);
 int shared_tail_splits(const SharedAttn& P);
+bool shared_tail_joins(const SharedAttn& P);
 // chained: behind the prefix's kernel, beside which it may run
 int shared_tail_launch(const SharedAttn& P, bool chained, cudaStream_t s);
 

@@ -16,6 +16,7 @@ constexpr int TL_ROWS = 16;
 constexpr int TL_KEYS = 16;                     // keys a warp takes a step
 constexpr int TL_STEP = TL_WARPS * TL_KEYS;
 constexpr int TL_STAGES = 3;
+constexpr int TL_FLIGHT = 8;                    // parts of a row on their way at once
 
 template <int HD>
 struct TlLayout {
@@ -44,7 +45,7 @@ __device__ __forceinline__ uint32_t tl_pack(float lo, float hi) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(32 * TL_WARPS, 2)
+__global__ void __launch_bounds__(32 * TL_WARPS, HD == 128 ? 2 : 3)
 shared_tail_kernel(const SharedAttn P) {
     using Lay = TlLayout<HD>;
     extern __shared__ __align__(128) unsigned char tl_smem[];
@@ -199,6 +200,82 @@ shared_tail_kernel(const SharedAttn P) {
         for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * j] * w, o[n][2 * j + 1] * w);
     }
     __syncthreads();
+    if (P.fused) {
+        // The tail's only part: what the merge would do with it and the prefix's parts, done here.  A warp takes a row, a
+        // lane four channels.
+        const int rows = min(per - row0, TL_ROWS), ch = lane * 4;
+        const int item = b / P.n_branches * P.n_kv + h;
+        const int n = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0;
+        grid_wait();             // the prefix's parts are there
+        for (int r0 = warp; r0 < rows; r0 += 2 * TL_WARPS) {      // two rows at a time, for their loads to overlap
+            int row[2];
+            float base[2], w_t[2], l_t[2], L[2], wi[2];
+            float4 acc[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = min(r0 + k * TL_WARPS, rows - 1);
+                row[k] = out_row0 + row0 + r;
+                float m_t = -CUDART_INF_F;
+                l_t[k] = L[k] = 0.f;
+                for (int w = 0; w < TL_WARPS; ++w) m_t = fmaxf(m_t, s_m[w][r]);
+                for (int w = 0; w < TL_WARPS; ++w) l_t[k] += s_m[w][r] > -CUDART_INF_F ? s_l[w][r] * exp2_approx(s_m[w][r] - m_t) : s_l[w][r];
+                float M = m_t;
+                for (int i = lane; i < n; i += 32) M = fmaxf(M, P.part_ml[(size_t)i * P.n_rows + row[k]].x);
+#pragma unroll
+                for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+                base[k] = M > -CUDART_INF_F ? M : 0.f;
+                w_t[k] = m_t > -CUDART_INF_F ? exp2_approx(m_t - base[k]) : 0.f;
+                acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (ch < HD)
+                    for (int w = 0; w < TL_WARPS; ++w) {
+                        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * TL_ROWS + r) * HD + ch);
+                        acc[k].x += x.x; acc[k].y += x.y; acc[k].z += x.z; acc[k].w += x.w;
+                    }
+                acc[k].x *= w_t[k]; acc[k].y *= w_t[k]; acc[k].z *= w_t[k]; acc[k].w *= w_t[k];
+            }
+            const float* src = P.part_o + (ch < P.vdim ? ch : 0);
+            for (int i0 = 0; i0 < n; i0 += 32) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float2 ml = i0 + lane < n ? P.part_ml[(size_t)(i0 + lane) * P.n_rows + row[k]] : make_float2(-CUDART_INF_F, 0.f);
+                    wi[k] = ml.x > -CUDART_INF_F ? exp2_approx(ml.x - base[k]) : 0.f;
+                    // a NaN among a part's logits, which a maximum passes over, is in its sum (or its maximum)
+                    L[k] += wi[k] > 0.f ? wi[k] * ml.y : ml.x != ml.x ? ml.x : ml.y != ml.y ? ml.y : 0.f;
+                }
+                const int count = min(n - i0, 32);
+                for (int j0 = 0; j0 < count; j0 += TL_FLIGHT) {
+                    float4 x[2][TL_FLIGHT];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int j = 0; j < TL_FLIGHT; ++j)
+                            x[k][j] = *reinterpret_cast<const float4*>(src + ((size_t)min(i0 + j0 + j, n - 1) * P.n_rows + row[k]) * P.vdim);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int j = 0; j < TL_FLIGHT; ++j) {
+                            const float wj = __shfl_sync(0xffffffffu, wi[k], (j0 + j) & 31);
+                            if (j0 + j < count && wj != 0.f) {      // what a part without keys has there is not used
+                                acc[k].x = __fmaf_rn(wj, x[k][j].x, acc[k].x); acc[k].y = __fmaf_rn(wj, x[k][j].y, acc[k].y);
+                                acc[k].z = __fmaf_rn(wj, x[k][j].z, acc[k].z); acc[k].w = __fmaf_rn(wj, x[k][j].w, acc[k].w);
+                            }
+                        }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int w = 16; w >= 1; w >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], w);
+                L[k] += w_t[k] > 0.f ? w_t[k] * l_t[k] : l_t[k] != l_t[k] ? l_t[k] : 0.f;
+                if (ch < P.vdim && r0 + k * TL_WARPS < rows) {   // no key seen: 0 (a NaN stays one)
+                    const float inv = L[k] == 0.f ? 0.f : 1.f / L[k];
+                    const uint2 y = make_uint2(tl_pack(acc[k].x * inv, acc[k].y * inv), tl_pack(acc[k].z * inv, acc[k].w * inv));
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + shared_row_offset(P, row[k], P.os) + ch) = y;
+                }
+            }
+        }
+        return;
+    }
     const size_t part = (size_t)(P.prefix_parts + split) * P.n_rows;
     for (int i = tid; i < TL_ROWS * (HD / 4); i += 32 * TL_WARPS) {
         const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
@@ -221,6 +298,9 @@ shared_tail_kernel(const SharedAttn P) {
     grid_wait();                 // so that who waits for this waits for the prefix too
 }
 
+// A block that joins the parts of its rows itself saves a launch and its round trips, as long as its warps have no more
+// than the two rows each that they join at a time (15 branches of 9 rows: 30 us that way, 25 with the merge's kernel).
+bool shared_tail_joins(const SharedAttn& P) { return P.tail_parts == 1 && P.group * P.n_q <= 2 * TL_WARPS; }
 bool shared_tail_supported(const SharedAttn& P, int dtype) { return dtype == HIRA_BF16 && P.dim <= 128 && P.vdim <= 128; }
 
 // Splits of a tail: two blocks an SM, none with less than two steps of its own.

@@ -7,7 +7,7 @@
 // and two groups of four warps turn S into P, each thread one row: no exchange between threads for maximum and sum.
 // The two groups are two independent chains, so that one group's exponentials run under the other's products:
 //   256 rows: a group has 128 rows of its own, both see every tile;
-//   128 rows: the groups take the tiles alternately, and each leaves a partial of its own (two partials a block).
+//   128 rows: the groups take the tiles alternately, and their sums are joined at the end.
 // The reference maximum of a row moves only when a tile exceeds it by 2^8: until then O and the sum stay as they are
 // (weights up to 256 lose nothing in floating point), and O in TMEM is rescaled in rare tiles instead of each.
 //
@@ -343,7 +343,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
         const int row = row0 + t;
         const float scale = fabsf(P.scale_log2);
         const uint32_t flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;     // a negative scale turns the queries round
-        uint32_t base = 0, segs = 0, n_s = 0, n_o = 0;
+        uint32_t base = 0, segs = 0, n_s = 0, n_o[2] = {0, 0};
         bool ok = true;
         while (walk.next(P, share, seg)) {
             const int prompt = seg.item / P.n_kv, h = seg.item % P.n_kv, n = seg.n;
@@ -453,33 +453,64 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     mbar_arrive(bar_p + 8 * w);
                 }
-                if (count > 0 && ok) {
-                    ok = st_wait(bar_o + 8 * w, n_o & 1);
-                    ++n_o;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+                    if (NT == 2 ? v == w : n > v) {      // the chains whose sums this group is going to read
+                        ok = ok && st_wait(bar_o + 8 * v, n_o[v] & 1);
+                        ++n_o[v];
+                    }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 base += 2 * n;
                 ++segs;
             }
             if (!ok) *fail = 1;
-            const int part = NT == 2 ? seg.part : 2 * seg.part + w;
-            if (warp_used) {
-                const bool mine = row < n_rows;
-                const size_t at = (size_t)part * P.n_rows + (mine ? shared_row(P, prompt, h, row) : 0);
-                if (mine) P.part_ml[at] = ok ? make_float2(m, l) : make_float2(CUDART_NAN_F, CUDART_NAN_F);
-                if (count > 0 && ok) {
-                    uint32_t o[16];
+            // What the run adds to its rows.  Chains with rows of their own leave them as they are; two chains over the same rows
+            // are joined here, each group writing half of the channels.
+            const bool mine = warp_used && row < n_rows;
+            const size_t at = (size_t)seg.part * P.n_rows + (mine ? shared_row(P, prompt, h, row) : 0);
+            float f[2] = {1.f, 1.f};       // factors of the chains' sums
+            if (NT == 1) {
+                float2* s_ml = reinterpret_cast<float2*>(sm);      // in the queries' place: the products have read them
+                s_ml[tid] = ok ? make_float2(m, l) : make_float2(CUDART_NAN_F, CUDART_NAN_F);
+                asm volatile("bar.sync 1, %0;" ::"n"(2 * ST_WG) : "memory");
+                const float2 c0 = s_ml[t], c1 = s_ml[ST_WG + t];
+                m = fmaxf(c0.x, c1.x);
+                const float base_m = m > -CUDART_INF_F ? m : 0.f;
+                f[0] = c0.x > -CUDART_INF_F ? exp2_approx(c0.x - base_m) : 0.f;
+                f[1] = c1.x > -CUDART_INF_F ? exp2_approx(c1.x - base_m) : 0.f;
+                // (a sum is NaN without a maximum where all logits were; a maximum is where a wait ran out)
+                l = (c0.x > -CUDART_INF_F ? f[0] * c0.y : c0.y) + (c1.x > -CUDART_INF_F ? f[1] * c1.y : c1.y);
+                if (c0.x != c0.x || c1.x != c1.x) m = CUDART_NAN_F;
+            } else if (!ok) {
+                m = CUDART_NAN_F;
+            }
+            if (mine && (NT == 2 || w == 0)) P.part_ml[at] = make_float2(m, l);
+            if (warp_used && n > 0 && ok) {
+                const int chains = NT == 2 || n < 2 ? 1 : 2, from = NT == 2 ? 0 : w * (HD / 2);
+                uint32_t o[16], o1[16];
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 16) {
-                        st_ld16(my_o + c, o);
-                        if (mine)
+                for (int c = from; c < from + (NT == 2 ? HD : HD / 2); c += 16) {
+                    st_ld16(tm_o + (NT == 2 ? w * HD : 0) + lanes + c, o);
+                    if (NT == 1) {
+                        if (chains == 2) st_ld16(tm_o + HD + lanes + c, o1);
 #pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                if (c + e < P.vdim)
-                                    *reinterpret_cast<float4*>(P.part_o + at * P.vdim + c + e) =
-                                        make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                        for (int e = 0; e < 16; ++e) {
+                            float y = __uint_as_float(o[e]) * f[0];
+                            if (chains == 2) y = __fmaf_rn(__uint_as_float(o1[e]), f[1], y);
+                            o[e] = __float_as_uint(y);
+                        }
                     }
+                    if (mine)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            if (c + e < P.vdim)
+                                *reinterpret_cast<float4*>(P.part_o + at * P.vdim + c + e) =
+                                    make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
                 }
+            }
+            if (NT == 1) {      // the other group's sums and statistics are read before they are written again
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(2 * ST_WG) : "memory");
             }
         }
     }
@@ -540,12 +571,11 @@ void shared_tc_plan(SharedAttn& P) {
     }
     if (shares > total) shares = total;
     P.shares = (int)shares;
-    P.parts_per_share = nt == 2 ? 1 : 2;
     // an item of T tiles spans at most this many runs of total / shares tiles
     const long long run = total / P.shares;
     long long runs = (P.item_tiles + run - 1) / run + 1;
     if (runs > P.shares) runs = P.shares;
-    P.prefix_parts = (int)runs * P.parts_per_share;
+    P.prefix_parts = (int)runs;
 }
 
 template <int HD, int NT>
