@@ -178,7 +178,7 @@ def _declare(lib):
     lib.hira_gather.restype = C.c_int
     lib.hira_gather.argtypes = [C.POINTER(HiraGatherItemStruct), I32, P, I32, I32, I32, P, P]
     lib.hira_gather_index.restype = C.c_int
-    lib.hira_gather_index.argtypes = [IX, IX, I32, I32, P, P, I64, P, P]
+    lib.hira_gather_index.argtypes = [IX, IX, I32, I32, P, P, I64, P, P, P]
     lib.hira_qk_norm_rope.restype = C.c_int
     lib.hira_qk_norm_rope.argtypes = [C.POINTER(HiraRopeStruct), P]
     lib.hira_assign.restype = C.c_int

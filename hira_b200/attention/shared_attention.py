@@ -217,7 +217,6 @@ class SharedPrompt:
                 raise ValueError(f"indices {host} do not keep {p} prompts apart, with equally many sequences each in their order")
         return idx
 
-    @torch.no_grad()
     def reorder(self, indices):
         """In place: sequence b goes on from what sequence indices[b] was (any may be picked many times).  Sequences
         that pick themselves are not touched, and prompts never are.  An index on the device that is out of range
@@ -229,7 +228,6 @@ class SharedPrompt:
             S.gather_rows([(self._k, self._k), (self._v, self._v)], idx, self._len, self.status)
         return self
 
-    @torch.no_grad()
     def select(self, indices) -> "SharedPrompt":
         """The picked sequences (forked where an index repeats, compacted where some are left out) over the same prompts."""
         idx = self._picks(indices)

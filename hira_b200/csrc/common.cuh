@@ -74,6 +74,23 @@ inline cudaError_t launch_chained(K kern, dim3 grid, dim3 block, size_t smem, cu
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
+// A kernel's limit of dynamic shared memory, raised once on each device (and again for more): asking for it on every
+// launch costs a microsecond of the host's.  One of these belongs to one kernel.
+struct SmemLimit {
+    static constexpr int DEVICES = 64;
+    int have[DEVICES] = {};      // racing threads store what they have raised it to
+    template <typename K>
+    cudaError_t raise(K kern, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const bool kept = dev >= 0 && dev < DEVICES;
+        if (kept && __atomic_load_n(&have[dev], __ATOMIC_RELAXED) >= bytes) return cudaSuccess;
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && kept) __atomic_store_n(&have[dev], bytes, __ATOMIC_RELAXED);
+        return e;
+    }
+};
 // tiles of `tile_parents` parent slots that can hold keys (hira_index_t::active_parents)
 int active_tiles(const hira_index_t* ix, int tile_parents);
 

@@ -59,15 +59,22 @@ __device__ __forceinline__ void gather_strip(const hira_gather_item_t& g, long l
 }
 
 __global__ void __launch_bounds__(GA_THREADS)
-gather_kernel(const __grid_constant__ GatherItems items, const long long* __restrict__ index, int n_src, int n_dst, int32_t* status) {
+gather_kernel(const __grid_constant__ GatherItems items, const long long* __restrict__ index, int n_src, int n_dst,
+              const int32_t* __restrict__ status_from, int32_t* status) {
     __shared__ int s_idx[GA_MAX_SEQ];
+    int bad = 0;
     for (int j = threadIdx.x; j < n_dst; j += GA_THREADS) {
         const long long i = index[j];
         const bool ok = i >= 0 && i < n_src;
-        if (!ok && status && blockIdx.x == 0) atomicOr(status, HIRA_STATUS_BAD_INDEX);
+        bad |= !ok;
         s_idx[j] = ok ? (int)i : -1;      // a sequence that is not there: left empty
     }
-    __syncthreads();
+    bad = __syncthreads_or(bad);
+    if (status && blockIdx.x == 0 && threadIdx.x == 0) {
+        const int now = bad ? HIRA_STATUS_BAD_INDEX : 0;
+        if (status_from) *status = *status_from | now;
+        else if (now) atomicOr(status, now);
+    }
     for (long long strip = blockIdx.x; strip < items.first[items.n]; strip += gridDim.x) {
         int a = 0;
         while (strip >= items.first[a + 1]) ++a;
@@ -199,8 +206,8 @@ permute_kernel(const __grid_constant__ GatherItems items, const long long* __res
 
 using namespace hira;
 
-extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, const int64_t* index, int32_t n_src, int32_t n_dst,
-                           int32_t in_place, int32_t* status, void* stream) {
+static int run_gather(const hira_gather_item_t* items, int32_t n_items, const int64_t* index, int32_t n_src, int32_t n_dst,
+                      int32_t in_place, const int32_t* status_from, int32_t* status, void* stream) {
     HIRA_CHECK_ARG(items && index, HIRA_ERR_ARG, "hira_gather: items and index must not be NULL");
     HIRA_CHECK_ARG(n_items >= 0 && n_items <= GA_ITEMS, HIRA_ERR_SHAPE, "hira_gather: %d arrays outside 0..%d", n_items, GA_ITEMS);
     HIRA_CHECK_ARG(n_src >= 1 && n_dst >= 1 && n_src <= GA_MAX_SEQ && n_dst <= GA_MAX_SEQ, HIRA_ERR_SHAPE,
@@ -232,7 +239,8 @@ extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, con
     const long long* idx = reinterpret_cast<const long long*>(index);
     if (in_place) {
         const int smem = n_dst * 64 > GA_STAGE_BYTES ? n_dst * 64 : GA_STAGE_BYTES;
-        const cudaError_t e = cudaFuncSetAttribute(permute_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        static SmemLimit limit;
+        const cudaError_t e = limit.raise(permute_kernel, smem);
         if (e != cudaSuccess) {
             set_error("hira_gather: cudaFuncSetAttribute(%d B smem): %s", smem, cudaGetErrorString(e));
             return HIRA_ERR_CUDA;
@@ -242,14 +250,19 @@ extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, con
         permute_kernel<<<(unsigned)blocks, GA_THREADS, smem, s>>>(G, idx, n_dst, smem, status);
     } else {
         const long long blocks = strips < 8 * SM_COUNT ? strips : 8 * SM_COUNT;
-        gather_kernel<<<(unsigned)blocks, GA_THREADS, 0, s>>>(G, idx, n_src, n_dst, status);
+        gather_kernel<<<(unsigned)blocks, GA_THREADS, 0, s>>>(G, idx, n_src, n_dst, status_from, status);
     }
     HIRA_CHECK_LAUNCH("hira_gather launch");
     return HIRA_OK;
 }
 
+extern "C" int hira_gather(const hira_gather_item_t* items, int32_t n_items, const int64_t* index, int32_t n_src, int32_t n_dst,
+                           int32_t in_place, int32_t* status, void* stream) {
+    return run_gather(items, n_items, index, n_src, n_dst, in_place, nullptr, status, stream);
+}
+
 extern "C" int hira_gather_index(const hira_index_t* from, const hira_index_t* to, int32_t n_src, int32_t n_dst, const int64_t* index,
-                                 void* samples, int64_t sample_bytes, int32_t* status, void* stream) {
+                                 void* samples, int64_t sample_bytes, const int32_t* status_from, int32_t* status, void* stream) {
     int rc = validate_index(from, false);
     if (rc == HIRA_OK) rc = validate_index(to, false);
     if (rc != HIRA_OK) return rc;
@@ -295,5 +308,5 @@ extern "C" int hira_gather_index(const hira_index_t* from, const hira_index_t* t
         it[n++] = hira_gather_item_t{samples, samples, heads * sample_bytes, heads * sample_bytes, sample_bytes, sample_bytes,
                                      sample_bytes, sample_bytes, heads, 0};
     }
-    return hira_gather(it, n, index, n_src, n_dst, in_place, status, stream);
+    return run_gather(it, n, index, n_src, n_dst, in_place, in_place ? nullptr : status_from, status, stream);
 }

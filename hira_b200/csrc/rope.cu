@@ -35,12 +35,13 @@ struct RopeParams {
     const void* sin;
     long long cs[2], ss[2]; // sequences, tokens
     long long units;        // groups of heads of all tokens
-    int n_tokens, dim, rotary, pairs, per_token;
+    int n_tokens, dim, rotary;
+    int q_units, per_token; // groups of a token's query heads, of all its heads
     int wide_tables;        // 16-byte loads of the tables
     float eps;
 };
 
-// channels 8c .. 8c + 7 of a table row; those from R on as cos = 1, sin = 0: they pass through
+// channels 8c .. 8c + 7 of a table row; those from R on as `other`
 template <typename TT>
 __device__ __forceinline__ void load_table(const TT* row, int c, int rotary, int wide, float other, float (&f)[8]) {
     if (wide && c * 8 + 8 <= rotary) {
@@ -50,136 +51,148 @@ __device__ __forceinline__ void load_table(const TT* row, int c, int rotary, int
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = c * 8 + e < rotary ? (float)row[c * 8 + e] : other;
 }
+// the partner of channel ch, and the sign it enters with
+template <int PAIRS>
+__device__ __forceinline__ int rope_partner(int ch, int half, float& sign) {
+    if (PAIRS == ROPE_INTERLEAVED) {
+        sign = ch & 1 ? 1.f : -1.f;
+        return ch ^ 1;
+    }
+    sign = ch < half ? -1.f : 1.f;
+    return ch < half ? ch + half : ch - half;
+}
 
-template <typename T, typename TT, int NCH, int HPG>
-__global__ void __launch_bounds__(RP_THREADS)
+// With the norm's factor r of a row, y_i = r (x_i a_i + x_p b_i), where a_i = w_i cos_i and b_i = +-w_p sin_i belong to the
+// token and are formed once for the group's heads.
+template <typename T, typename TT, int NCH, int HPG, int PAIRS>
+__global__ void __launch_bounds__(RP_THREADS, HPG == 1 || NCH > 2 ? 1 : sizeof(T) == 2 ? 5 : 4)
 rope_kernel(const RopeParams P) {
     const int lane = threadIdx.x & (GROUP - 1);
     const long long unit = (long long)blockIdx.x * RP_GROUPS + threadIdx.x / GROUP;
     if (unit >= P.units) return;
     const long long bt = unit / P.per_token;
-    const int h0 = (int)(unit - bt * P.per_token) * HPG, b = (int)(bt / P.n_tokens), token = (int)(bt - (long long)b * P.n_tokens);
-    const int nq = P.side[0].heads, heads = nq + P.side[1].heads;
+    const int b = (int)(bt / P.n_tokens), token = (int)(bt - (long long)b * P.n_tokens);
+    int h0 = (int)(unit - bt * P.per_token) * HPG;
+    const bool keys = h0 >= P.q_units * HPG;          // a group's heads are all of one side
+    if (keys) h0 -= P.q_units * HPG;
+    const RopeSide& S = P.side[keys];
+    const int n = min(S.heads - h0, HPG), half = P.rotary / 2;
+    const T* x0 = reinterpret_cast<const T*>(S.x) + b * S.xs[0] + h0 * S.xs[1] + token * S.xs[2];
+    const T* w = reinterpret_cast<const T*>(S.w);
+    bool in[NCH];      // chunks of the row
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) in[i] = (lane + GROUP * i) * 8 < P.dim;
     RawChunk<T> raw[HPG][NCH];
-    const T* x[HPG];
 #pragma unroll
-    for (int j = 0; j < HPG; ++j) {
-        const int hh = min(h0 + j, heads - 1);
-        const RopeSide& S = P.side[hh >= nq];
-        x[j] = reinterpret_cast<const T*>(S.x) + b * S.xs[0] + (hh >= nq ? hh - nq : hh) * S.xs[1] + token * S.xs[2];
+    for (int j = 0; j < HPG; ++j)
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = lane + GROUP * i;
-            if (c * 8 < P.dim) raw[j][i] = load_chunk_coherent<T>(x[j], c);
-            else raw[j][i] = zero_chunk<T>();
-        }
-    }
-    float cs[NCH][8], sn[NCH][8];
+        for (int i = 0; i < NCH; ++i)
+            raw[j][i] = in[i] && j < n ? load_chunk_coherent<T>(x0 + j * S.xs[1], lane + GROUP * i) : zero_chunk<T>();
+    float ca[NCH][8], cb[NCH][8];
     const TT* cos = reinterpret_cast<const TT*>(P.cos) + b * P.cs[0] + token * P.cs[1];
     const TT* sin = reinterpret_cast<const TT*>(P.sin) + b * P.ss[0] + token * P.ss[1];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int c = lane + GROUP * i;
-        load_table<TT>(cos, c, P.rotary, P.wide_tables, 1.f, cs[i]);
-        load_table<TT>(sin, c, P.rotary, P.wide_tables, 0.f, sn[i]);
+        load_table<TT>(cos, c, P.rotary, P.wide_tables, 1.f, ca[i]);
+        load_table<TT>(sin, c, P.rotary, P.wide_tables, 0.f, cb[i]);
+        float own[8];
+        if (w && in[i]) {
+            to_float(load_chunk<T>(w, c), own);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ca[i][e] *= own[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int ch = c * 8 + e;
+            if (ch < P.rotary) {
+                float sign;
+                const int q = rope_partner<PAIRS>(ch, half, sign);
+                cb[i][e] *= w ? sign * (float)w[q] : sign;
+            }
+        }
     }
-    const int half = P.rotary / 2;
+    T* y0 = reinterpret_cast<T*>(S.y) + b * S.ys[0] + h0 * S.ys[1] + token * S.ys[2];
 #pragma unroll
     for (int j = 0; j < HPG; ++j) {
-        const int hh = h0 + j;
-        if (hh >= heads) break;          // the same for the group
-        const RopeSide& S = P.side[hh >= nq];
-        const T* w = reinterpret_cast<const T*>(S.w);
+        if (j >= n) break;               // the same for the group
+        const T* x = x0 + j * S.xs[1];
         float v[NCH][8], r = 1.f;
-        Acc2 acc{0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            to_float(raw[j][i], v[i]);
-            chunk_fma(acc, v[i], v[i]);
-        }
-        // the norm of chunk c's channels (v itself, or partners read again) with their weights
-        auto scale = [&](float (&y)[8], int c) {
-            float ww[8];
-            to_float(load_chunk<T>(w, c), ww);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = y[e] * r * ww[e];
-        };
+        for (int i = 0; i < NCH; ++i) to_float(raw[j][i], v[i]);
         if (w) {
-            r = rsqrtf(group_sum(acc.e + acc.o) / (float)P.dim + P.eps);
+            Acc2 acc{0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < NCH; ++i)
-                if ((lane + GROUP * i) * 8 < P.dim) scale(v[i], lane + GROUP * i);
+            for (int i = 0; i < NCH; ++i) chunk_fma(acc, v[i], v[i]);
+            r = rsqrtf(group_sum(acc.e + acc.o) / (float)P.dim + P.eps);
         }
         float o[NCH][8];
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int c = lane + GROUP * i;
-            float p[8];                  // partners, with the sign they enter with
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = 0.f;
-            if (c * 8 < P.rotary) {
-                if (P.pairs == ROPE_INTERLEAVED) {
+            for (int e = 0; e < 8; ++e) o[i][e] = v[i][e] * ca[i][e];
+            if (c * 8 >= P.rotary) continue;
+            float p[8];
+            if (PAIRS == ROPE_INTERLEAVED) {
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        if (c * 8 + e < P.rotary) {
-                            p[e] = -v[i][e + 1];
-                            p[e + 1] = v[i][e];
-                        }
-                } else if (NCH == 2 && P.pairs == ROPE_LANE) {
+                for (int e = 0; e < 8; ++e) p[e] = v[i][e ^ 1];
+            } else if (PAIRS == ROPE_LANE) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = i == 0 ? -v[NCH - 1][e] : v[0][e];
-                } else if (P.pairs == ROPE_SINGLE) {
+                for (int e = 0; e < 8; ++e) p[e] = v[NCH - 1 - i][e];
+            } else if (PAIRS == ROPE_CHUNK) {
+                to_float(load_chunk_coherent<T>(x, c * 8 < half ? c + half / 8 : c - half / 8), p);      // this row again, from L1
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int ch = c * 8 + e;
-                        if (ch < P.rotary) {
-                            const int q = ch < half ? ch + half : ch - half;
-                            const float y = w ? (float)x[j][q] * r * (float)w[q] : (float)x[j][q];
-                            p[e] = ch < half ? -y : y;
-                        }
-                    }
-                } else {
-                    const bool first = c * 8 < half;
-                    const int q = first ? c + half / 8 : c - half / 8;
-                    to_float(load_chunk_coherent<T>(x[j], q), p);      // this row again, from L1
-                    if (w) scale(p, q);
-                    if (first)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) p[e] = -p[e];
+                for (int e = 0; e < 8; ++e) {
+                    const int ch = c * 8 + e;
+                    p[e] = ch < P.rotary ? (float)x[ch < half ? ch + half : ch - half] : 0.f;
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[i][e] = __fmaf_rn(p[e], sn[i][e], v[i][e] * cs[i][e]);
+            for (int e = 0; e < 8; ++e)      // a chunk may be rotated in part: what passes through has no partner
+                if (PAIRS == ROPE_LANE || PAIRS == ROPE_CHUNK || c * 8 + e < P.rotary) o[i][e] = __fmaf_rn(p[e], cb[i][e], o[i][e]);
         }
-        __syncwarp(group_mask());        // the output may be the input: every lane has read its partners
-        T* y = reinterpret_cast<T*>(S.y) + b * S.ys[0] + (hh >= nq ? hh - nq : hh) * S.ys[1] + token * S.ys[2];
+        if (w)
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = lane + GROUP * i;
-            if (c * 8 < P.dim) store_chunk(y, c, o[i]);
-        }
+            for (int i = 0; i < NCH; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[i][e] *= r;
+        __syncwarp(group_mask());        // the output may be the input: every lane has read its partners
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+            if (in[i]) store_chunk(y0 + j * S.ys[1], lane + GROUP * i, o[i]);
     }
 }
 
-template <typename T, typename TT, int NCH>
-static int launch_rope_n(RopeParams& P, int batch, cudaStream_t s) {
-    const int heads = P.side[0].heads + P.side[1].heads;
-    const long long tokens = (long long)batch * P.n_tokens;
-    // One head a group while that does not fill the GPU with threads several times over; else four.
-    const bool four = tokens * heads > 8ll * SM_COUNT * RP_GROUPS;
-    P.per_token = four ? (heads + 3) / 4 : heads;
-    P.units = tokens * P.per_token;
+template <typename T, typename TT, int NCH, int HPG, int PAIRS>
+static int launch_rope_hp(RopeParams& P, int batch, cudaStream_t s) {
+    P.q_units = (P.side[0].heads + HPG - 1) / HPG;
+    P.per_token = P.q_units + (P.side[1].heads + HPG - 1) / HPG;
+    P.units = (long long)batch * P.n_tokens * P.per_token;
     const long long blocks = (P.units + RP_GROUPS - 1) / RP_GROUPS;
-    HIRA_CHECK_ARG(blocks < (1ll << 31), HIRA_ERR_SHAPE, "hira_qk_norm_rope: %lld head rows exceed the grid limit", tokens * heads);
-    if (four) rope_kernel<T, TT, NCH, 4><<<(unsigned)blocks, RP_THREADS, 0, s>>>(P);
-    else rope_kernel<T, TT, NCH, 1><<<(unsigned)blocks, RP_THREADS, 0, s>>>(P);
+    HIRA_CHECK_ARG(blocks < (1ll << 31), HIRA_ERR_SHAPE, "hira_qk_norm_rope: %lld groups of heads exceed the grid limit", P.units);
+    rope_kernel<T, TT, NCH, HPG, PAIRS><<<(unsigned)blocks, RP_THREADS, 0, s>>>(P);
     HIRA_CHECK_LAUNCH("hira_qk_norm_rope launch");
     return HIRA_OK;
 }
+template <typename T, typename TT, int NCH>
+static int launch_rope_n(RopeParams& P, int pairs, int batch, cudaStream_t s) {
+    // One head a group while that does not fill the GPU with threads several times over; else four.
+    const bool four = (long long)batch * P.n_tokens * (P.side[0].heads + P.side[1].heads) > 8ll * SM_COUNT * RP_GROUPS;
+    if (NCH == 2 && pairs == ROPE_LANE)
+        return four ? launch_rope_hp<T, TT, NCH, 4, ROPE_LANE>(P, batch, s) : launch_rope_hp<T, TT, NCH, 1, ROPE_LANE>(P, batch, s);
+    if (pairs == ROPE_CHUNK || pairs == ROPE_LANE)
+        return four ? launch_rope_hp<T, TT, NCH, 4, ROPE_CHUNK>(P, batch, s) : launch_rope_hp<T, TT, NCH, 1, ROPE_CHUNK>(P, batch, s);
+    if (pairs == ROPE_INTERLEAVED)
+        return four ? launch_rope_hp<T, TT, NCH, 4, ROPE_INTERLEAVED>(P, batch, s) : launch_rope_hp<T, TT, NCH, 1, ROPE_INTERLEAVED>(P, batch, s);
+    return launch_rope_hp<T, TT, NCH, 1, ROPE_SINGLE>(P, batch, s);
+}
 template <typename T, typename TT>
-static int launch_rope(RopeParams& P, int batch, cudaStream_t s) {
+static int launch_rope(RopeParams& P, int pairs, int batch, cudaStream_t s) {
     const int nch = chunks_per_lane(P.dim);
-    return nch == 1 ? launch_rope_n<T, TT, 1>(P, batch, s) : nch == 2 ? launch_rope_n<T, TT, 2>(P, batch, s) : launch_rope_n<T, TT, 4>(P, batch, s);
+    return nch == 1 ? launch_rope_n<T, TT, 1>(P, pairs, batch, s) : nch == 2 ? launch_rope_n<T, TT, 2>(P, pairs, batch, s)
+                                                                             : launch_rope_n<T, TT, 4>(P, pairs, batch, s);
 }
 
 }  // namespace hira
@@ -219,9 +232,9 @@ extern "C" int hira_qk_norm_rope(const hira_rope_t* a, void* stream) {
     // a token's tables may start anywhere, its weights too (they are loaded in 16-byte pieces)
     const int ts = (int)elem_size(a->table_dtype);
     P.wide_tables = (((uintptr_t)a->cos | (uintptr_t)a->sin | (uintptr_t)((P.cs[0] | P.cs[1] | P.ss[0] | P.ss[1]) * ts)) & 15) == 0;
-    P.pairs = a->interleaved ? ROPE_INTERLEAVED : a->rotary % 16 ? ROPE_SINGLE : a->rotary == 128 && a->dim <= 128 ? ROPE_LANE : ROPE_CHUNK;
+    const int pairs = a->interleaved ? ROPE_INTERLEAVED : a->rotary % 16 ? ROPE_SINGLE : a->rotary == 128 && a->dim <= 128 ? ROPE_LANE : ROPE_CHUNK;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (a->dtype == HIRA_BF16)
-        return a->table_dtype == HIRA_BF16 ? launch_rope<__nv_bfloat16, __nv_bfloat16>(P, a->batch, s) : launch_rope<__nv_bfloat16, float>(P, a->batch, s);
-    return a->table_dtype == HIRA_BF16 ? launch_rope<float, __nv_bfloat16>(P, a->batch, s) : launch_rope<float, float>(P, a->batch, s);
+        return a->table_dtype == HIRA_BF16 ? launch_rope<__nv_bfloat16, __nv_bfloat16>(P, pairs, a->batch, s) : launch_rope<__nv_bfloat16, float>(P, pairs, a->batch, s);
+    return a->table_dtype == HIRA_BF16 ? launch_rope<float, __nv_bfloat16>(P, pairs, a->batch, s) : launch_rope<float, float>(P, pairs, a->batch, s);
 }

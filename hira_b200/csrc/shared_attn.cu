@@ -313,7 +313,8 @@ static int launch_simt(const SharedAttn& P, bool chained, cudaStream_t s) {
     const int per = P.group * P.n_q, rows = TAIL ? per : P.n_branches * per;
     const size_t smem = sizeof(float) * ((size_t)(8 * RPT + SA_KEYS) * (P.dim + SA_PAD) + (size_t)SA_KEYS * (P.vdim + SA_PAD) +
                                          (size_t)SA_KEYS * (8 * RPT + SA_PAD));
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(kern, (int)smem);
     if (e != cudaSuccess) {
         set_error("hira_shared_attn: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));
         return HIRA_ERR_CUDA;

@@ -318,7 +318,8 @@ template <int HD>
 static int tl_launch(const SharedAttn& P, bool chained, cudaStream_t s) {
     auto kern = shared_tail_kernel<HD>;
     const int smem = TlLayout<HD>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(kern, smem);
     if (e == cudaSuccess) {
         const dim3 grid((unsigned)((P.group * P.n_q + TL_ROWS - 1) / TL_ROWS), (unsigned)P.tail_parts, (unsigned)(P.n_prompts * P.n_branches * P.n_kv));
         if (chained) {

@@ -582,7 +582,8 @@ template <int HD, int NT>
 static int st_launch(const SharedAttn& P, int row_blocks, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
     auto kern = shared_tc_kernel<HD, NT>;
     const size_t smem = (size_t)(NT + st_stages<HD, NT>()) * StLayout<HD>::TILE_BYTES + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    const cudaError_t e = limit.raise(kern, (int)smem);
     if (e != cudaSuccess) {
         set_error("hira_shared_attn: cudaFuncSetAttribute(%zu B smem): %s", smem, cudaGetErrorString(e));
         return HIRA_ERR_CUDA;

@@ -6,6 +6,7 @@ the arrays follow the reference's CUDAIndexer attributes (indexer/cuda.py:40-54)
 """
 from __future__ import annotations
 
+import copy
 import ctypes as C
 from dataclasses import dataclass
 from functools import lru_cache
@@ -136,6 +137,21 @@ class IndexState:
     @property
     def struct(self):
         return self._byref
+
+    def like(self, n_heads: int) -> "IndexState":
+        """A state of the same shape for another number of heads; its arrays (and its status) are not filled."""
+        new = copy.copy(self)
+        new.n_heads = n_heads
+        for name in self.ARRAYS + self.Q8_ARRAYS:
+            t = getattr(self, name)
+            if t is not None:
+                setattr(new, name, torch.empty((n_heads, *t.shape[1:]), dtype=t.dtype, device=t.device))
+        new.status = torch.empty_like(self.status)
+        new._append_bytes, new._append_ws = {}, (None, 0)
+        new._streams = {L.current_stream(self.device)} if self.device.type == "cuda" else set()
+        new.__dict__.pop("_tile_parents", None)
+        new.refresh_struct()
+        return new
 
     def state_dict(self) -> dict:
         d = {name: getattr(self, name) for name in self.ARRAYS if getattr(self, name) is not None}
@@ -702,21 +718,23 @@ def gather_rows(pairs, index: torch.Tensor, used_rows: int, status: Optional[tor
                         1 if src is dst else 0, L.ptr(status)), "hira_gather")
 
 
-def _with_q8(st: IndexState) -> L.HiraIndexStruct:
+def _with_q8(st: IndexState):
     """The struct of `st` with its int8 side copy, also when enable_int8_copy has left that out of the view."""
+    if not st.int8_copy or st._struct.children_q8:
+        return st._byref
     s = L.HiraIndexStruct.from_buffer_copy(st._struct)
     for name in st.Q8_ARRAYS:
         setattr(s, name, L.ptr(getattr(st, name)))
-    return s
+    return C.byref(s)
 
 
 def gather_index(src: IndexState, dst: IndexState, index: torch.Tensor, n_src: int, samples: Optional[torch.Tensor] = None):
-    """hira_gather_index: sequences `index` of `src` (of `n_src`, heads folded) into `dst`, which may be `src`."""
+    """hira_gather_index: sequences `index` of `src` (of `n_src`, heads folded) into `dst`, which may be `src`; another one
+    takes its status on as well."""
     lib = L.load()
-    a, b = _with_q8(src), _with_q8(dst)
     nbytes = 0 if samples is None else samples[0].numel() * samples.element_size()
-    L.check(L.on_device(src.arrays_device.index, lib.hira_gather_index, C.byref(a), C.byref(b), n_src, index.numel(), L.ptr(index),
-                        L.ptr(samples), nbytes, L.ptr(dst.status)), "hira_gather_index")
+    L.check(L.on_device(src.arrays_device.index, lib.hira_gather_index, _with_q8(src), _with_q8(dst), n_src, index.numel(), L.ptr(index),
+                        L.ptr(samples), nbytes, None if src is dst else L.ptr(src.status), L.ptr(dst.status)), "hira_gather_index")
 
 
 class RopePlan:

@@ -436,7 +436,6 @@ class CUDAIndexer(BaseIndexer):
         return self
 
     # ---- sequences forked, reordered, compacted ------------------------------
-    @torch.no_grad()
     def reorder(self, indices):
         """In place: sequence b (of the B that were built) becomes what sequence indices[b] was; any may be picked many
         times.  Sequences that pick themselves are not touched, and nothing is allocated.  `indices` (B,): on the host it
@@ -452,7 +451,6 @@ class CUDAIndexer(BaseIndexer):
         S.gather_index(st, st, idx, self.batch, drawn[1] if drawn is not None and drawn[0] is st else None)
         return self
 
-    @torch.no_grad()
     def select(self, indices) -> "CUDAIndexer":
         """A new index of the picked sequences: forked where an index repeats, compacted where some are left out.  This
         one stays as it is.  An index on the device that is out of range leaves an empty sequence and is reported by
@@ -464,10 +462,7 @@ class CUDAIndexer(BaseIndexer):
             raise ValueError("no sequence picked")
         heads = self.num_heads // self.batch
         new = copy.copy(self)
-        new.state = S.IndexState(n_heads=n * heads, dim=st.dim, vdim=st.vdim, bf=st.bf, depth=st.depth, cap_parents=st.cap_parents,
-                                 dtype=st.dtype, vdtype=st.vdtype, device=st.device, with_values=st.values is not None,
-                                 int8_copy=st.int8_copy, cleared=False)
-        new.state.status.copy_(st.status)
+        new.state = st.like(n * heads)
         new.num_heads, new.batch = n * heads, n
         new._snapshot = new._scan_slots = new._searched = new._pending_append = new._pinned = new._tau_samples = None
         new._scan_pending = new._searched_fresh = False

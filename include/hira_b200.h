@@ -566,9 +566,10 @@ int hira_gather(const hira_gather_item_t* items, int32_t n_items, const int64_t*
 /* hira_gather over the arrays of an index (heads folded as sequence * heads + head, `from` and `to` of one capacity;
  * from == to: in place), the int8 side copy with them.  Visits the parent slots below from->active_parents (0 = all).
  * samples: optional [heads of all sequences][sample_bytes] of rows drawn from the index (threshold finder), which
- * follow their sequences; in place only. */
+ * follow their sequences; in place only.  status_from: optional device word that *status starts from (not in place:
+ * *status then need not be set before). */
 int hira_gather_index(const hira_index_t* from, const hira_index_t* to, int32_t n_src, int32_t n_dst, const int64_t* index,
-                      void* samples, int64_t sample_bytes, int32_t* status, void* stream);
+                      void* samples, int64_t sample_bytes, const int32_t* status_from, int32_t* status, void* stream);
 
 /* Norms of the query and key heads and the rotation by position in one pass, from q, k to q_out, k_out (which may be
  * q, k themselves):

@@ -149,8 +149,8 @@ def test_library_refuses_gathers_that_do_not_fit():
     assert lib.hira_gather(one(n_seg=0), 1, 4096, 1, 1, 0, None, None) == L.HIRA_OK      # nothing to move
     a = S.IndexState(n_heads=4, dim=64, vdim=64, bf=8, depth=2, cap_parents=16, dtype=torch.float32, vdtype=torch.float32, device="cpu")
     b = S.IndexState(n_heads=6, dim=64, vdim=64, bf=8, depth=2, cap_parents=17, dtype=torch.float32, vdtype=torch.float32, device="cpu")
-    assert lib.hira_gather_index(a.struct, b.struct, 2, 3, 4096, None, 0, None, None) == L.HIRA_ERR_SHAPE
-    assert lib.hira_gather_index(a.struct, a.struct, 3, 3, 4096, None, 0, None, None) == L.HIRA_ERR_SHAPE
+    assert lib.hira_gather_index(a.struct, b.struct, 2, 3, 4096, None, 0, None, None, None) == L.HIRA_ERR_SHAPE
+    assert lib.hira_gather_index(a.struct, a.struct, 3, 3, 4096, None, 0, None, None, None) == L.HIRA_ERR_SHAPE
 
 
 @pytest.mark.parametrize("kw,code", [
