@@ -51,17 +51,6 @@ __device__ __forceinline__ void load_table(const TT* row, int c, int rotary, int
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = c * 8 + e < rotary ? (float)row[c * 8 + e] : other;
 }
-// the partner of channel ch, and the sign it enters with
-template <int PAIRS>
-__device__ __forceinline__ int rope_partner(int ch, int half, float& sign) {
-    if (PAIRS == ROPE_INTERLEAVED) {
-        sign = ch & 1 ? 1.f : -1.f;
-        return ch ^ 1;
-    }
-    sign = ch < half ? -1.f : 1.f;
-    return ch < half ? ch + half : ch - half;
-}
-
 // With the norm's factor r of a row, y_i = r (x_i a_i + x_p b_i), where a_i = w_i cos_i and b_i = +-w_p sin_i belong to the
 // token and are formed once for the group's heads.
 template <typename T, typename TT, int NCH, int HPG, int PAIRS>
@@ -96,21 +85,29 @@ rope_kernel(const RopeParams P) {
         const int c = lane + GROUP * i;
         load_table<TT>(cos, c, P.rotary, P.wide_tables, 1.f, ca[i]);
         load_table<TT>(sin, c, P.rotary, P.wide_tables, 0.f, cb[i]);
-        float own[8];
+        float own[8], other[8];      // weights of the chunk's channels, and of their partners
         if (w && in[i]) {
             to_float(load_chunk<T>(w, c), own);
+            if (PAIRS == ROPE_CHUNK || PAIRS == ROPE_LANE) {
+                if (c * 8 < P.rotary) to_float(load_chunk<T>(w, c * 8 < half ? c + half / 8 : c - half / 8), other);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int ch = c * 8 + e;
+                    if (PAIRS == ROPE_INTERLEAVED) other[e] = own[e ^ 1];
+                    else other[e] = ch < P.rotary ? (float)w[ch < half ? ch + half : ch - half] : 0.f;
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) ca[i][e] *= own[e];
         }
+        if (c * 8 < P.rotary)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int ch = c * 8 + e;
-            if (ch < P.rotary) {
-                float sign;
-                const int q = rope_partner<PAIRS>(ch, half, sign);
-                cb[i][e] *= w ? sign * (float)w[q] : sign;
+            for (int e = 0; e < 8; ++e) {
+                const bool first = PAIRS == ROPE_INTERLEAVED ? (e & 1) == 0 : c * 8 + e < half;      // of its pair
+                const float f = w ? other[e] : 1.f;
+                cb[i][e] *= first ? -f : f;
             }
-        }
     }
     T* y0 = reinterpret_cast<T*>(S.y) + b * S.ys[0] + h0 * S.ys[1] + token * S.ys[2];
 #pragma unroll

@@ -25,29 +25,35 @@ constexpr int SA_PAD = 4;         // floats behind each row in shared memory: ro
 // (RPT + 4 16-byte loads for 16 RPT FMAs), for the weighted sums RPT rows x V / 16 channels.  A row's softmax
 // statistics stay with its 16 lanes, so the blocks only meet to exchange tiles.  fp32 products and sums throughout.
 // ---------------------------------------------------------------------------
-// rows k0 .. k0 + 63 of keys or values into shared memory as fp32; those from `len` on as 0, nothing of them is read
+// Rows k0 .. k0 + 63 of keys or values into shared memory as fp32; those from `len` on as 0, nothing of them is read.
+// A thread keeps its piece of the rows where the pieces divide the threads.
+template <typename F>
+__device__ __forceinline__ void sa_pieces(int pieces, F&& f) {
+    if (SA_THREADS % pieces == 0) {
+        const int c = threadIdx.x % pieces, step = SA_THREADS / pieces;
+#pragma unroll 4
+        for (int r = threadIdx.x / pieces; r < SA_KEYS; r += step) f(r, c);
+    } else {
+        for (int i = threadIdx.x; i < SA_KEYS * pieces; i += SA_THREADS) f(i / pieces, i % pieces);
+    }
+}
 __device__ __forceinline__ void sa_load_tile(float* dst, int ld, const float* src, long long stride, int k0, int len, int width) {
     const uint32_t d0 = (uint32_t)__cvta_generic_to_shared(dst);
-    const int pieces = width / 4;
-    for (int i = threadIdx.x; i < SA_KEYS * pieces; i += SA_THREADS) {
-        const int r = i / pieces, c = i - r * pieces;
+    sa_pieces(width / 4, [&](int r, int c) {
         const bool there = k0 + r < len;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d0 + (uint32_t)(r * ld + c * 4) * 4),
                      "l"(there ? src + (k0 + r) * stride + c * 4 : src), "r"(there ? 16 : 0) : "memory");
-    }
+    });
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 }
 __device__ __forceinline__ void sa_load_tile(float* dst, int ld, const __nv_bfloat16* src, long long stride, int k0, int len, int width) {
-    const int pieces = width / 8;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < SA_KEYS * pieces; i += SA_THREADS) {
-        const int r = i / pieces, c = i - r * pieces;
+    sa_pieces(width / 8, [&](int r, int c) {
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (k0 + r < len) to_float(load_chunk<__nv_bfloat16>(src + (k0 + r) * stride, c), f);
         float4* d = reinterpret_cast<float4*>(dst + r * ld + c * 8);
         d[0] = make_float4(f[0], f[1], f[2], f[3]);
         d[1] = make_float4(f[4], f[5], f[6], f[7]);
-    }
+    });
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 }
 template <int N>
@@ -213,6 +219,190 @@ shared_simt_kernel(const SharedAttn P) {
 }
 
 // ---------------------------------------------------------------------------
+// The same for few rows (8 or 16 a block), where shared memory's ports bound the kernel above: here a thread forms one
+// key's products with ALL rows (half of the channels each; the key is read once, the queries are broadcasts), a warp
+// then takes whole rows for their softmax, and for the weighted sums a warp takes 16 of the 64 keys and a lane four
+// channels of all rows.  The four warps' sums are added up once, at the end.
+// ---------------------------------------------------------------------------
+template <typename T, int ROWS, int NV, bool TAIL>
+__global__ void __launch_bounds__(SA_THREADS)
+shared_few_kernel(const SharedAttn P) {
+    extern __shared__ __align__(16) float sa_smem[];
+    const int ldk = P.dim + SA_PAD, ldv = P.vdim + SA_PAD;
+    float* s_q = sa_smem;                       // [ROWS][ldk]
+    float* s_k = s_q + ROWS * ldk;              // [SA_KEYS][ldk]
+    float* s_v = s_k + SA_KEYS * ldk;           // [SA_KEYS][ldv]
+    float* s_p = s_v + SA_KEYS * ldv;           // [SA_KEYS][ROWS + SA_PAD]: logits, then weights
+    constexpr int LDP = ROWS + SA_PAD;
+    __shared__ float s_alpha[ROWS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int row0 = blockIdx.x * ROWS, split = blockIdx.y;
+    const int item = blockIdx.z, h = item % P.n_kv, owner = item / P.n_kv;      // prompt, or branch of a tail
+    const int per = P.group * P.n_q;
+    const int n_rows = TAIL ? per : P.n_branches * per;
+    const int n_splits = TAIL ? P.tail_parts : P.prefix_parts;
+    const int len = TAIL ? shared_tail_len(P, owner) : shared_prefix_len(P, owner);
+    const T* gk = reinterpret_cast<const T*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
+    const T* gv = reinterpret_cast<const T*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
+    const long long ks = TAIL ? P.tks[2] : P.pks[2], vs = TAIL ? P.tvs[2] : P.pvs[2];
+    auto out_row = [&](int r) {
+        return TAIL ? (owner * P.n_kv + h) * per + r : shared_row(P, owner, h, r);
+    };
+    const int tiles = (len + SA_KEYS - 1) / SA_KEYS;
+    const int t0 = (int)((long long)split * tiles / n_splits), t1 = (int)((long long)(split + 1) * tiles / n_splits);
+    if (t0 < t1) sa_load_tile(s_k, ldk, gk, ks, t0 * SA_KEYS, len, P.dim);
+    const int kc = P.dim / 8;
+    for (int i = tid; i < ROWS * kc; i += SA_THREADS) {
+        const int r = i / kc, c = i - r * kc;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (row0 + r < n_rows)
+            to_float(load_chunk<T>(reinterpret_cast<const T*>(P.q) + shared_row_offset(P, out_row(row0 + r), P.qs), c), f);
+        float4* d = reinterpret_cast<float4*>(s_q + r * ldk + c * 8);
+        d[0] = make_float4(f[0], f[1], f[2], f[3]);
+        d[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    constexpr int WROWS = ROWS / 4;             // rows of a warp's softmax: warp, warp + 4, ...
+    float m[WROWS], l[WROWS], o[ROWS][NV][4];
+#pragma unroll
+    for (int a = 0; a < WROWS; ++a) {
+        m[a] = -CUDART_INF_F;
+        l[a] = 0.f;
+    }
+#pragma unroll
+    for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[a][c][e] = 0.f;
+    const int key = tid & 63, half = tid >> 6, d0 = half ? (P.dim / 8 + 1) / 2 * 8 : 0, d1 = half ? P.dim : (P.dim / 8 + 1) / 2 * 8;
+    for (int t = t0; t < t1; ++t) {
+        const int k0 = t * SA_KEYS;
+        sa_load_tile(s_v, ldv, gv, vs, k0, len, P.vdim);
+        sa_landed<1>();
+        __syncthreads();      // the keys are there (and the queries)
+        float s[ROWS];
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a) s[a] = 0.f;
+#pragma unroll 2
+        for (int d = d0; d < d1; d += 4) {
+            const float4 kk = *reinterpret_cast<const float4*>(s_k + key * ldk + d);
+#pragma unroll
+            for (int a = 0; a < ROWS; ++a) {
+                const float4 qq = *reinterpret_cast<const float4*>(s_q + a * ldk + d);
+                s[a] = __fmaf_rn(qq.x, kk.x, s[a]);
+                s[a] = __fmaf_rn(qq.y, kk.y, s[a]);
+                s[a] = __fmaf_rn(qq.z, kk.z, s[a]);
+                s[a] = __fmaf_rn(qq.w, kk.w, s[a]);
+            }
+        }
+        if (half)
+#pragma unroll
+            for (int a = 0; a < ROWS; a += 4) *reinterpret_cast<float4*>(s_p + key * LDP + a) = make_float4(s[a], s[a + 1], s[a + 2], s[a + 3]);
+        __syncthreads();      // the keys are used up, the second halves there
+        if (t + 1 < t1) sa_load_tile(s_k, ldk, gk, ks, k0 + SA_KEYS, len, P.dim);
+        if (!half)
+#pragma unroll
+            for (int a = 0; a < ROWS; a += 4) {
+                float4* at = reinterpret_cast<float4*>(s_p + key * LDP + a);
+                const float4 x = *at;
+                *at = make_float4(s[a] + x.x, s[a + 1] + x.y, s[a + 2] + x.z, s[a + 3] + x.w);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < WROWS; ++a) {
+            const int r = warp + 4 * a, seen = TAIL ? len - (P.n_q - 1 - (row0 + r) % P.n_q) : len;
+            float x[2], mx;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) x[j] = k0 + lane + 32 * j < seen ? s_p[(lane + 32 * j) * LDP + r] * P.scale_log2 : -CUDART_INF_F;
+            mx = fmaxf(x[0], x[1]);
+#pragma unroll
+            for (int w = 16; w >= 1; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+            const float nm = fmaxf(m[a], mx), base = nm > -CUDART_INF_F ? nm : 0.f;
+            const float alpha = exp2_approx(m[a] - base);
+            m[a] = nm;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                x[j] = exp2_approx(x[j] - base);
+                sum += x[j];
+                s_p[(lane + 32 * j) * LDP + r] = x[j];
+            }
+#pragma unroll
+            for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            l[a] = __fmaf_rn(l[a], alpha, sum);
+            if (lane == 0) s_alpha[r] = alpha;
+        }
+        if (t + 1 < t1) sa_landed<1>();
+        else sa_landed<0>();
+        __syncthreads();      // the values and the weights are there
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a) {
+            const float alpha = s_alpha[a];
+#pragma unroll
+            for (int c = 0; c < NV; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[a][c][e] *= alpha;
+        }
+#pragma unroll 2
+        for (int k = warp * (SA_KEYS / 4); k < (warp + 1) * (SA_KEYS / 4); ++k) {
+            float4 v[NV];
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int ch = lane * 4 + 128 * c;
+                v[c] = ch < P.vdim ? *reinterpret_cast<const float4*>(s_v + k * ldv + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int a = 0; a < ROWS; a += 4) {
+                const float4 p = *reinterpret_cast<const float4*>(s_p + k * LDP + a);
+                const float pp[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int c = 0; c < NV; ++c) {
+                        o[a + b][c][0] = __fmaf_rn(pp[b], v[c].x, o[a + b][c][0]);
+                        o[a + b][c][1] = __fmaf_rn(pp[b], v[c].y, o[a + b][c][1]);
+                        o[a + b][c][2] = __fmaf_rn(pp[b], v[c].z, o[a + b][c][2]);
+                        o[a + b][c][3] = __fmaf_rn(pp[b], v[c].w, o[a + b][c][3]);
+                    }
+            }
+        }
+        __syncthreads();      // the values are used up
+    }
+    // the warps' sums added up, in the tiles' place
+    float* s_o = s_k;         // [4][ROWS][ldv]
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int ch = lane * 4 + 128 * c;
+            if (ch < P.vdim) *reinterpret_cast<float4*>(s_o + (warp * ROWS + a) * ldv + ch) = make_float4(o[a][c][0], o[a][c][1], o[a][c][2], o[a][c][3]);
+        }
+    __syncthreads();
+    const int part = (TAIL ? P.prefix_parts : 0) + split;
+#pragma unroll
+    for (int a = 0; a < WROWS; ++a) {
+        const int r = warp + 4 * a;
+        if (row0 + r >= n_rows) continue;
+        const size_t at = (size_t)part * P.n_rows + out_row(row0 + r);
+        if (lane == 0) P.part_ml[at] = make_float2(m[a], l[a]);
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int ch = lane * 4 + 128 * c;
+            if (ch >= P.vdim) continue;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float4 x = *reinterpret_cast<const float4*>(s_o + (w * ROWS + r) * ldv + ch);
+                y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+            }
+            *reinterpret_cast<float4*>(P.part_o + at * P.vdim + ch) = y;
+        }
+    }
+    if (TAIL) grid_wait();      // so that who waits for this waits for the prefix too
+}
+
+// ---------------------------------------------------------------------------
 // The partials of an output row joined, by W warps: each weighs all parts (a lane a part), sums every W-th and the
 // first adds the sums up.  A few megabytes out of L2: bound by the round trips, so all loads of a round are issued at
 // once, and where a row has many parts four warps share them.
@@ -308,8 +498,13 @@ shared_merge_kernel(const SharedAttn P) {
 }
 
 template <typename T, int RPT, int NV, bool TAIL>
+static auto simt_kernel() {      // NV: 64 channels each of 16 lanes, or (few rows) 128 each of a warp
+    if constexpr (RPT <= 2) return shared_few_kernel<T, 8 * RPT, NV / 2, TAIL>;
+    else return shared_simt_kernel<T, RPT, NV, TAIL>;
+}
+template <typename T, int RPT, int NV, bool TAIL>
 static int launch_simt(const SharedAttn& P, bool chained, cudaStream_t s) {
-    auto kern = shared_simt_kernel<T, RPT, NV, TAIL>;
+    auto kern = simt_kernel<T, RPT, NV, TAIL>();
     const int per = P.group * P.n_q, rows = TAIL ? per : P.n_branches * per;
     const size_t smem = sizeof(float) * ((size_t)(8 * RPT + SA_KEYS) * (P.dim + SA_PAD) + (size_t)SA_KEYS * (P.vdim + SA_PAD) +
                                          (size_t)SA_KEYS * (8 * RPT + SA_PAD));

@@ -6,7 +6,6 @@ the arrays follow the reference's CUDAIndexer attributes (indexer/cuda.py:40-54)
 """
 from __future__ import annotations
 
-import copy
 import ctypes as C
 from dataclasses import dataclass
 from functools import lru_cache
@@ -140,17 +139,21 @@ class IndexState:
 
     def like(self, n_heads: int) -> "IndexState":
         """A state of the same shape for another number of heads; its arrays (and its status) are not filled."""
-        new = copy.copy(self)
-        new.n_heads = n_heads
+        new = object.__new__(type(self))
+        d = new.__dict__
+        d.update(self.__dict__)
+        d.pop("_tile_parents", None)
+        s = L.HiraIndexStruct.from_buffer_copy(self._struct)
         for name in self.ARRAYS + self.Q8_ARRAYS:
-            t = getattr(self, name)
+            t = d[name]
             if t is not None:
-                setattr(new, name, torch.empty((n_heads, *t.shape[1:]), dtype=t.dtype, device=t.device))
+                t = d[name] = t.new_empty((n_heads, *t.shape[1:]))
+                setattr(s, name, t.data_ptr())
+        s.n_heads = new.n_heads = n_heads
         new.status = torch.empty_like(self.status)
         new._append_bytes, new._append_ws = {}, (None, 0)
         new._streams = {L.current_stream(self.device)} if self.device.type == "cuda" else set()
-        new.__dict__.pop("_tile_parents", None)
-        new.refresh_struct()
+        new._struct, new._byref = s, C.byref(s)
         return new
 
     def state_dict(self) -> dict:

@@ -20,7 +20,6 @@ Differences by design:
 """
 from __future__ import annotations
 
-import copy
 from enum import Enum
 from typing import Optional
 
@@ -461,7 +460,8 @@ class CUDAIndexer(BaseIndexer):
         if n == 0:
             raise ValueError("no sequence picked")
         heads = self.num_heads // self.batch
-        new = copy.copy(self)
+        new = object.__new__(type(self))
+        new.__dict__.update(self.__dict__)
         new.state = st.like(n * heads)
         new.num_heads, new.batch = n * heads, n
         new._snapshot = new._scan_slots = new._searched = new._pending_append = new._pinned = new._tau_samples = None
