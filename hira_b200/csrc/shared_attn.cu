@@ -546,12 +546,13 @@ static int launch_simt_rows(const SharedAttn& P, bool chained, cudaStream_t s) {
     return launch_simt<T, 8, 2, TAIL>(P, chained, s);
 }
 
-// Splits of the keys: enough blocks for two an SM, none with fewer than two tiles of its own.
+// Splits of the keys: as many blocks as are resident at once (three an SM of those with few rows, else two), none with
+// fewer than two tiles.
 static int simt_splits(int rows, int items, int len, int vdim) {
     if (len <= 0) return 0;
     const int block_rows = simt_rows(rows, vdim), tiles = (len + SA_KEYS - 1) / SA_KEYS;
     const long long blocks = (long long)((rows + block_rows - 1) / block_rows) * items;
-    long long splits = (2 * SM_COUNT + blocks - 1) / blocks;
+    long long splits = (block_rows <= 16 ? 3 : 2) * SM_COUNT / blocks;
     if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
     if (splits > 64) splits = 64;
     return splits < 1 ? 1 : (int)splits;

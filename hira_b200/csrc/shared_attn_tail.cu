@@ -16,6 +16,7 @@ constexpr int TL_ROWS = 16;
 constexpr int TL_KEYS = 16;                     // keys a warp takes a step
 constexpr int TL_STEP = TL_WARPS * TL_KEYS;
 constexpr int TL_STAGES = 3;
+constexpr float TL_SLACK = 8.0f;
 constexpr int TL_FLIGHT = 8;                    // parts of a row on their way at once
 
 template <int HD>
@@ -44,6 +45,81 @@ __device__ __forceinline__ uint32_t tl_pack(float lo, float hi) {
     return d;
 }
 
+// A block's rows: the tail's sums (in shared memory, of each warp) and the prefix's n parts joined and written.  A warp
+// takes R rows at a time, a lane four channels of each.
+template <int HD, int R>
+__device__ __forceinline__ void tl_join(const SharedAttn& P, const float (*s_m)[TL_ROWS], const float (*s_l)[TL_ROWS], const float* s_o, int n,
+                                        int rows, int first_row) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = lane * 4;
+    for (int r0 = warp; r0 < rows; r0 += R * TL_WARPS) {
+        int row[R];
+        float base[R], w_t[R], l_t[R], L[R], wi[R];
+        float4 acc[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int r = min(r0 + k * TL_WARPS, rows - 1);
+            row[k] = first_row + r;
+            float m_t = -CUDART_INF_F;
+            l_t[k] = L[k] = 0.f;
+            for (int w = 0; w < TL_WARPS; ++w) m_t = fmaxf(m_t, s_m[w][r]);
+            for (int w = 0; w < TL_WARPS; ++w) l_t[k] += s_m[w][r] > -CUDART_INF_F ? s_l[w][r] * exp2_approx(s_m[w][r] - m_t) : s_l[w][r];
+            float M = m_t;
+            for (int i = lane; i < n; i += 32) M = fmaxf(M, P.part_ml[(size_t)i * P.n_rows + row[k]].x);
+#pragma unroll
+            for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+            base[k] = M > -CUDART_INF_F ? M : 0.f;
+            w_t[k] = m_t > -CUDART_INF_F ? exp2_approx(m_t - base[k]) : 0.f;
+            acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (ch < HD)
+                for (int w = 0; w < TL_WARPS; ++w) {
+                    const float4 x = *reinterpret_cast<const float4*>(s_o + (w * TL_ROWS + r) * HD + ch);
+                    acc[k].x += x.x; acc[k].y += x.y; acc[k].z += x.z; acc[k].w += x.w;
+                }
+            acc[k].x *= w_t[k]; acc[k].y *= w_t[k]; acc[k].z *= w_t[k]; acc[k].w *= w_t[k];
+        }
+        const float* src = P.part_o + (ch < P.vdim ? ch : 0);
+        for (int i0 = 0; i0 < n; i0 += 32) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const float2 ml = i0 + lane < n ? P.part_ml[(size_t)(i0 + lane) * P.n_rows + row[k]] : make_float2(-CUDART_INF_F, 0.f);
+                wi[k] = ml.x > -CUDART_INF_F ? exp2_approx(ml.x - base[k]) : 0.f;
+                // a NaN among a part's logits, which a maximum passes over, is in its sum (or its maximum)
+                L[k] += wi[k] > 0.f ? wi[k] * ml.y : ml.x != ml.x ? ml.x : ml.y != ml.y ? ml.y : 0.f;
+            }
+            const int count = min(n - i0, 32);
+            for (int j0 = 0; j0 < count; j0 += TL_FLIGHT) {
+                float4 x[R][TL_FLIGHT];
+#pragma unroll
+                for (int k = 0; k < R; ++k)
+#pragma unroll
+                    for (int j = 0; j < TL_FLIGHT; ++j)
+                        x[k][j] = *reinterpret_cast<const float4*>(src + ((size_t)min(i0 + j0 + j, n - 1) * P.n_rows + row[k]) * P.vdim);
+#pragma unroll
+                for (int k = 0; k < R; ++k)
+#pragma unroll
+                    for (int j = 0; j < TL_FLIGHT; ++j) {
+                        const float wj = __shfl_sync(0xffffffffu, wi[k], (j0 + j) & 31);
+                        if (j0 + j < count && wj != 0.f) {      // what a part without keys has there is not used
+                            acc[k].x = __fmaf_rn(wj, x[k][j].x, acc[k].x); acc[k].y = __fmaf_rn(wj, x[k][j].y, acc[k].y);
+                            acc[k].z = __fmaf_rn(wj, x[k][j].z, acc[k].z); acc[k].w = __fmaf_rn(wj, x[k][j].w, acc[k].w);
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+#pragma unroll
+            for (int w = 16; w >= 1; w >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], w);
+            L[k] += w_t[k] > 0.f ? w_t[k] * l_t[k] : l_t[k] != l_t[k] ? l_t[k] : 0.f;
+            if (ch < P.vdim && r0 + k * TL_WARPS < rows) {   // no key seen: 0 (a NaN stays one)
+                const float inv = L[k] == 0.f ? 0.f : 1.f / L[k];
+                const uint2 y = make_uint2(tl_pack(acc[k].x * inv, acc[k].y * inv), tl_pack(acc[k].z * inv, acc[k].w * inv));
+                *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + shared_row_offset(P, row[k], P.os) + ch) = y;
+            }
+        }
+    }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(32 * TL_WARPS, HD == 128 ? 2 : 3)
 shared_tail_kernel(const SharedAttn P) {
@@ -63,17 +139,27 @@ shared_tail_kernel(const SharedAttn P) {
     const int steps_all = (len + TL_STEP - 1) / TL_STEP;
     const int t0 = (int)((long long)split * steps_all / P.tail_parts), t1 = (int)((long long)(split + 1) * steps_all / P.tail_parts);
     const uint32_t ring = smem_u32(tl_smem) + warp * TL_STAGES * Lay::STAGE;
+    // A lane copies the same 16 bytes of every RPI-th of a step's keys and values.
+    constexpr int CH = HD / 8, RPI = 32 / CH, ITER = TL_KEYS / RPI;
+    const int lr = lane / CH, lc = lane % CH;
+    const uint32_t dst0 = ring + lr * Lay::ROW;
+    const bool in_k = lc * 8 < P.dim, in_v = lc * 8 < P.vdim;      // behind the row's channels: 0
     auto load = [&](int t, int stage) {
         const int k0 = t * TL_STEP + warp * TL_KEYS;
         if (t < t1 && k0 < len) {
-            constexpr int CH = HD / 8;
+            const __nv_bfloat16* src_k = gk + (k0 + lr) * P.tks[2] + lc * 8;
+            const __nv_bfloat16* src_v = gv + (k0 + lr) * P.tvs[2] + lc * 8;
+            const long long step_k = RPI * P.tks[2], step_v = RPI * P.tvs[2];
+            const uint32_t dst = dst0 + stage * Lay::STAGE;
+            const bool whole = k0 + TL_KEYS <= len;
 #pragma unroll
-            for (int i = lane; i < TL_KEYS * CH; i += 32) {
-                const int r = i / CH, c = i % CH;
-                const uint32_t dst = ring + stage * Lay::STAGE + r * Lay::ROW + ((c ^ (r & 7)) << 4);
-                const bool row = k0 + r < len;       // behind the last key, and behind the row's channels: 0
-                tl_cp16(dst, row && c * 8 < P.dim ? gk + (k0 + r) * P.tks[2] + c * 8 : gk, row && c * 8 < P.dim);
-                tl_cp16(dst + TL_KEYS * Lay::ROW, row && c * 8 < P.vdim ? gv + (k0 + r) * P.tvs[2] + c * 8 : gv, row && c * 8 < P.vdim);
+            for (int i = 0; i < ITER; ++i) {
+                const uint32_t at = dst + i * RPI * Lay::ROW + ((lc ^ ((lr + i * RPI) & 7)) << 4);
+                const bool row = whole || k0 + lr + i * RPI < len;       // behind the last key: 0
+                tl_cp16(at, row && in_k ? src_k : gk, row && in_k);
+                tl_cp16(at + TL_KEYS * Lay::ROW, row && in_v ? src_v : gv, row && in_v);
+                src_k += step_k;
+                src_v += step_v;
             }
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
@@ -131,40 +217,49 @@ shared_tail_kernel(const SharedAttn P) {
                     tl_mma(s[n], q[2 * k], kk[0], kk[1]);
                     tl_mma(s[n], q[2 * k + 1], kk[2], kk[3]);
                 }
-            float f[2];
+            // The reference maximum of a row moves only when a step exceeds it by 2^8, as in the prefix's kernel.
+            float mx[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float mx = -CUDART_INF_F;
+                mx[j] = -CUDART_INF_F;
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float& x = s[n][2 * j + e];
                         x = k0 + n * 8 + tig * 2 + e < seen[j] ? x * P.scale_log2 : -CUDART_INF_F;
-                        mx = fmaxf(mx, x);
+                        mx[j] = fmaxf(mx[j], x);
                     }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float nm = fmaxf(m[j], mx), base = nm > -CUDART_INF_F ? nm : 0.f;
-                f[j] = exp2_approx(m[j] - base);
-                m[j] = nm;
-                float sum = 0.f;
+                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
+                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
+            }
+            if (__any_sync(0xffffffffu, mx[0] > m[0] + TL_SLACK || mx[1] > m[1] + TL_SLACK)) {
+                float f[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const bool rise = mx[j] > m[j] + TL_SLACK;       // from -inf on: always, unless the step is -inf too
+                    f[j] = rise ? exp2_approx(m[j] - mx[j]) : 1.f;
+                    if (rise) m[j] = mx[j];
+                    l[j] *= f[j];
+                }
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n) {
+                    o[n][0] *= f[0]; o[n][1] *= f[0];
+                    o[n][2] *= f[1]; o[n][3] *= f[1];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float base = m[j] > -CUDART_INF_F ? m[j] : 0.f;
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float& x = s[n][2 * j + e];
                         x = exp2_approx(x - base);
-                        sum += x;
+                        l[j] += x;      // this lane's keys; the four lanes of a row are added at the end
                     }
-                l[j] = __fmaf_rn(l[j], f[j], sum);      // this lane's keys; the four lanes of a row are added at the end
             }
-            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f))
-#pragma unroll
-                for (int n = 0; n < HD / 8; ++n) {
-                    o[n][0] *= f[0]; o[n][1] *= f[0];
-                    o[n][2] *= f[1]; o[n][3] *= f[1];
-                }
             const uint32_t p[4] = {tl_pack(s[0][0], s[0][1]), tl_pack(s[0][2], s[0][3]), tl_pack(s[1][0], s[1][1]), tl_pack(s[1][2], s[1][3])};
 #pragma unroll
             for (int n = 0; n < HD / 16; ++n) {
@@ -201,79 +296,13 @@ shared_tail_kernel(const SharedAttn P) {
     }
     __syncthreads();
     if (P.fused) {
-        // The tail's only part: what the merge would do with it and the prefix's parts, done here.  A warp takes a row, a
-        // lane four channels.
-        const int rows = min(per - row0, TL_ROWS), ch = lane * 4;
+        // the tail's only part: what the merge would do with it and the prefix's parts, done here
+        const int rows = min(per - row0, TL_ROWS);
         const int item = b / P.n_branches * P.n_kv + h;
         const int n = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0;
         grid_wait();             // the prefix's parts are there
-        for (int r0 = warp; r0 < rows; r0 += 2 * TL_WARPS) {      // two rows at a time, for their loads to overlap
-            int row[2];
-            float base[2], w_t[2], l_t[2], L[2], wi[2];
-            float4 acc[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int r = min(r0 + k * TL_WARPS, rows - 1);
-                row[k] = out_row0 + row0 + r;
-                float m_t = -CUDART_INF_F;
-                l_t[k] = L[k] = 0.f;
-                for (int w = 0; w < TL_WARPS; ++w) m_t = fmaxf(m_t, s_m[w][r]);
-                for (int w = 0; w < TL_WARPS; ++w) l_t[k] += s_m[w][r] > -CUDART_INF_F ? s_l[w][r] * exp2_approx(s_m[w][r] - m_t) : s_l[w][r];
-                float M = m_t;
-                for (int i = lane; i < n; i += 32) M = fmaxf(M, P.part_ml[(size_t)i * P.n_rows + row[k]].x);
-#pragma unroll
-                for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-                base[k] = M > -CUDART_INF_F ? M : 0.f;
-                w_t[k] = m_t > -CUDART_INF_F ? exp2_approx(m_t - base[k]) : 0.f;
-                acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (ch < HD)
-                    for (int w = 0; w < TL_WARPS; ++w) {
-                        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * TL_ROWS + r) * HD + ch);
-                        acc[k].x += x.x; acc[k].y += x.y; acc[k].z += x.z; acc[k].w += x.w;
-                    }
-                acc[k].x *= w_t[k]; acc[k].y *= w_t[k]; acc[k].z *= w_t[k]; acc[k].w *= w_t[k];
-            }
-            const float* src = P.part_o + (ch < P.vdim ? ch : 0);
-            for (int i0 = 0; i0 < n; i0 += 32) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float2 ml = i0 + lane < n ? P.part_ml[(size_t)(i0 + lane) * P.n_rows + row[k]] : make_float2(-CUDART_INF_F, 0.f);
-                    wi[k] = ml.x > -CUDART_INF_F ? exp2_approx(ml.x - base[k]) : 0.f;
-                    // a NaN among a part's logits, which a maximum passes over, is in its sum (or its maximum)
-                    L[k] += wi[k] > 0.f ? wi[k] * ml.y : ml.x != ml.x ? ml.x : ml.y != ml.y ? ml.y : 0.f;
-                }
-                const int count = min(n - i0, 32);
-                for (int j0 = 0; j0 < count; j0 += TL_FLIGHT) {
-                    float4 x[2][TL_FLIGHT];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int j = 0; j < TL_FLIGHT; ++j)
-                            x[k][j] = *reinterpret_cast<const float4*>(src + ((size_t)min(i0 + j0 + j, n - 1) * P.n_rows + row[k]) * P.vdim);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int j = 0; j < TL_FLIGHT; ++j) {
-                            const float wj = __shfl_sync(0xffffffffu, wi[k], (j0 + j) & 31);
-                            if (j0 + j < count && wj != 0.f) {      // what a part without keys has there is not used
-                                acc[k].x = __fmaf_rn(wj, x[k][j].x, acc[k].x); acc[k].y = __fmaf_rn(wj, x[k][j].y, acc[k].y);
-                                acc[k].z = __fmaf_rn(wj, x[k][j].z, acc[k].z); acc[k].w = __fmaf_rn(wj, x[k][j].w, acc[k].w);
-                            }
-                        }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int w = 16; w >= 1; w >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], w);
-                L[k] += w_t[k] > 0.f ? w_t[k] * l_t[k] : l_t[k] != l_t[k] ? l_t[k] : 0.f;
-                if (ch < P.vdim && r0 + k * TL_WARPS < rows) {   // no key seen: 0 (a NaN stays one)
-                    const float inv = L[k] == 0.f ? 0.f : 1.f / L[k];
-                    const uint2 y = make_uint2(tl_pack(acc[k].x * inv, acc[k].y * inv), tl_pack(acc[k].z * inv, acc[k].w * inv));
-                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + shared_row_offset(P, row[k], P.os) + ch) = y;
-                }
-            }
-        }
+        if (rows <= TL_WARPS) tl_join<HD, 1>(P, s_m, s_l, s_o, n, rows, out_row0 + row0);
+        else tl_join<HD, 2>(P, s_m, s_l, s_o, n, rows, out_row0 + row0);
         return;
     }
     const size_t part = (size_t)(P.prefix_parts + split) * P.n_rows;
