@@ -238,7 +238,7 @@ def current_stream(device=None) -> int:
 def on_device(index: int, call, *args):
     """`call(*args, stream)` with the device `index` current and its current stream; the device is switched only where
     it is not current already."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         return call(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return call(*args, torch._C._cuda_getCurrentRawStream(index))

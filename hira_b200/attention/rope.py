@@ -19,8 +19,8 @@ _TYPES = (torch.float32, torch.bfloat16)
 _plans = {}
 
 
-def _layout(t: Optional[torch.Tensor]):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+def _layout(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype, t.get_device()
 
 
 def _check_apart(o: torch.Tensor, x: torch.Tensor, other: torch.Tensor, name: str):
@@ -57,8 +57,10 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     if torch.is_grad_enabled():
         refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
     # calls of a layout that has been checked before go straight to the library
-    layout = (_layout(query), _layout(key), _layout(cos), _layout(sin), _layout(q_weight), _layout(k_weight), _layout(out_q), _layout(out_k),
-              eps, interleaved)
+    layout = (query.shape, query.stride(), query.dtype, query.get_device(), key.shape, key.stride(), key.dtype, key.get_device(),
+              cos.shape, cos.stride(), cos.dtype, cos.get_device(), sin.shape, sin.stride(), sin.dtype, sin.get_device(),
+              None if q_weight is None else _layout(q_weight), None if k_weight is None else _layout(k_weight),
+              None if out_q is None else _layout(out_q), None if out_k is None else _layout(out_k), eps, interleaved)
     plan = _plans.get(layout)
     if plan is not None:
         if out_q is not None:

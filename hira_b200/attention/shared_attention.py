@@ -72,8 +72,9 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     if out is None and (tail_keys is None or tail_values is not None and tail_keys.shape[:-1] == tail_values.shape[:-1]) \
             and (prefix_lens is None or torch.is_tensor(prefix_lens) and prefix_lens.is_cuda) \
             and (tail_lens is None or torch.is_tensor(tail_lens) and tail_lens.is_cuda):
-        layout = (_layout(query), _layout(prefix_keys), _layout(prefix_values), _tail_layout(tail_keys), _tail_layout(tail_values),
-                  _layout(prefix_lens), _layout(tail_lens), scaling)
+        layout = (query.shape, query.stride(), query.dtype, query.get_device(), prefix_keys.shape, prefix_keys.stride(), prefix_keys.dtype,
+                  prefix_keys.get_device(), prefix_values.shape, prefix_values.stride(), prefix_values.dtype, prefix_values.get_device(),
+                  _tail_layout(tail_keys), _tail_layout(tail_values), _layout(prefix_lens), _layout(tail_lens), scaling)
         plan = _plans.get(layout)
         if plan is not None:
             done = plan(query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
@@ -186,6 +187,7 @@ class SharedPrompt:
                 t[:, :, :self._len] = old[i][:, :, :self._len]
             new.append(t)
         self._k, self._v = new
+        self._moves = S.RowMoves([(self._k, self._k), (self._v, self._v)])
 
     @torch.no_grad()
     def append(self, keys: torch.Tensor, values: torch.Tensor):
@@ -225,7 +227,7 @@ class SharedPrompt:
         if idx.numel() != self.batch:
             raise ValueError(f"{idx.numel()} indices for {self.batch} sequences")
         if self._len:
-            S.gather_rows([(self._k, self._k), (self._v, self._v)], idx, self._len, self.status)
+            S.gather_rows(self._moves, idx, self._len, self.status)
         return self
 
     def select(self, indices) -> "SharedPrompt":
@@ -237,7 +239,7 @@ class SharedPrompt:
         new = SharedPrompt(self.prefix_keys, self.prefix_values, n // self.prefix_keys.shape[0], max_tail=self._k.shape[2])
         new.prefix_lens, new._len = self.prefix_lens, self._len
         if self._len:
-            S.gather_rows([(self._k, new._k), (self._v, new._v)], idx, self._len, new.status)
+            S.gather_rows(S.RowMoves([(self._k, new._k), (self._v, new._v)]), idx, self._len, new.status)
         return new
 
     def check_status(self):

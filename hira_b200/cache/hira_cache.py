@@ -176,7 +176,7 @@ class HiraCacheLayer(CacheLayerMixin):
         idx = S.check_picks(beam_idx, self.B, self._queue_k.device)
         self.indexer.reorder(idx)
         if self.queued_len:
-            S.gather_rows([(self._queue_k, self._queue_k), (self._queue_v, self._queue_v)], idx, self.queued_len)
+            S.gather_rows(S.RowMoves([(self._queue_k, self._queue_k), (self._queue_v, self._queue_v)]), idx, self.queued_len)
 
     def batch_select_indices(self, indices):
         """Keeps the picked sequences, in their order; one that is picked several times is forked."""
@@ -191,7 +191,7 @@ class HiraCacheLayer(CacheLayerMixin):
         old, self.B, n = (self._queue_k, self._queue_v), idx.numel(), self.queued_len
         self._queue_k, self._queue_v = (torch.empty((self.B, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in old)
         if n:
-            S.gather_rows(list(zip(old, (self._queue_k, self._queue_v))), idx, n)
+            S.gather_rows(S.RowMoves(list(zip(old, (self._queue_k, self._queue_v)))), idx, n)
         self.queued_keys, self.queued_values = self._queue_k[:, :, :n], self._queue_v[:, :, :n]
 
     def batch_repeat_interleave(self, repeats: int):

@@ -705,20 +705,32 @@ def check_picks(indices, n: int, device) -> torch.Tensor:
     return t.to(device=device, dtype=torch.int64).contiguous()
 
 
-def gather_rows(pairs, index: torch.Tensor, used_rows: int, status: Optional[torch.Tensor] = None):
-    """hira_gather of the first `used_rows` rows of (source, destination) tensors (B, H, rows, D) whose rows are
-    contiguous; source and destination the same tensor: in place."""
-    lib = L.load()
-    items = (L.HiraGatherItemStruct * len(pairs))()
-    for it, (src, dst) in zip(items, pairs):
-        e = src.element_size()
-        it.src, it.dst, it.n_seg = src.data_ptr(), dst.data_ptr(), src.shape[1]
-        it.src_seq_stride, it.src_seg_stride = src.stride(0) * e, src.stride(1) * e
-        it.dst_seq_stride, it.dst_seg_stride = dst.stride(0) * e, dst.stride(1) * e
-        it.bytes = it.bytes_filled = used_rows * src.shape[3] * e
-    src, dst = pairs[0]
-    L.check(L.on_device(src.get_device(), lib.hira_gather, items, len(pairs), L.ptr(index), src.shape[0], index.numel(),
-                        1 if src is dst else 0, L.ptr(status)), "hira_gather")
+class RowMoves:
+    """What hira_gather is told about (source, destination) tensors (B, H, rows, D) whose rows are contiguous; source and
+    destination the same tensor: in place."""
+
+    def __init__(self, pairs):
+        src, dst = pairs[0]
+        self.pairs, self.index, self.n_src, self.in_place = pairs, src.get_device(), src.shape[0], int(src is dst)
+        self.items = (L.HiraGatherItemStruct * len(pairs))()
+        self.row_bytes = []
+        for it, (src, dst) in zip(self.items, pairs):
+            e = src.element_size()
+            it.src, it.dst, it.n_seg = src.data_ptr(), dst.data_ptr(), src.shape[1]
+            it.src_seq_stride, it.src_seg_stride = src.stride(0) * e, src.stride(1) * e
+            it.dst_seq_stride, it.dst_seg_stride = dst.stride(0) * e, dst.stride(1) * e
+            self.row_bytes.append(src.shape[3] * e)
+
+
+def gather_rows(moves: RowMoves, index: torch.Tensor, used_rows: int, status: Optional[torch.Tensor] = None):
+    """hira_gather of the first `used_rows` rows."""
+    items = type(moves.items).from_buffer_copy(moves.items)      # one of its own for every call
+    for it, row in zip(items, moves.row_bytes):
+        it.bytes = it.bytes_filled = used_rows * row
+    rc = L.on_device(moves.index, L.load().hira_gather, items, len(items), index.data_ptr(), moves.n_src, index.numel(), moves.in_place,
+                     L.ptr(status))
+    if rc:
+        L.check(rc, "hira_gather")
 
 
 def _with_q8(st: IndexState):

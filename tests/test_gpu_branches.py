@@ -244,12 +244,12 @@ def test_rows_gathered_into_other_memory_and_in_place(picks, rows, dim, dtype):
     src = torch.randn((n, h, cap, dim), generator=gen).to(dtype).cuda()
     idx = torch.tensor(picks, device="cuda")
     dst = torch.full((len(picks), h, cap, dim), 7.0, dtype=dtype, device="cuda")
-    S.gather_rows([(src, dst)], idx, used)
+    S.gather_rows(S.RowMoves([(src, dst)]), idx, used)
     assert torch.equal(dst[:, :, :used], src[idx][:, :, :used]) and (dst[:, :, used:] == 7).all()
     full = torch.cat([idx, torch.arange(len(picks), n, device="cuda")])
     want = src.clone()
     want[:, :, :used] = src[full][:, :, :used]
-    S.gather_rows([(src, src)], full, used)
+    S.gather_rows(S.RowMoves([(src, src)]), full, used)
     assert torch.equal(src, want)
 
 
@@ -259,14 +259,14 @@ def test_many_sequences_permuted_in_place(n):
     src = torch.randn((n, 2, 9, 8), generator=gen).cuda()
     for idx in (torch.randperm(n, generator=gen), torch.randint(n, (n,), generator=gen), torch.roll(torch.arange(n), 1)):
         want = src[idx.cuda()].clone()
-        S.gather_rows([(src, src)], idx.cuda(), 9)
+        S.gather_rows(S.RowMoves([(src, src)]), idx.cuda(), 9)
         assert torch.equal(src, want)
 
 
 def test_a_sequence_that_does_not_exist_changes_nothing_and_is_reported():
     src = torch.randn((4, 2, 8, 16), device="cuda")
     keep, status = src.clone(), torch.zeros(1, dtype=torch.int32, device="cuda")
-    S.gather_rows([(src, src)], torch.tensor([1, 4, -1, 0], device="cuda"), 8, status)
+    S.gather_rows(S.RowMoves([(src, src)]), torch.tensor([1, 4, -1, 0], device="cuda"), 8, status)
     assert torch.equal(src, keep[[1, 1, 2, 0]]) and int(status) == 8
     prompt = SharedPrompt(keep[:1], keep[:1], 4, max_tail=8).append(keep, keep)
     prompt.check_status()
