@@ -14,6 +14,7 @@ present) attends densely over the prompt; a decode step
 """
 from __future__ import annotations
 
+import weakref
 from typing import Optional
 
 import torch
@@ -46,6 +47,10 @@ def _samples_for(indexer, sample_size: int) -> torch.Tensor:
     slots = r.topk(s, dim=1).indices                              # (H, s)
     rows = st.children.gather(1, slots.unsqueeze(-1).expand(-1, -1, st.dim)).contiguous()
     indexer._tau_samples = (st, rows)
+    # all that are still in use follow their sequences when those are reordered
+    if cached is None or cached[0] is not st:
+        indexer._tau_drawn = []
+    indexer._tau_drawn.append(weakref.ref(rows))
     return rows
 
 

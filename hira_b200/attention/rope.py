@@ -67,6 +67,8 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
             _check_apart(out_q, query, key, "out_q")
         if out_k is not None:
             _check_apart(out_k, key, query, "out_k")
+            if out_q is not None and out_q.data_ptr() == out_k.data_ptr() and out_q.numel():
+                raise ValueError("out_q and out_k are the same memory")
         done = plan(query, key, cos, sin, q_weight, k_weight, out_q, out_k)
         if done is not None:
             return done
@@ -99,6 +101,8 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
         if o.shape != x.shape or o.dtype != x.dtype or not S.writable_rows(o):
             raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype} with aligned contiguous rows")
         _check_apart(o, x, key if x is query else query, name)
+    if out_q is not None and out_k is not None and out_q.numel() and out_q.data_ptr() == out_k.data_ptr():
+        raise ValueError("out_q and out_k are the same memory")
     if not query.is_cuda:
         raise ValueError("hira_qk_norm_rope needs CUDA tensors (there is no CPU fallback)")
     args = (S.with_rows(query), S.with_rows(key), cos, sin, *(None if w is None else S.aligned(w.contiguous()) for w in (q_weight, k_weight)))

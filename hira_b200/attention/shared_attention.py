@@ -62,22 +62,22 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     whatever it holds).  On the host they are checked; on the device they are cut to 0..L and 0..T.  A query that
     sees no key at all gives 0.
 
-    fp32 or bf16, all of one type; D and V multiples of 8 up to 256.  fp32 is computed in fp32; bf16 with fp32
+    fp32 or bf16, all of one type; D and V multiples of 8 up to 256; B * H_kv up to 65,535.  fp32 is computed in fp32; bf16 with fp32
     sums and statistics.  Rows have to be contiguous and 16-byte aligned: what is not is copied first.  `out` has
     to be so.  No backward pass.  A key hidden from one query token but not from another has to be finite."""
     if torch.is_grad_enabled():
         refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
     # calls of a layout that has been checked before go straight to the library
     layout = None
-    if out is None and (tail_keys is None or tail_values is not None and tail_keys.shape[:-1] == tail_values.shape[:-1]) \
+    if (tail_keys is None or tail_values is not None and tail_keys.shape[:-1] == tail_values.shape[:-1]) \
             and (prefix_lens is None or torch.is_tensor(prefix_lens) and prefix_lens.is_cuda) \
             and (tail_lens is None or torch.is_tensor(tail_lens) and tail_lens.is_cuda):
         layout = (query.shape, query.stride(), query.dtype, query.get_device(), prefix_keys.shape, prefix_keys.stride(), prefix_keys.dtype,
                   prefix_keys.get_device(), prefix_values.shape, prefix_values.stride(), prefix_values.dtype, prefix_values.get_device(),
-                  _tail_layout(tail_keys), _tail_layout(tail_values), _layout(prefix_lens), _layout(tail_lens), scaling)
+                  _tail_layout(tail_keys), _tail_layout(tail_values), _layout(prefix_lens), _layout(tail_lens), _layout(out), scaling)
         plan = _plans.get(layout)
         if plan is not None:
-            done = plan(query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
+            done = plan(query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens, out)
             if done is not None:
                 return done
     if (tail_keys is None) != (tail_values is None):
@@ -127,6 +127,13 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     if layout is not None and all(a is b for a, b in zip(args, given)):
         S.remember(_plans, layout, plan)
     return plan(*args, out)
+
+
+def _keep(*tensors):
+    """For tensors that may be dropped while the current stream still reads them, another stream's among them."""
+    for t in tensors:
+        if t.is_cuda:
+            t.record_stream(torch.cuda.current_stream(t.device))
 
 
 class SharedPrompt:
@@ -185,6 +192,7 @@ class SharedPrompt:
             t = torch.empty((self.batch, like.shape[1], rows, like.shape[3]), dtype=like.dtype, device=like.device)
             if old is not None:
                 t[:, :, :self._len] = old[i][:, :, :self._len]
+                _keep(old[i])
             new.append(t)
         self._k, self._v = new
         self._moves = S.RowMoves([(self._k, self._k), (self._v, self._v)])
@@ -240,6 +248,7 @@ class SharedPrompt:
         new.prefix_lens, new._len = self.prefix_lens, self._len
         if self._len:
             S.gather_rows(S.RowMoves([(self._k, new._k), (self._v, new._v)]), idx, self._len, new.status)
+            _keep(self._k, self._v)
         return new
 
     def check_status(self):

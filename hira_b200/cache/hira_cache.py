@@ -192,6 +192,8 @@ class HiraCacheLayer(CacheLayerMixin):
         self._queue_k, self._queue_v = (torch.empty((self.B, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in old)
         if n:
             S.gather_rows(S.RowMoves(list(zip(old, (self._queue_k, self._queue_v)))), idx, n)
+            for t in old:         # dropped now, and perhaps another stream's
+                t.record_stream(torch.cuda.current_stream(t.device))
         self.queued_keys, self.queued_values = self._queue_k[:, :, :n], self._queue_v[:, :, :n]
 
     def batch_repeat_interleave(self, repeats: int):

@@ -341,7 +341,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
         const uint32_t my_s = tm_s + w * ST_KEYS + lanes, my_o = tm_o + w * HD + lanes;
         const bool warp_used = row0 + (warp & 3) * 32 < n_rows;          // rows behind the last: nothing to compute
         const int row = row0 + t;
-        const float scale = fabsf(P.scale_log2);
+        const float scale = fmaxf(fabsf(P.scale_log2), 1.2e-38f);        // never 0, which a masked score's -inf would turn into NaN
         const uint32_t flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;     // a negative scale turns the queries round
         uint32_t base = 0, segs = 0, n_s = 0, n_o[2] = {0, 0};
         bool ok = true;
@@ -546,13 +546,13 @@ static bool st_make_map(CUtensorMap* map, const void* base, int width, const Sha
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Strides that a tensor map takes: forward, and below 2^40 bytes.
+// Strides that a tensor map takes: forward, rows that do not overlap, and below 2^40 bytes.
 bool shared_tc_supported(const SharedAttn& P, int dtype) {
     if (dtype != HIRA_BF16 || P.prefix_len == 0 || P.dim > 128 || P.vdim > 128 || (P.dim > 64) != (P.vdim > 64)) return false;
     const int n[3] = {P.n_prompts, P.n_kv, P.prefix_len};
     for (int i = 0; i < 3; ++i)
         if (n[i] > 1 && (P.pks[i] < 1 || P.pvs[i] < 1 || P.pks[i] >= (1ll << 39) || P.pvs[i] >= (1ll << 39))) return false;
-    return true;
+    return P.prefix_len == 1 || (P.pks[2] >= P.dim && P.pvs[2] >= P.vdim);
 }
 
 void shared_tc_plan(SharedAttn& P) {

@@ -446,8 +446,13 @@ class CUDAIndexer(BaseIndexer):
         if self._scan_pending:
             self._scan_slots.fill_(-1)    # that scan was of other sequences
             self._scan_pending = False
-        drawn = getattr(self, "_tau_samples", None)
-        S.gather_index(st, st, idx, self.batch, drawn[1] if drawn is not None and drawn[0] is st else None)
+        self._searched_fresh = False      # an update on a side stream has to wait for this, not for the search before it
+        # rows that the threshold is found from, each set of them that somebody still holds
+        drawn = [rows for rows in (ref() for ref in getattr(self, "_tau_drawn", ())) if rows is not None]
+        S.gather_index(st, st, idx, self.batch, drawn[0] if drawn else None)
+        for rows in drawn[1:]:
+            rows = rows.view(self.batch, -1, *rows.shape[1:])
+            S.gather_rows(S.RowMoves([(rows, rows)]), idx, rows.shape[2])
         return self
 
     def select(self, indices) -> "CUDAIndexer":
@@ -465,8 +470,10 @@ class CUDAIndexer(BaseIndexer):
         new.state = st.like(n * heads)
         new.num_heads, new.batch = n * heads, n
         new._snapshot = new._scan_slots = new._searched = new._pending_append = new._pinned = new._tau_samples = None
+        new._tau_drawn = []
         new._scan_pending = new._searched_fresh = False
         S.gather_index(st, new.state, idx, self.batch)
+        st.used_on(torch.cuda.current_stream(st.device))     # the caller may drop this one right away
         return new
 
     def _settled(self) -> S.IndexState:

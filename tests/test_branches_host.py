@@ -65,6 +65,9 @@ def test_rotation_refuses_types_and_outputs():
     buf = _t(2, 6, 5, 64)
     with pytest.raises(ValueError, match="apart"):       # one row off: rows would be overwritten before they are read
         hira_qk_norm_rope(buf[:, :4, :4], buf[:, 4:, :4], c, c, out_q=buf[:, :4, 1:])
+    same = _t(2, 4, 4, 64)
+    with pytest.raises(ValueError, match="same memory"):
+        hira_qk_norm_rope(q, k, c, c, out_q=same, out_k=same[:, :2])
     with pytest.raises(ValueError, match="query is"):
         hira_qk_norm_rope(q, k.float(), c, c)
     with pytest.raises(ValueError, match="no backward"):

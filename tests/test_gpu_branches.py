@@ -46,7 +46,7 @@ def _exact(q, pk, pv, tk, tv, plens=None, tlens=None, scaling=None):
                 o, mean = probs @ w, probs @ w.abs()
                 # a logit: d products summed in 32 bits (2^-22 a step where the tensor cores cut instead of rounding), times
                 # the scale and log2(e), less the maximum, and the exponential itself (2^-22); numerator and denominator
-                logit = scaling * (x.abs() @ k.abs().T).amax(-1, keepdim=True)
+                logit = abs(scaling) * (x.abs() @ k.abs().T).amax(-1, keepdim=True)
                 off = 2 * (logit * (d + 8) * 2.0 ** -22 + 2.0 ** -21)
                 # sums over the keys in 32 bits; with bf16 each weight is rounded once more; the output once
                 # (and its exponential may be a polynomial's, 7.5e-5 off, in numerator and denominator)
@@ -157,6 +157,51 @@ def test_layouts_strides_and_out(dtype):
     assert hira_shared_attention(q, pk, pv, tk, tv, out=out.transpose(1, 2)).data_ptr() == out.data_ptr()
     assert torch.equal(out.transpose(1, 2), base)
     _check(hira_shared_attention(q, pk, pv, tk, tv, scaling=0.7), _exact(q, pk, pv, tk, tv, scaling=0.7))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scaling", [-0.11, 0.0, 1e-4])
+def test_scalings_of_any_sign(dtype, scaling):
+    t = _qkv(1, 3, 2, 2, 2, 128, 128, 333, 70, dtype, seed=21)
+    _check(hira_shared_attention(*t, scaling=scaling), _exact(*t, scaling=scaling))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_overlap_and_tails_of_one_for_all(dtype):
+    gen = torch.Generator().manual_seed(22)
+    line = torch.randn(8 * 300 + 128, generator=gen).to(dtype).cuda()
+    keys = line.as_strided((1, 2, 200, 64), (0, 8 * 50, 8, 1))             # windows of one line
+    q, _, pv, tk, tv = _qkv(1, 4, 2, 2, 1, 64, 64, 200, 9, dtype, seed=22)
+    tk, tv = tk[:1].expand(4, -1, -1, -1), tv[:1].expand(4, -1, -1, -1)
+    _check(hira_shared_attention(q, keys, pv, tk, tv), _exact(q, keys.contiguous(), pv, tk.contiguous(), tv.contiguous()))
+
+
+def test_tails_of_every_length_through_one_layout():
+    """Calls of one layout with a tail that grows, a buffer of one row and one of many, and an `out` of the caller's."""
+    q, pk, pv, tk, tv = _qkv(1, 3, 2, 2, 1, 128, 128, 200, 130, torch.bfloat16, seed=23)
+    for cap in (1, 2, 130):
+        bk, bv = tk[:, :, :cap].contiguous(), tv[:, :, :cap].contiguous()
+        for n in [x for x in (0, 1, 2, 3, 63, 64, 65, 128, 130) if x <= cap]:
+            want = _exact(q, pk, pv, bk[:, :, :n] if n else None, bv[:, :, :n] if n else None)
+            _check(hira_shared_attention(q, pk, pv, bk[:, :, :n], bv[:, :, :n]), want)
+            out = torch.full((3, 1, 4, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
+            for _ in range(2):
+                hira_shared_attention(q, pk, pv, bk[:, :, :n], bv[:, :, :n], out=out.transpose(1, 2))
+            _check(out.transpose(1, 2), want)
+
+
+def test_many_calls_at_once_on_two_streams():
+    cases = [(_qkv(2, 5, 2, 4, 1, 128, 128, 700 + 13 * i, 33 + i, torch.bfloat16, seed=30 + i)) for i in range(6)]
+    want = [hira_shared_attention(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for rounds in range(5):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append((i, hira_shared_attention(*c)))
+    torch.cuda.synchronize()
+    assert all(bool((x == want[i]).all()) for i, x in got)
 
 
 def test_large_logits_of_either_sign():
@@ -354,6 +399,48 @@ def test_reordered_index_attends_as_its_new_sequences(depth, picks):
         ix.update(k[:, :, :1], v[:, :, :1], scanned=True)
     ix.update(k[:, :, :1], v[:, :, :1])
     ix.check_status()
+
+
+def test_every_set_of_samples_follows_its_sequences():
+    from hira_b200.attention.hira_attention import _samples_for
+    ix, k, v = _index(4, 2, 500, 64, torch.bfloat16, 3)
+    sets = [_samples_for(ix, s) for s in (32, 64, 100)]
+    before = [s.clone() for s in sets]
+    ix.reorder([3, 0, 0, 1])
+    for s, old in zip(sets, before):
+        assert torch.equal(s.view(4, 2, *s.shape[1:]), old.view(4, 2, *s.shape[1:])[[3, 0, 0, 1]])
+
+
+def test_an_update_on_a_side_stream_waits_for_the_reordering():
+    from hira_b200 import CUDASearcher, CacheOutput
+    ix, k, v = _index(3, 2, 2000, 128, torch.bfloat16, 3, max_context=3000)
+    ref = ix.select([0, 1, 2])         # (the channel scales of the int8 copy differ between two builds)
+    q, side = torch.randn((3, 4, 1, 128), device="cuda"), torch.cuda.Stream()
+    for t in range(4):
+        picks = torch.tensor([(t + 1) % 3, t % 3, 0], device="cuda")
+        for index, stream in ((ix, side), (ref, None)):
+            hira_decode_attention(q, CacheOutput(None, None, None, None, index, CUDASearcher()), threshold_method="none")
+            index.reorder(picks)
+            index.update(k[:, :, t:t + 1] * 0.9, v[:, :, t:t + 1], stream=stream)
+    ix.wait_pending_update()
+    torch.cuda.synchronize()
+    for a, t in _arrays(ix).items():
+        assert torch.equal(t, _arrays(ref)[a]), a
+
+
+def test_an_index_selected_on_another_stream_is_whole_when_the_old_one_is_dropped():
+    ix, k, v = _index(2, 2, 20000, 128, torch.bfloat16, 3)
+    want = {a: t[[1, 0, 1]].clone() for a, t in _arrays(ix).items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        new = ix.select([1, 0, 1])
+    del ix
+    junk = [torch.full((1 << 26,), 7, dtype=torch.int32, device="cuda") for _ in range(4)]      # takes freed memory, if any is
+    torch.cuda.synchronize()
+    del junk
+    for a, t in _arrays(new).items():
+        assert torch.equal(t, want[a]), a
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
