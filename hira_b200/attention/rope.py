@@ -24,7 +24,7 @@ def _layout(t: torch.Tensor):
 
 
 def _check_apart(o: torch.Tensor, x: torch.Tensor, other: torch.Tensor, name: str):
-    if o.data_ptr() == x.data_ptr() and o.stride() == x.stride():
+    if o.data_ptr() == x.data_ptr() and o.stride() == x.stride() and (other.data_ptr() != x.data_ptr() or not o.numel()):
         return
     own = o.untyped_storage().data_ptr()
     if own == x.untyped_storage().data_ptr() or own == other.untyped_storage().data_ptr():
@@ -56,6 +56,7 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     or memory apart from both inputs (part of a cache, say).  No backward pass."""
     if torch.is_grad_enabled():
         refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
+    eps, interleaved = float(eps), bool(interleaved)
     # calls of a layout that has been checked before go straight to the library
     layout = (query.shape, query.stride(), query.dtype, query.get_device(), key.shape, key.stride(), key.dtype, key.get_device(),
               cos.shape, cos.stride(), cos.dtype, cos.get_device(), sin.shape, sin.stride(), sin.dtype, sin.get_device(),
@@ -158,13 +159,19 @@ def _is_head_rms_norm(norm, width: int) -> bool:
 def patch_attention(model, hira_config=None, *, interleaved: bool = False) -> int:
     """Gives every attention layer of `model` (a module with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx)
     `hira_attention_forward` as its forward; returns how many there were.  Run the model under `torch.no_grad()` with
-    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.  Layers whose heads are normalised in a way that `hira_qk_norm_rope` does not
-    do (over other widths than a head's) are refused."""
+    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.  Layers that compute
+    something else are refused: other norms than RMS norms of single heads, sliding windows, capped logits, sinks, no
+    rotation."""
     layers = [m for m in model.modules()
               if all(hasattr(m, a) for a in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "layer_idx"))]
     if not layers:
         raise ValueError("the model has no attention layer with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx")
     for m in layers:
+        for name in ("sliding_window", "attn_logit_softcapping", "sinks"):
+            if getattr(m, name, None) is not None:
+                raise ValueError(f"layer {m.layer_idx} has {name}, which a HiraCache's attention does not know")
+        if not getattr(m, "use_rope", True):
+            raise ValueError(f"layer {m.layer_idx} does not rotate its heads")
         for name in ("q_norm", "k_norm"):
             norm = getattr(m, name, None)
             if norm is None:

@@ -67,6 +67,8 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     to be so.  No backward pass.  A key hidden from one query token but not from another has to be finite."""
     if torch.is_grad_enabled():
         refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
+    if scaling is not None:
+        scaling = float(scaling)      # a tensor's value, not the tensor, goes with the layout
     # calls of a layout that has been checked before go straight to the library
     layout = None
     if (tail_keys is None or tail_values is not None and tail_keys.shape[:-1] == tail_values.shape[:-1]) \
@@ -139,12 +141,12 @@ def _keep(*tensors):
 class SharedPrompt:
     """P prompts kept once, and the tails of their P * branches continuations.
 
-        prompt = SharedPrompt(keys, values, branches=16)      # (P, H_kv, L, D), (P, H_kv, L, V): not copied
+        prompt = SharedPrompt(keys, values, branches=16)      # (P, H_kv, L, D), (P, H_kv, L, V)
         prompt.append(k, v)                                   # (P * 16, H_kv, m, D), (P * 16, H_kv, m, V)
         out = prompt.attend(query)                            # (P * 16, H_q, m, D) -> (P * 16, H_q, m, V)
         prompt.reorder(indices)                               # sequence b goes on from what indices[b] was
 
-    Tails grow by doubling; `max_tail` reserves room for that many tokens, so that nothing moves while a graph
+    Prompts are not copied, unless their rows are not contiguous or not 16-byte aligned.  Tails grow by doubling; `max_tail` reserves room for that many tokens, so that nothing moves while a graph
     that was captured with them lives."""
 
     def __init__(self, prefix_keys: torch.Tensor, prefix_values: torch.Tensor, branches: int, *, prefix_lens=None,
@@ -159,7 +161,7 @@ class SharedPrompt:
             raise ValueError(f"{branches} branches of {prefix_keys.shape[0]} prompts")
         if prefix_keys.dtype not in _TYPES:
             raise ValueError(f"unsupported dtype {prefix_keys.dtype}: float32 or bfloat16")
-        self.prefix_keys, self.prefix_values = prefix_keys, prefix_values
+        self.prefix_keys, self.prefix_values = S.with_rows(prefix_keys), S.with_rows(prefix_values)
         self.prefix_lens = _lengths(prefix_lens, prefix_keys.shape[0], prefix_keys.shape[2], prefix_keys.device, "prefix_lens")
         self.branches = int(branches)
         self.status = torch.zeros((1,), dtype=torch.int32, device=prefix_keys.device)

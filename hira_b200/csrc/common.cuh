@@ -17,6 +17,7 @@
 // fully used 128-byte line: lanes 0..7 read bytes [0,128) of a bf16 row with
 // their first chunk and [128,256) with their second.
 #pragma once
+#include <mutex>
 
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
@@ -78,7 +79,8 @@ inline cudaError_t launch_chained(K kern, dim3 grid, dim3 block, size_t smem, cu
 // launch costs a microsecond of the host's.  One of these belongs to one kernel.
 struct SmemLimit {
     static constexpr int DEVICES = 64;
-    int have[DEVICES] = {};      // racing threads store what they have raised it to
+    int have[DEVICES] = {};
+    std::mutex busy;
     template <typename K>
     cudaError_t raise(K kern, int bytes) {
         int dev = 0;
@@ -86,6 +88,8 @@ struct SmemLimit {
         if (e != cudaSuccess) return e;
         const bool kept = dev >= 0 && dev < DEVICES;
         if (kept && __atomic_load_n(&have[dev], __ATOMIC_RELAXED) >= bytes) return cudaSuccess;
+        std::lock_guard<std::mutex> one(busy);      // a thread that needs less must not lower it again
+        if (kept && have[dev] >= bytes) return cudaSuccess;
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e == cudaSuccess && kept) __atomic_store_n(&have[dev], bytes, __ATOMIC_RELAXED);
         return e;

@@ -167,3 +167,34 @@ def test_library_refuses_rotations_that_do_not_fit(kw, code):
     for n, v in kw.items():
         setattr(a, n, v)
     assert L.load().hira_qk_norm_rope(C.byref(a), None) == code
+
+
+def test_rotation_refuses_to_overwrite_heads_that_are_queries_and_keys_at_once():
+    x, c = _t(2, 4, 4, 64), _t(2, 4, 64)
+    for kw in (dict(out_q=x), dict(out_k=x)):
+        with pytest.raises(ValueError, match="apart"):
+            hira_qk_norm_rope(x, x, c, c, **kw)
+
+
+def test_shared_prompt_copies_rows_that_are_not_aligned_once():
+    k = torch.randn(2, 2, 9, 64).bfloat16()
+    flat = torch.cat([k.new_zeros(1), k.flatten()])
+    odd = flat[1:].view(k.shape)
+    p = SharedPrompt(odd, k, 2)
+    assert p.prefix_values is k and p.prefix_keys is not odd and torch.equal(p.prefix_keys, k)
+    assert S.row_strides(p.prefix_keys) is not None
+
+
+@pytest.mark.parametrize("name,value", [("sliding_window", 4096), ("attn_logit_softcapping", 50.0), ("sinks", torch.zeros(4)), ("use_rope", False)])
+def test_layers_that_compute_something_else_are_not_patched(name, value):
+    layer = torch.nn.Module()
+    for proj in ("q_proj", "k_proj", "v_proj", "o_proj"):
+        setattr(layer, proj, torch.nn.Linear(8, 8))
+    layer.head_dim, layer.layer_idx, layer.sliding_window = 8, 0, None
+    model, before = torch.nn.ModuleList([layer]), layer.forward
+    setattr(layer, name, value)
+    with pytest.raises(ValueError, match="layer 0"):
+        patch_attention(model)
+    assert layer.forward == before
+    setattr(layer, name, None if name != "use_rope" else True)
+    assert patch_attention(model) == 1
