@@ -425,6 +425,15 @@ shared_merge_kernel(const SharedAttn P) {
     const int np = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0, n = np + P.tail_parts, gap = P.prefix_parts - np;
     auto part = [&](int i) { return (size_t)(i < np ? i : i + gap) * P.n_rows + row; };
     grid_wait();
+    // the first parts' rows are asked for together with the maxima that weigh them: one round trip less
+    float4 x[SA_FLIGHT];
+    auto load = [&](int c, int i0) {
+        const int ch = lane * 4 + c * 128;
+        const float* src = P.part_o + (ch < P.vdim ? ch : 0);
+#pragma unroll
+        for (int j = 0; j < SA_FLIGHT; ++j) x[j] = *reinterpret_cast<const float4*>(src + part(min(i0 + j * W, n - 1)) * P.vdim);
+    };
+    if (n > 0) load(0, wi);
     float M = -CUDART_INF_F;
     bool bad = false;
     for (int i = lane; i < n; i += 32) {
@@ -449,13 +458,9 @@ shared_merge_kernel(const SharedAttn P) {
     float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const int ch = lane * 4 + c * 128;
         if (c * 128 >= P.vdim) break;
-        const float* src = P.part_o + (ch < P.vdim ? ch : 0);
         for (int i0 = wi; i0 < n; i0 += W * SA_FLIGHT) {
-            float4 x[SA_FLIGHT];
-#pragma unroll
-            for (int j = 0; j < SA_FLIGHT; ++j) x[j] = *reinterpret_cast<const float4*>(src + part(min(i0 + j * W, n - 1)) * P.vdim);
+            if (c > 0 || i0 != wi) load(c, i0);
 #pragma unroll
             for (int j = 0; j < SA_FLIGHT; ++j) {
                 const float w = i0 + j * W < n ? s_w[slot][i0 + j * W] : 0.f;

@@ -55,10 +55,22 @@ __device__ __forceinline__ void tl_join(const SharedAttn& P, const float (*s_m)[
         int row[R];
         float base[R], w_t[R], l_t[R], L[R], wi[R];
         float4 acc[R];
+        // the first parts' rows are asked for together with the maxima that weigh them: one round trip less
+        float4 x[R][TL_FLIGHT];
+        const float* src = P.part_o + (ch < P.vdim ? ch : 0);
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int j = 0; j < TL_FLIGHT; ++j)
+                    x[k][j] = *reinterpret_cast<const float4*>(src + ((size_t)min(i0 + j, n - 1) * P.n_rows + row[k]) * P.vdim);
+        };
+#pragma unroll
+        for (int k = 0; k < R; ++k) row[k] = first_row + min(r0 + k * TL_WARPS, rows - 1);
+        if (n > 0) load(0);
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const int r = min(r0 + k * TL_WARPS, rows - 1);
-            row[k] = first_row + r;
             float m_t = -CUDART_INF_F;
             l_t[k] = L[k] = 0.f;
             for (int w = 0; w < TL_WARPS; ++w) m_t = fmaxf(m_t, s_m[w][r]);
@@ -77,7 +89,6 @@ __device__ __forceinline__ void tl_join(const SharedAttn& P, const float (*s_m)[
                 }
             acc[k].x *= w_t[k]; acc[k].y *= w_t[k]; acc[k].z *= w_t[k]; acc[k].w *= w_t[k];
         }
-        const float* src = P.part_o + (ch < P.vdim ? ch : 0);
         for (int i0 = 0; i0 < n; i0 += 32) {
 #pragma unroll
             for (int k = 0; k < R; ++k) {
@@ -88,12 +99,7 @@ __device__ __forceinline__ void tl_join(const SharedAttn& P, const float (*s_m)[
             }
             const int count = min(n - i0, 32);
             for (int j0 = 0; j0 < count; j0 += TL_FLIGHT) {
-                float4 x[R][TL_FLIGHT];
-#pragma unroll
-                for (int k = 0; k < R; ++k)
-#pragma unroll
-                    for (int j = 0; j < TL_FLIGHT; ++j)
-                        x[k][j] = *reinterpret_cast<const float4*>(src + ((size_t)min(i0 + j0 + j, n - 1) * P.n_rows + row[k]) * P.vdim);
+                if (i0 + j0 > 0) load(i0 + j0);
 #pragma unroll
                 for (int k = 0; k < R; ++k)
 #pragma unroll
