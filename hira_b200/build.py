@@ -19,7 +19,7 @@ PROFILE_LIB_PATH = PKG_DIR / "libhira_b200_profile.so"   # the same library with
 OBJ_DIR = CSRC / "build"
 
 SOURCES = ["api.cu", "search.cu", "search_q8.cu", "attention.cu", "append.cu", "threshold.cu", "build.cu", "assign_tc.cu", "exchange.cu",
-           "shared_attn.cu", "shared_attn_tc.cu", "shared_attn_tail.cu", "gather.cu", "rope.cu"]
+           "shared_attn.cu", "shared_attn_tc.cu", "shared_attn_mma.cu", "gather.cu", "rope.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -18,14 +18,14 @@ constexpr int SA_KEYS = 64;       // keys a tile
 constexpr int SA_PAD = 4;         // floats behind each row in shared memory: rows 4 banks apart
 
 // ---------------------------------------------------------------------------
-// CUDA-core kernel for what the tensor cores do not serve: fp32, and rows wider than 128.
+// CUDA-core kernel for fp32.
 //
-// One block takes ROWS = 8 * RPT query rows of one item against a run of the item's keys, in tiles of 64 held as fp32
-// in shared memory.  16 lanes share RPT rows: for the products of a tile a lane has RPT rows x 4 keys in registers
+// One block takes ROWS = 8 * RPT query rows of one item against a run of the item's keys, in tiles of 64 in
+// shared memory.  16 lanes share RPT rows: for the products of a tile a lane has RPT rows x 4 keys in registers
 // (RPT + 4 16-byte loads for 16 RPT FMAs), for the weighted sums RPT rows x V / 16 channels.  A row's softmax
 // statistics stay with its 16 lanes, so the blocks only meet to exchange tiles.  fp32 products and sums throughout.
 // ---------------------------------------------------------------------------
-// Rows k0 .. k0 + 63 of keys or values into shared memory as fp32; those from `len` on as 0, nothing of them is read.
+// Rows k0 .. k0 + 63 of keys or values into shared memory; those from `len` on as 0, nothing of them is read.
 // A thread keeps its piece of the rows where the pieces divide the threads.
 template <typename F>
 __device__ __forceinline__ void sa_pieces(int pieces, F&& f) {
@@ -46,20 +46,10 @@ __device__ __forceinline__ void sa_load_tile(float* dst, int ld, const float* sr
     });
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 }
-__device__ __forceinline__ void sa_load_tile(float* dst, int ld, const __nv_bfloat16* src, long long stride, int k0, int len, int width) {
-    sa_pieces(width / 8, [&](int r, int c) {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (k0 + r < len) to_float(load_chunk<__nv_bfloat16>(src + (k0 + r) * stride, c), f);
-        float4* d = reinterpret_cast<float4*>(dst + r * ld + c * 8);
-        d[0] = make_float4(f[0], f[1], f[2], f[3]);
-        d[1] = make_float4(f[4], f[5], f[6], f[7]);
-    });
-    asm volatile("cp.async.commit_group;\n" ::: "memory");
-}
 template <int N>
 __device__ __forceinline__ void sa_landed() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
-template <typename T, int RPT, int NV, bool TAIL>
+template <int RPT, int NV, bool TAIL>
 __global__ void __launch_bounds__(SA_THREADS)
 shared_simt_kernel(const SharedAttn P) {
     constexpr int ROWS = 8 * RPT;
@@ -71,6 +61,7 @@ shared_simt_kernel(const SharedAttn P) {
     float* s_p = s_v + SA_KEYS * ldv;           // [SA_KEYS][ROWS + SA_PAD]
     constexpr int LDP = ROWS + SA_PAD;
 
+    grid_trigger();             // who follows waits before it reads
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int row0 = blockIdx.x * ROWS, split = blockIdx.y;
     const int item = blockIdx.z, h = item % P.n_kv, owner = item / P.n_kv;      // prompt, or branch of a tail
@@ -78,8 +69,8 @@ shared_simt_kernel(const SharedAttn P) {
     const int n_rows = TAIL ? per : P.n_branches * per;
     const int n_splits = TAIL ? P.tail_parts : P.prefix_parts;
     const int len = TAIL ? shared_tail_len(P, owner) : shared_prefix_len(P, owner);
-    const T* gk = reinterpret_cast<const T*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
-    const T* gv = reinterpret_cast<const T*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
+    const float* gk = reinterpret_cast<const float*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
+    const float* gv = reinterpret_cast<const float*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
     const long long ks = TAIL ? P.tks[2] : P.pks[2], vs = TAIL ? P.tvs[2] : P.pvs[2];
     auto out_row = [&](int r) {
         return TAIL ? (owner * P.n_kv + h) * per + r : shared_row(P, owner, h, r);
@@ -90,7 +81,7 @@ shared_simt_kernel(const SharedAttn P) {
         const int r = i / kc, c = i - r * kc;
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (row0 + r < n_rows)
-            to_float(load_chunk<T>(reinterpret_cast<const T*>(P.q) + shared_row_offset(P, out_row(row0 + r), P.qs), c), f);
+            to_float(load_chunk<float>(reinterpret_cast<const float*>(P.q) + shared_row_offset(P, out_row(row0 + r), P.qs), c), f);
         float4* d = reinterpret_cast<float4*>(s_q + r * ldk + c * 8);
         d[0] = make_float4(f[0], f[1], f[2], f[3]);
         d[1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -215,7 +206,7 @@ shared_simt_kernel(const SharedAttn P) {
             if (ch < P.vdim) *reinterpret_cast<float4*>(P.part_o + at * P.vdim + ch) = make_float4(o[a][c][0], o[a][c][1], o[a][c][2], o[a][c][3]);
         }
     }
-    if (TAIL) grid_wait();      // so that who waits for this waits for the prefix too
+    if (!TAIL) grid_wait();     // so that who waits for this waits for the tails too
 }
 
 // ---------------------------------------------------------------------------
@@ -224,7 +215,7 @@ shared_simt_kernel(const SharedAttn P) {
 // then takes whole rows for their softmax, and for the weighted sums a warp takes 16 of the 64 keys and a lane four
 // channels of all rows.  The four warps' sums are added up once, at the end.
 // ---------------------------------------------------------------------------
-template <typename T, int ROWS, int NV, bool TAIL>
+template <int ROWS, int NV, bool TAIL>
 __global__ void __launch_bounds__(SA_THREADS)
 shared_few_kernel(const SharedAttn P) {
     extern __shared__ __align__(16) float sa_smem[];
@@ -235,6 +226,7 @@ shared_few_kernel(const SharedAttn P) {
     float* s_p = s_v + SA_KEYS * ldv;           // [SA_KEYS][ROWS + SA_PAD]: logits, then weights
     constexpr int LDP = ROWS + SA_PAD;
     __shared__ float s_alpha[ROWS];
+    grid_trigger();             // who follows waits before it reads
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = blockIdx.x * ROWS, split = blockIdx.y;
     const int item = blockIdx.z, h = item % P.n_kv, owner = item / P.n_kv;      // prompt, or branch of a tail
@@ -242,8 +234,8 @@ shared_few_kernel(const SharedAttn P) {
     const int n_rows = TAIL ? per : P.n_branches * per;
     const int n_splits = TAIL ? P.tail_parts : P.prefix_parts;
     const int len = TAIL ? shared_tail_len(P, owner) : shared_prefix_len(P, owner);
-    const T* gk = reinterpret_cast<const T*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
-    const T* gv = reinterpret_cast<const T*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
+    const float* gk = reinterpret_cast<const float*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
+    const float* gv = reinterpret_cast<const float*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
     const long long ks = TAIL ? P.tks[2] : P.pks[2], vs = TAIL ? P.tvs[2] : P.pvs[2];
     auto out_row = [&](int r) {
         return TAIL ? (owner * P.n_kv + h) * per + r : shared_row(P, owner, h, r);
@@ -256,7 +248,7 @@ shared_few_kernel(const SharedAttn P) {
         const int r = i / kc, c = i - r * kc;
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (row0 + r < n_rows)
-            to_float(load_chunk<T>(reinterpret_cast<const T*>(P.q) + shared_row_offset(P, out_row(row0 + r), P.qs), c), f);
+            to_float(load_chunk<float>(reinterpret_cast<const float*>(P.q) + shared_row_offset(P, out_row(row0 + r), P.qs), c), f);
         float4* d = reinterpret_cast<float4*>(s_q + r * ldk + c * 8);
         d[0] = make_float4(f[0], f[1], f[2], f[3]);
         d[1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -399,7 +391,7 @@ shared_few_kernel(const SharedAttn P) {
             *reinterpret_cast<float4*>(P.part_o + at * P.vdim + ch) = y;
         }
     }
-    if (TAIL) grid_wait();      // so that who waits for this waits for the prefix too
+    if (!TAIL) grid_wait();     // so that who waits for this waits for the tails too
 }
 
 // ---------------------------------------------------------------------------
@@ -502,14 +494,14 @@ shared_merge_kernel(const SharedAttn P) {
     }
 }
 
-template <typename T, int RPT, int NV, bool TAIL>
+template <int RPT, int NV, bool TAIL>
 static auto simt_kernel() {      // NV: 64 channels each of 16 lanes, or (few rows) 128 each of a warp
-    if constexpr (RPT <= 2) return shared_few_kernel<T, 8 * RPT, NV / 2, TAIL>;
-    else return shared_simt_kernel<T, RPT, NV, TAIL>;
+    if constexpr (RPT <= 2) return shared_few_kernel<8 * RPT, NV / 2, TAIL>;
+    else return shared_simt_kernel<RPT, NV, TAIL>;
 }
-template <typename T, int RPT, int NV, bool TAIL>
+template <int RPT, int NV, bool TAIL>
 static int launch_simt(const SharedAttn& P, bool chained, cudaStream_t s) {
-    auto kern = simt_kernel<T, RPT, NV, TAIL>();
+    auto kern = simt_kernel<RPT, NV, TAIL>();
     const int per = P.group * P.n_q, rows = TAIL ? per : P.n_branches * per;
     const size_t smem = sizeof(float) * ((size_t)(8 * RPT + SA_KEYS) * (P.dim + SA_PAD) + (size_t)SA_KEYS * (P.vdim + SA_PAD) +
                                          (size_t)SA_KEYS * (8 * RPT + SA_PAD));
@@ -537,18 +529,18 @@ static int launch_simt(const SharedAttn& P, bool chained, cudaStream_t s) {
 // rows a block takes: no more than there are, so that a few rows do not pay for the products of many
 static int simt_rows(int rows, int vdim) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 || vdim > 128 ? 32 : 64; }
 
-template <typename T, bool TAIL>
+template <bool TAIL>
 static int launch_simt_rows(const SharedAttn& P, bool chained, cudaStream_t s) {
     const int per = P.group * P.n_q, rows = simt_rows(TAIL ? per : P.n_branches * per, P.vdim);
     if (P.vdim > 128) {
-        if (rows == 8) return launch_simt<T, 1, 4, TAIL>(P, chained, s);
-        if (rows == 16) return launch_simt<T, 2, 4, TAIL>(P, chained, s);
-        return launch_simt<T, 4, 4, TAIL>(P, chained, s);
+        if (rows == 8) return launch_simt<1, 4, TAIL>(P, chained, s);
+        if (rows == 16) return launch_simt<2, 4, TAIL>(P, chained, s);
+        return launch_simt<4, 4, TAIL>(P, chained, s);
     }
-    if (rows == 8) return launch_simt<T, 1, 2, TAIL>(P, chained, s);
-    if (rows == 16) return launch_simt<T, 2, 2, TAIL>(P, chained, s);
-    if (rows == 32) return launch_simt<T, 4, 2, TAIL>(P, chained, s);
-    return launch_simt<T, 8, 2, TAIL>(P, chained, s);
+    if (rows == 8) return launch_simt<1, 2, TAIL>(P, chained, s);
+    if (rows == 16) return launch_simt<2, 2, TAIL>(P, chained, s);
+    if (rows == 32) return launch_simt<4, 2, TAIL>(P, chained, s);
+    return launch_simt<8, 2, TAIL>(P, chained, s);
 }
 
 // Splits of the keys: as many blocks as are resident at once (three an SM of those with few rows, else two), none with
@@ -601,11 +593,16 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
         P.pks[i] = st[0][i]; P.pvs[i] = st[1][i]; P.tks[i] = st[2][i]; P.tvs[i] = st[3][i]; P.qs[i] = st[4][i]; P.os[i] = st[5][i];
     }
     const int per = a->group * a->n_q;
-    if (shared_tc_supported(P, a->dtype)) shared_tc_plan(P);
-    else P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
-    P.tail_parts = shared_tail_supported(P, a->dtype) ? shared_tail_splits(P)
-                                                      : simt_splits(per, a->n_prompts * a->n_branches * a->n_kv, a->tail_len, a->vdim);
-    P.fused = shared_tail_supported(P, a->dtype) && shared_tail_joins(P);
+    const int branches = a->n_prompts * a->n_branches * a->n_kv;
+    if (a->dtype == HIRA_BF16) {
+        P.tail_parts = shared_mma_splits(P, true);
+        if (shared_tc_supported(P)) shared_tc_plan(P);
+        else P.prefix_parts = shared_mma_splits(P, false);
+        P.fused = shared_tail_joins(P);
+    } else {
+        P.tail_parts = simt_splits(per, branches, a->tail_len, a->vdim);
+        P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
+    }
     return HIRA_OK;
 }
 static size_t shared_parts_bytes(const SharedAttn& P) {
@@ -615,14 +612,17 @@ static size_t shared_parts_bytes(const SharedAttn& P) {
 template <typename T>
 static int run_shared(const SharedAttn& P, cudaStream_t s) {
     // The first kernel starts when all before it on the stream is done; the ones behind it may start beside it, so each
-    // waits for the one before it by its end (the merge: at its start).
+    // waits for the one before it by its end (the merge: at its start).  With bf16 the prefix's kernel takes whole SMs, and
+    // the tail's joins the parts where it can: the tails come second.  With fp32 they come first, so that their few blocks run
+    // beside the prefix's instead of behind them (2 prompts x 4 branches of 8 heads, 4,100 keys: 29 us, the other way 35).
     int rc = HIRA_OK;
-    if (P.shares > 0) rc = shared_tc_launch(P, s);
-    else if (P.prefix_parts > 0) rc = launch_simt_rows<T, false>(P, false, s);
-    if (rc != HIRA_OK) return rc;
-    if (P.tail_parts > 0)
-        rc = shared_tail_supported(P, sizeof(T) == 2 ? HIRA_BF16 : HIRA_F32) ? shared_tail_launch(P, P.prefix_parts > 0, s)
-                                                                            : launch_simt_rows<T, true>(P, P.prefix_parts > 0, s);
+    if (sizeof(T) == 2) {
+        if (P.prefix_parts > 0) rc = P.shares > 0 ? shared_tc_launch(P, s) : shared_mma_launch(P, false, false, s);
+        if (rc == HIRA_OK && P.tail_parts > 0) rc = shared_mma_launch(P, true, P.prefix_parts > 0, s);
+    } else {
+        if (P.tail_parts > 0) rc = launch_simt_rows<true>(P, false, s);
+        if (rc == HIRA_OK && P.prefix_parts > 0) rc = launch_simt_rows<false>(P, P.tail_parts > 0, s);
+    }
     if (rc != HIRA_OK || P.fused) return rc;
     const int parts = P.prefix_parts + P.tail_parts;
     const bool many = parts > SA_FLIGHT;

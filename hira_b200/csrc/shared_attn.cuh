@@ -68,13 +68,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-bool shared_tc_supported(const SharedAttn& P, int dtype);
+bool shared_tc_supported(const SharedAttn& P);
 void shared_tc_plan(SharedAttn& P);
 int shared_tc_launch(const SharedAttn& P, cudaStream_t s);
-bool shared_tail_supported(const SharedAttn& P, int dtype);
-int shared_tail_splits(const SharedAttn& P);
+int shared_mma_splits(const SharedAttn& P, bool tail);
 bool shared_tail_joins(const SharedAttn& P);
 // chained: behind the prefix's kernel, beside which it may run
-int shared_tail_launch(const SharedAttn& P, bool chained, cudaStream_t s);
+int shared_mma_launch(const SharedAttn& P, bool tail, bool chained, cudaStream_t s);
 
 }  // namespace hira

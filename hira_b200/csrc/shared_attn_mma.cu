@@ -1,10 +1,11 @@
-// The tails of hira_shared_attn for bf16 rows of up to 128: few query rows (group x tokens) against keys of their own.
+// The tails of hira_shared_attn for bf16, and the prefixes that the tcgen05 kernel does not take (rows wider than 128, strides
+// that a tensor map does not take): few query rows against keys of their own.
 //
-// Bound by the tails' bytes: 16 query rows cost 16-bit matrix products that hide behind the loads.  A block of four
-// warps takes 16 rows of one (branch, kv head) against a run of its keys; each warp takes 16 keys of every 64, through
-// a ring of its own (cp.async, no barrier between warps), with softmax statistics of its own, and the four join once, at
-// the end.  Products by mma.sync m16n8k16: the rows are too few for a tcgen05 tile, which would be 7/8 empty.
-// 64 branches x 8 heads x 256 keys (134 MB): see the launch below for what it measured.
+// Bound by the keys' bytes: 16 query rows cost 16-bit matrix products that hide behind the loads.  A block of four
+// warps takes 16 rows of one item -- (branch, kv head) or (prompt, kv head) -- against a run of its keys; each warp takes 16
+// keys of every 64, through a ring of its own (cp.async, no barrier between warps), with softmax statistics of its own, and
+// the four join once, at the end.  Products by mma.sync m16n8k16: a tail's rows are too few for a tcgen05 tile, which would be
+// 7/8 empty.  TAIL_FIGURES
 #include "shared_attn.cuh"
 #include "tc_common.cuh"
 #include <math_constants.h>
@@ -23,7 +24,8 @@ template <int HD>
 struct TlLayout {
     static constexpr int ROW = HD * 2;                              // bytes
     static constexpr int STAGE = 2 * TL_KEYS * ROW;                 // keys, then values, of one warp
-    static constexpr int BYTES = TL_WARPS * TL_STAGES * STAGE;      // the joined sums (16 x HD floats a warp) fit too
+    static constexpr int STAGES = HD == 256 ? 2 : TL_STAGES;
+    static constexpr int BYTES = TL_WARPS * STAGES * STAGE;         // the joined sums (16 x HD floats a warp) fit too
 };
 
 __device__ __forceinline__ void tl_cp16(uint32_t dst, const void* src, bool there) {
@@ -126,25 +128,28 @@ __device__ __forceinline__ void tl_join(const SharedAttn& P, const float (*s_m)[
     }
 }
 
-template <int HD>
-__global__ void __launch_bounds__(32 * TL_WARPS, HD == 128 ? 2 : 3)
-shared_tail_kernel(const SharedAttn P) {
+template <int HD, bool TAIL>
+__global__ void __launch_bounds__(32 * TL_WARPS, HD == 256 ? 1 : HD == 128 ? 2 : 3)
+shared_mma_kernel(const SharedAttn P) {
     using Lay = TlLayout<HD>;
     extern __shared__ __align__(128) unsigned char tl_smem[];
     __shared__ float s_m[TL_WARPS][TL_ROWS], s_l[TL_WARPS][TL_ROWS];
     grid_trigger();      // the merge waits before it reads
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
     const int row0 = blockIdx.x * TL_ROWS, split = blockIdx.y;
-    const int b = blockIdx.z / P.n_kv, h = blockIdx.z % P.n_kv, per = P.group * P.n_q;
-    const int len = shared_tail_len(P, b);
-    const __nv_bfloat16* gk = reinterpret_cast<const __nv_bfloat16*>(P.tk) + b * P.tks[0] + h * P.tks[1];
-    const __nv_bfloat16* gv = reinterpret_cast<const __nv_bfloat16*>(P.tv) + b * P.tvs[0] + h * P.tvs[1];
-    const int out_row0 = (b * P.n_kv + h) * per;
+    const int owner = blockIdx.z / P.n_kv, h = blockIdx.z % P.n_kv, per = P.group * P.n_q;      // a tail's branch, or a prompt
+    const int n_rows = TAIL ? per : P.n_branches * per, n_splits = TAIL ? P.tail_parts : P.prefix_parts;
+    const int len = TAIL ? shared_tail_len(P, owner) : shared_prefix_len(P, owner);
+    const __nv_bfloat16* gk = reinterpret_cast<const __nv_bfloat16*>(TAIL ? P.tk : P.pk) + owner * (TAIL ? P.tks[0] : P.pks[0]) + h * (TAIL ? P.tks[1] : P.pks[1]);
+    const __nv_bfloat16* gv = reinterpret_cast<const __nv_bfloat16*>(TAIL ? P.tv : P.pv) + owner * (TAIL ? P.tvs[0] : P.pvs[0]) + h * (TAIL ? P.tvs[1] : P.pvs[1]);
+    const long long ks = TAIL ? P.tks[2] : P.pks[2], vs = TAIL ? P.tvs[2] : P.pvs[2];
+    const int out_row0 = (owner * P.n_kv + h) * per;      // of a tail
+    auto out_row = [&](int r) { return TAIL ? out_row0 + r : shared_row(P, owner, h, r); };
 
     // this warp's steps: 16 keys of every 64
     const int steps_all = (len + TL_STEP - 1) / TL_STEP;
-    const int t0 = (int)((long long)split * steps_all / P.tail_parts), t1 = (int)((long long)(split + 1) * steps_all / P.tail_parts);
-    const uint32_t ring = smem_u32(tl_smem) + warp * TL_STAGES * Lay::STAGE;
+    const int t0 = (int)((long long)split * steps_all / n_splits), t1 = (int)((long long)(split + 1) * steps_all / n_splits);
+    const uint32_t ring = smem_u32(tl_smem) + warp * Lay::STAGES * Lay::STAGE;
     // A lane copies the same 16 bytes of every RPI-th of a step's keys and values.
     constexpr int CH = HD / 8, RPI = 32 / CH, ITER = TL_KEYS / RPI;
     const int lr = lane / CH, lc = lane % CH;
@@ -153,9 +158,9 @@ shared_tail_kernel(const SharedAttn P) {
     auto load = [&](int t, int stage) {
         const int k0 = t * TL_STEP + warp * TL_KEYS;
         if (t < t1 && k0 < len) {
-            const __nv_bfloat16* src_k = gk + (k0 + lr) * P.tks[2] + lc * 8;
-            const __nv_bfloat16* src_v = gv + (k0 + lr) * P.tvs[2] + lc * 8;
-            const long long step_k = RPI * P.tks[2], step_v = RPI * P.tvs[2];
+            const __nv_bfloat16* src_k = gk + (k0 + lr) * ks + lc * 8;
+            const __nv_bfloat16* src_v = gv + (k0 + lr) * vs + lc * 8;
+            const long long step_k = RPI * ks, step_v = RPI * vs;
             const uint32_t dst = dst0 + stage * Lay::STAGE;
             const bool whole = k0 + TL_KEYS <= len;
 #pragma unroll
@@ -171,27 +176,27 @@ shared_tail_kernel(const SharedAttn P) {
         asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
 #pragma unroll
-    for (int i = 0; i < TL_STAGES - 1; ++i) load(t0 + i, i);
+    for (int i = 0; i < Lay::STAGES - 1; ++i) load(t0 + i, i);
 
     // queries as the products want them: rows g and g + 8, two channels a register
     uint32_t q[HD / 16][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int r = row0 + g + 8 * j;
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(P.q) + (r < per ? shared_row_offset(P, out_row0 + r, P.qs) : 0);
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(P.q) + (r < n_rows ? shared_row_offset(P, out_row(r), P.qs) : 0);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int ch = k * 16 + u * 8 + tig * 2;
-                q[k][j + 2 * u] = r < per && ch < P.dim ? *reinterpret_cast<const uint32_t*>(src + ch) : 0u;
+                q[k][j + 2 * u] = r < n_rows && ch < P.dim ? *reinterpret_cast<const uint32_t*>(src + ch) : 0u;
             }
     }
     int seen[2];
     float m[2], l[2], o[HD / 8][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        seen[j] = len - (P.n_q - 1 - (row0 + g + 8 * j) % P.n_q);
+        seen[j] = TAIL ? len - (P.n_q - 1 - (row0 + g + 8 * j) % P.n_q) : len;
         m[j] = -CUDART_INF_F;
         l[j] = 0.f;
     }
@@ -201,9 +206,9 @@ shared_tail_kernel(const SharedAttn P) {
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
     for (int t = t0; t < t1; ++t) {
-        const int stage = (t - t0) % TL_STAGES;
-        load(t + TL_STAGES - 1, (t - t0 + TL_STAGES - 1) % TL_STAGES);
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(TL_STAGES - 1) : "memory");
+        const int stage = (t - t0) % Lay::STAGES;
+        load(t + Lay::STAGES - 1, (t - t0 + Lay::STAGES - 1) % Lay::STAGES);
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(Lay::STAGES - 1) : "memory");
         __syncwarp();
         const int k0 = t * TL_STEP + warp * TL_KEYS;
         if (k0 < len) {          // the same for the warp
@@ -301,27 +306,27 @@ shared_tail_kernel(const SharedAttn P) {
         for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * j] * w, o[n][2 * j + 1] * w);
     }
     __syncthreads();
-    if (P.fused) {
+    if constexpr (TAIL && HD <= 128) if (P.fused) {
         // the tail's only part: what the merge would do with it and the prefix's parts, done here
         const int rows = min(per - row0, TL_ROWS);
-        const int item = b / P.n_branches * P.n_kv + h;
+        const int item = owner / P.n_branches * P.n_kv + h;
         const int n = P.prefix_parts > 0 ? shared_item_parts(P, item) : 0;
         grid_wait();             // the prefix's parts are there
         if (rows <= TL_WARPS) tl_join<HD, 1>(P, s_m, s_l, s_o, n, rows, out_row0 + row0);
         else tl_join<HD, 2>(P, s_m, s_l, s_o, n, rows, out_row0 + row0);
         return;
     }
-    const size_t part = (size_t)(P.prefix_parts + split) * P.n_rows;
+    const size_t part = (size_t)((TAIL ? P.prefix_parts : 0) + split) * P.n_rows;
     for (int i = tid; i < TL_ROWS * (HD / 4); i += 32 * TL_WARPS) {
         const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-        if (row0 + r >= per || c >= P.vdim) continue;
+        if (row0 + r >= n_rows || c >= P.vdim) continue;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < TL_WARPS; ++w) {
             const float4 x = *reinterpret_cast<const float4*>(s_o + (w * TL_ROWS + r) * HD + c);
             a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
         }
-        const size_t at = part + out_row0 + row0 + r;
+        const size_t at = part + out_row(row0 + r);
         *reinterpret_cast<float4*>(P.part_o + at * P.vdim + c) = a;
         if (c == 0) {
             float top = -CUDART_INF_F, sum = 0.f;
@@ -330,33 +335,35 @@ shared_tail_kernel(const SharedAttn P) {
             P.part_ml[at] = make_float2(top, sum);
         }
     }
-    grid_wait();                 // so that who waits for this waits for the prefix too
+    if (TAIL) grid_wait();       // so that who waits for this waits for the prefix too
 }
 
 // A block that joins the parts of its rows itself saves a launch and its round trips, as long as its warps have no more
 // than the two rows each that they join at a time (15 branches of 9 rows: 30 us that way, 25 with the merge's kernel).
-bool shared_tail_joins(const SharedAttn& P) { return P.tail_parts == 1 && P.group * P.n_q <= 2 * TL_WARPS; }
-bool shared_tail_supported(const SharedAttn& P, int dtype) { return dtype == HIRA_BF16 && P.dim <= 128 && P.vdim <= 128; }
+bool shared_tail_joins(const SharedAttn& P) { return P.tail_parts == 1 && P.group * P.n_q <= 2 * TL_WARPS && P.dim <= 128 && P.vdim <= 128; }
 
-// Splits of a tail: two blocks an SM, none with less than two steps of its own.
-int shared_tail_splits(const SharedAttn& P) {
-    if (P.tail_len <= 0) return 0;
-    const long long blocks = (long long)((P.group * P.n_q + TL_ROWS - 1) / TL_ROWS) * P.n_prompts * P.n_branches * P.n_kv;
-    const int steps = (P.tail_len + TL_STEP - 1) / TL_STEP;
-    long long s = 2 * SM_COUNT / blocks;
+static int tl_width(const SharedAttn& P) { return P.dim > 128 || P.vdim > 128 ? 256 : P.dim > 64 || P.vdim > 64 ? 128 : 64; }
+// Splits of the keys: two blocks an SM (one of 256 channels), none with less than two steps of its own.
+int shared_mma_splits(const SharedAttn& P, bool tail) {
+    const int len = tail ? P.tail_len : P.prefix_len, rows = P.group * P.n_q * (tail ? 1 : P.n_branches);
+    if (len <= 0) return 0;
+    const long long blocks = (long long)((rows + TL_ROWS - 1) / TL_ROWS) * P.n_prompts * (tail ? P.n_branches : 1) * P.n_kv;
+    const int steps = (len + TL_STEP - 1) / TL_STEP;
+    long long s = (tl_width(P) == 256 ? 1 : 2) * SM_COUNT / blocks;
     if (s > steps / 2) s = steps / 2;
     if (s > 32) s = 32;
     return s < 1 ? 1 : (int)s;
 }
 
-template <int HD>
+template <int HD, bool TAIL>
 static int tl_launch(const SharedAttn& P, bool chained, cudaStream_t s) {
-    auto kern = shared_tail_kernel<HD>;
-    const int smem = TlLayout<HD>::BYTES;
+    auto kern = shared_mma_kernel<HD, TAIL>;
+    const int smem = TlLayout<HD>::BYTES, rows = P.group * P.n_q * (TAIL ? 1 : P.n_branches);
     static SmemLimit limit;
     cudaError_t e = limit.raise(kern, smem);
     if (e == cudaSuccess) {
-        const dim3 grid((unsigned)((P.group * P.n_q + TL_ROWS - 1) / TL_ROWS), (unsigned)P.tail_parts, (unsigned)(P.n_prompts * P.n_branches * P.n_kv));
+        const dim3 grid((unsigned)((rows + TL_ROWS - 1) / TL_ROWS), (unsigned)(TAIL ? P.tail_parts : P.prefix_parts),
+                        (unsigned)(P.n_prompts * (TAIL ? P.n_branches : 1) * P.n_kv));
         if (chained) {
             e = launch_chained(kern, grid, dim3(32 * TL_WARPS), smem, s, P);
         } else {
@@ -365,13 +372,18 @@ static int tl_launch(const SharedAttn& P, bool chained, cudaStream_t s) {
         }
     }
     if (e != cudaSuccess) {
-        set_error("hira_shared_attn tail launch: %s", cudaGetErrorString(e));
+        set_error("hira_shared_attn launch: %s", cudaGetErrorString(e));
         return HIRA_ERR_CUDA;
     }
     return HIRA_OK;
 }
-int shared_tail_launch(const SharedAttn& P, bool chained, cudaStream_t s) {
-    return P.dim > 64 || P.vdim > 64 ? tl_launch<128>(P, chained, s) : tl_launch<64>(P, chained, s);
+template <bool TAIL>
+static int tl_launch_width(const SharedAttn& P, bool chained, cudaStream_t s) {
+    const int w = tl_width(P);
+    return w == 256 ? tl_launch<256, TAIL>(P, chained, s) : w == 128 ? tl_launch<128, TAIL>(P, chained, s) : tl_launch<64, TAIL>(P, chained, s);
+}
+int shared_mma_launch(const SharedAttn& P, bool tail, bool chained, cudaStream_t s) {
+    return tail ? tl_launch_width<true>(P, chained, s) : tl_launch_width<false>(P, chained, s);
 }
 
 }  // namespace hira

@@ -547,8 +547,8 @@ static bool st_make_map(CUtensorMap* map, const void* base, int width, const Sha
 }
 
 // Strides that a tensor map takes: forward, rows that do not overlap, and below 2^40 bytes.
-bool shared_tc_supported(const SharedAttn& P, int dtype) {
-    if (dtype != HIRA_BF16 || P.prefix_len == 0 || P.dim > 128 || P.vdim > 128 || (P.dim > 64) != (P.vdim > 64)) return false;
+bool shared_tc_supported(const SharedAttn& P) {
+    if (P.prefix_len == 0 || P.dim > 128 || P.vdim > 128 || (P.dim > 64) != (P.vdim > 64)) return false;
     const int n[3] = {P.n_prompts, P.n_kv, P.prefix_len};
     for (int i = 0; i < 3; ++i)
         if (n[i] > 1 && (P.pks[i] < 1 || P.pvs[i] < 1 || P.pks[i] >= (1ll << 39) || P.pvs[i] >= (1ll << 39))) return false;
