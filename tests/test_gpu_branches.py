@@ -205,6 +205,20 @@ def test_many_calls_at_once_on_two_streams():
     assert all(bool((x == want[i]).all()) for i, x in got)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 20, 2, 4, 1, 256, 256, 1501, 33), (1, 5, 1, 3, 2, 136, 64, 4000, 260), (1, 17, 2, 1, 1, 64, 248, 65, 1),
+                                   (1, 1, 40, 4, 1, 256, 256, 700, 16)], ids=lambda s: "x".join(map(str, s)))
+def test_wide_rows_in_several_row_blocks_and_splits(shape, dtype):
+    q, pk, pv, tk, tv = _qkv(*shape, dtype, seed=81)
+    p, b, lens = shape[0], shape[0] * shape[1], [shape[7] - 40] + [0] * (shape[0] - 1)
+    _check(hira_shared_attention(q, pk, pv, tk, tv), _exact(q, pk, pv, tk, tv))
+    tl = [i % (shape[8] + 1) for i in range(b)]
+    pk[:, :, shape[7] - 40:], pv[:, :, shape[7] - 40:] = float("nan"), float("nan")      # behind the lengths
+    if p > 1:
+        pk[1:], pv[1:] = float("nan"), float("nan")
+    _check(hira_shared_attention(q, pk, pv, tk, tv, prefix_lens=lens, tail_lens=tl), _exact(q, pk, pv, tk, tv, lens, tl))
+
+
 def test_threads_that_call_at_once_with_rows_of_different_widths():
     cases = [_qkv(1, 3, 2, 2, 1, d, v, 150, 70, dtype, seed=50 + d + v)
              for d, v in ((256, 256), (64, 64), (8, 8), (128, 128), (128, 256)) for dtype in (torch.float32, torch.bfloat16)]
