@@ -596,7 +596,7 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
     const int branches = a->n_prompts * a->n_branches * a->n_kv;
     if (a->dtype == HIRA_BF16) {
         P.tail_parts = shared_mma_splits(P, true);
-        if (shared_tc_supported(P)) shared_tc_plan(P);
+        if (shared_tc_supported(P) && !shared_mma_prefers(P)) shared_tc_plan(P);
         else P.prefix_parts = shared_mma_splits(P, false);
         P.fused = shared_tail_joins(P);
     } else {
@@ -625,6 +625,8 @@ static int run_shared(const SharedAttn& P, cudaStream_t s) {
     }
     if (rc != HIRA_OK || P.fused) return rc;
     const int parts = P.prefix_parts + P.tail_parts;
+    // four warps a row where its parts fill their flights (36 rows of some 30 parts: 28.7 us the whole call, 32.8 with one), one
+    // where they do not (2,048 rows of 2 parts: 41 us, 45 with four)
     const bool many = parts > SA_FLIGHT;
     const int rows = many ? 1 : SA_MERGE_WARPS;
     const dim3 grid((unsigned)((P.n_rows + rows - 1) / rows));

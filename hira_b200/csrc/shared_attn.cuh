@@ -71,6 +71,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 bool shared_tc_supported(const SharedAttn& P);
 void shared_tc_plan(SharedAttn& P);
 int shared_tc_launch(const SharedAttn& P, cudaStream_t s);
+bool shared_mma_prefers(const SharedAttn& P);
 int shared_mma_splits(const SharedAttn& P, bool tail);
 bool shared_tail_joins(const SharedAttn& P);
 // chained: behind the prefix's kernel, beside which it may run

@@ -1,5 +1,5 @@
 // The tails of hira_shared_attn for bf16, and the prefixes that the tcgen05 kernel does not take (rows wider than 128, strides
-// that a tensor map does not take): few query rows against keys of their own.
+// that a tensor map does not take, few keys): few query rows against keys of their own.
 //
 // Bound by the keys' bytes: 16 query rows cost 16-bit matrix products that hide behind the loads.  A block of four
 // warps takes 16 rows of one item -- (branch, kv head) or (prompt, kv head) -- against a run of its keys; each warp takes 16
@@ -343,6 +343,13 @@ shared_mma_kernel(const SharedAttn P) {
 bool shared_tail_joins(const SharedAttn& P) { return P.tail_parts == 1 && P.group * P.n_q <= 2 * TL_WARPS && P.dim <= 128 && P.vdim <= 128; }
 
 static int tl_width(const SharedAttn& P) { return P.dim > 128 || P.vdim > 128 ? 256 : P.dim > 64 || P.vdim > 64 ? 128 : 64; }
+// Prefixes of few rows or keys: 16 rows a block, each block row reading the keys again, start sooner than tcgen05 tiles.  8 heads
+// on the device, this way and the other: 8 to 32 rows a head 300 keys 12.3 / 14.4 us, 2,000 keys 14.3..16.4 / 16.4..20.5, 9,000
+// keys 20.5..22.6 / 22.5..24.6; 64 rows 2,000 keys 18.4 / 20.5, 9,000 keys 28.7 / 26.6, 32,768 keys 57 / 37.
+bool shared_mma_prefers(const SharedAttn& P) {
+    const long long row_blocks = ((long long)P.n_branches * P.group * P.n_q + TL_ROWS - 1) / TL_ROWS;
+    return row_blocks * P.n_prompts * P.n_kv * P.prefix_len <= 1280ll * SM_COUNT;
+}
 // Splits of the keys: two blocks an SM (one of 256 channels), none with less than two steps of its own.
 int shared_mma_splits(const SharedAttn& P, bool tail) {
     const int len = tail ? P.tail_len : P.prefix_len, rows = P.group * P.n_q * (tail ? 1 : P.n_branches);

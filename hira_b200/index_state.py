@@ -152,7 +152,7 @@ class IndexState:
         s.n_heads = new.n_heads = n_heads
         new.status = torch.empty_like(self.status)
         new._append_bytes, new._append_ws = {}, (None, 0)
-        new._streams = {L.current_stream(self.device)} if self.device.type == "cuda" else set()
+        new._streams = {torch._C._cuda_getCurrentRawStream(self.arrays_device.index)} if self.device.type == "cuda" else set()
         new._struct, new._byref = s, C.byref(s)
         return new
 

@@ -473,7 +473,8 @@ class CUDAIndexer(BaseIndexer):
         new._tau_drawn = []
         new._scan_pending = new._searched_fresh = False
         S.gather_index(st, new.state, idx, self.batch)
-        st.used_on(torch.cuda.current_stream(st.device))     # the caller may drop this one right away
+        if torch._C._cuda_getCurrentRawStream(st.arrays_device.index) not in st._streams:
+            st.used_on(torch.cuda.current_stream(st.device))     # the caller may drop this one right away
         return new
 
     def _settled(self) -> S.IndexState:
