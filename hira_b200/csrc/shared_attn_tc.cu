@@ -13,6 +13,10 @@
 //
 // The tiles of all items are dealt out in equal runs, one to each SM, whatever the items' number: a run may end
 // inside an item and go on in the next one.  Every wait is bounded; a block whose wait ran out leaves NaN.
+//
+// Measured (8 heads of 128): 16 branches x 4 heads a key head at 32,768 keys 27 us (134 MB: 5.0 TB/s; 6.3 in the loop, the
+// rest is some 1.7 us before the first product and 1.6 behind the last); 64 branches at 131,072 keys 130 us (4.1 TB/s and
+// 1.05 PFLOP/s: exponentials of two groups, products and the hand-overs between them, none of which is busy all the time).
 #include "shared_attn.cuh"
 #include "tc_common.cuh"
 

@@ -522,11 +522,11 @@ int hira_assign(const void* points, const void* cents, int32_t dtype,
  *   out[b][hq][t] = softmax(sm_scale q[b][hq][t] . K) V,   K = prefix[prompt][hq / group][0 .. prefix_len)
  *                                                           ++ tail[b][hq / group][0 .. tail_len - (n_q - 1 - t)).
  * The last n_q keys of a tail are those of the query tokens, so token t does not see the ones behind it.  A row that
- * sees no key is 0.  Softmax and sums in fp32, the output rounded once to `dtype`; with bf16 rows of up to 128 the
- * softmax weights enter the tensor cores as bf16, each off by at most 2^-8 of itself, as the output's own rounding.
+ * sees no key is 0.  Softmax and sums in fp32, the output rounded once to `dtype`; with bf16 the softmax weights enter
+ * the tensor cores as bf16, each off by at most 2^-8 of itself, as the output's own rounding.
  * What lies behind a length is never used, whatever it holds.
  * All rows start on 16-byte boundaries with their elements one behind another; strides are in elements: (prompt or
- * branch, head, row or token).  Any of them may be 0 or negative on the tails, the queries and the CUDA-core path.
+ * branch, head, row or token).  Any of them may be 0 or negative (not of the output).
  * `workspace` belongs to the call until it is done; hira_shared_attn_workspace_bytes gives its size (16-byte aligned). */
 typedef struct hira_shared_attn {
     const void* q;              /* [n_prompts * n_branches][n_kv * group][n_q][dim]   */
