@@ -280,6 +280,79 @@ def test_a_nan_in_sight_reaches_the_rows_that_see_it_and_no_other(dtype):
     assert bool(torch.isnan(hira_shared_attention(q, pk * float("nan"), pv)).all())
 
 
+def _in_long_buffer(q, *rows):
+    """The prompts' rows at the front of buffers so long (and NaN behind them) that their tiles go to the tcgen05 kernel, which few
+    rows and keys do not; and how many of them there are."""
+    p, h, n, _ = rows[0].shape
+    blocks = -(-q.shape[0] // p * (q.shape[1] // h) * q.shape[2] // 16)
+    room = max(n, 1280 * 148 // (blocks * p * h) + 1)
+    out = []
+    for t in rows:
+        buf = torch.full((p, h, room, t.shape[3]), float("nan"), dtype=t.dtype, device="cuda")
+        buf[:, :, :n] = t
+        out.append(buf)
+    return (*out, [n] * p)
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if max(s[5], s[6]) <= 128], ids=lambda s: "x".join(map(str, s)))
+def test_short_prompts_in_long_buffers(shape):
+    q, pk, pv, tk, tv = _qkv(*shape, torch.bfloat16, seed=91)
+    bk, bv, lens = _in_long_buffer(q, pk, pv)
+    _check(hira_shared_attention(q, bk, bv, tk, tv, prefix_lens=lens), _exact(q, pk, pv, tk, tv))
+    _check(hira_shared_attention(q, bk, bv, prefix_lens=lens), _exact(q, pk, pv, None, None))
+    for scaling in (-0.11, 0.0):
+        _check(hira_shared_attention(q, bk, bv, tk, tv, prefix_lens=lens, scaling=scaling), _exact(q, pk, pv, tk, tv, scaling=scaling))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [2, 17])
+def test_lengths_in_long_buffers(n, d):
+    p, h, g, lq, tail = 6, 2, 4, 2, 5
+    lens = [0, 1, 127, 128, 129, 390]
+    q, pk, pv, tk, tv = _qkv(p, n, h, g, lq, d, d, 390, tail, torch.bfloat16, seed=92)
+    for a, ln in enumerate(lens):
+        pk[a, :, ln:], pv[a, :, ln:] = float("nan"), float("inf")
+    bk, bv, _ = _in_long_buffer(q, pk, pv)
+    tl = [i % (tail + 1) for i in range(p * n)]
+    got = hira_shared_attention(q, bk, bv, tk, tv, prefix_lens=torch.tensor(lens, device="cuda"), tail_lens=tl)
+    _check(got, _exact(q, pk, pv, tk, tv, lens, tl))
+    assert (got[0] == 0).all()                   # no key in sight
+    tokens_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, bk, bv, tk, tv)]
+    out = torch.full((p * n, lq, h * g, d), float("nan"), dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    assert torch.equal(hira_shared_attention(*tokens_first, prefix_lens=lens, tail_lens=tl, out=out), got)
+
+
+def test_logits_and_nans_in_long_buffers():
+    q, pk, pv, tk, tv = _qkv(1, 5, 2, 4, 1, 128, 128, 700, 40, torch.bfloat16, seed=93)
+    bk, bv, lens = _in_long_buffer(q, pk, pv)
+    for f in (30.0, -30.0):
+        _check(hira_shared_attention(q * f, bk, bv, tk, tv, prefix_lens=lens), _exact(q * f, pk, pv, tk, tv))
+    up = torch.linspace(-20, 20, 700, device="cuda").view(1, 1, 700, 1)      # the running maximum moves on in every tile
+    pk2 = (torch.nn.functional.normalize(q[:1, :1].float(), dim=-1) * up).to(torch.bfloat16).expand_as(pk)
+    bk2, _, _ = _in_long_buffer(q, pk2, pv)
+    _check(hira_shared_attention(q, bk2, bv, tk, tv, prefix_lens=lens), _exact(q, pk2, pv, tk, tv))
+    good = hira_shared_attention(q, bk, bv, tk, tv, prefix_lens=lens)
+    bk[0, 1, 300, 7] = float("nan")
+    got = hira_shared_attention(q, bk, bv, tk, tv, prefix_lens=lens)
+    assert torch.equal(got[:, :4], good[:, :4]) and bool(torch.isnan(got[:, 4:]).all())
+    bk[0, 1, 300, 7] = 0.0
+    static = [x.clone() for x in (q, tk, tv)]
+    want = hira_shared_attention(q, bk, bv, tk, tv, prefix_lens=lens)
+    dev_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(hira_shared_attention(static[0], bk, bv, *static[1:], prefix_lens=dev_lens))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):                            # two at once
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_prefix_beyond_two_gibi_elements():
     h, d, ctx = 1, 128, (1 << 24) + 77         # 2^31 elements and more: offsets beyond 32 bits
     k = torch.zeros((1, h, ctx, d), dtype=torch.bfloat16, device="cuda")
