@@ -7,6 +7,7 @@ and key head (where the model has one) and the rotation by position, fifteen or 
 """
 from __future__ import annotations
 
+import copy
 from types import MethodType
 from typing import Optional
 
@@ -156,28 +157,142 @@ def _is_head_rms_norm(norm, width: int) -> bool:
     return bool(((got - want).abs() <= 2 * torch.finfo(w.dtype).eps * want.abs() + 1e-6).all())
 
 
+_PARTS = ("q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm")
+
+
+def _known_difference(m) -> Optional[str]:
+    """What a layer says of itself that a HiraCache's attention does not do: where it stands on the layer, and where the layer
+    has no word of its own, in its config (whose mask or kernel arguments a single forward does not show)."""
+    config = getattr(m, "config", None)
+    for name in ("sliding_window", "attention_chunk_size", "attn_logit_softcapping", "sinks", "clip_qkv"):
+        if name == "sliding_window" and not hasattr(m, name) and not getattr(config, "use_sliding_window", True):
+            continue
+        if (getattr(m, name) if hasattr(m, name) else getattr(config, name, None) if name != "attention_chunk_size" else None) is not None:
+            return f"has {name}, which a HiraCache's attention does not know"
+    types = getattr(config, "layer_types", None)
+    if types is not None and isinstance(m.layer_idx, int) and m.layer_idx < len(types) \
+            and types[m.layer_idx] not in ("full_attention", "attention", "hybrid"):
+        return f"is of type {types[m.layer_idx]}, which a HiraCache's attention does not know"
+    if types is None and getattr(config, "attention_chunk_size", None) is not None:
+        return "has attention_chunk_size, which a HiraCache's attention does not know"
+    if not getattr(m, "use_rope", True):
+        return "does not rotate its heads"
+    if not getattr(m, "is_causal", True):
+        return "is not causal"
+    for name, _ in (*m.named_parameters(), *m.named_buffers()):
+        if name.split(".")[0] not in _PARTS and "inv_freq" not in name:      # frequencies: the rotation is compared anyway
+            return f"has {name}, which hira_attention_forward does not use"
+    return None
+
+
+def _rotated(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    """The rotation of `hira_qk_norm_rope`, in elementary operations."""
+    r = cos.shape[-1]
+    t = x[..., :r]
+    if interleaved:
+        other = torch.stack([-t[..., 1::2], t[..., 0::2]], dim=-1).flatten(-2)
+    else:
+        other = torch.cat([-t[..., r // 2:], t[..., :r // 2]], dim=-1)
+    return torch.cat([t * cos[:, None] + other * sin[:, None], x[..., r:]], dim=-1)
+
+
+def _plain_forward(m, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool, norms: bool) -> torch.Tensor:
+    """What `hira_attention_forward` makes of a prompt, in elementary operations; cos None: the scores before rotation and softmax."""
+    b, n, _ = x.shape
+    q, k, v = (proj(x).view(b, n, -1, m.head_dim).transpose(1, 2) for proj in (m.q_proj, m.k_proj, m.v_proj))
+    if norms:
+        q, k = (t if norm is None else norm(t) for t, norm in ((q, getattr(m, "q_norm", None)), (k, getattr(m, "k_norm", None))))
+    if cos is not None:
+        q, k = _rotated(q, cos, sin, interleaved), _rotated(k, cos, sin, interleaved)
+    scaling = getattr(m, "scaling", None)
+    s = (m.head_dim ** -0.5 if scaling is None else scaling) * (q @ k.repeat_interleave(q.shape[1] // k.shape[1], dim=1).transpose(-1, -2))
+    if cos is None:
+        return s
+    s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=x.device).triu(1), float("-inf"))
+    o = torch.softmax(s, dim=-1) @ v.repeat_interleave(q.shape[1] // v.shape[1], dim=1)
+    return m.o_proj(o.transpose(1, 2).reshape(b, n, -1))
+
+
+@torch.no_grad()
+def _own_forward_differs(layer, widths, interleaved: bool) -> Optional[str]:
+    """Runs a copy of the layer with the forward of its class and with `_plain_forward` on a few random tokens in 64 bits, and
+    says what is wrong where they disagree.  The tables have a value of its own for every channel, so that another pairing of
+    the channels, or another use of the tables, shows; logits of about 2 and of about 200, so that a cap or a clip shows.
+    `widths`: numbers of rotated channels that the model may use.  A layer without a forward has nothing to disagree with."""
+    own = type(layer).forward
+    if own is torch.nn.Module.forward:
+        return None
+    why = None
+    try:
+        m = copy.deepcopy(layer).double().eval()
+        if hasattr(getattr(m, "config", None), "_attn_implementation"):
+            m.config._attn_implementation = "eager"
+        w, n = m.q_proj.weight, 7
+        g = torch.Generator().manual_seed(1)
+
+        def rnd(*shape):
+            return torch.randn(shape, generator=g, dtype=torch.float64).to(w.device)
+        x = rnd(1, n, w.shape[1])
+        mask = torch.full((1, 1, n, n), torch.finfo(torch.float64).min, dtype=torch.float64, device=w.device).triu(1)
+        std = float(_plain_forward(m, x, None, None, interleaved, True).std())
+        for r in widths:
+            cos, sin = rnd(1, n, r).tanh(), rnd(1, n, r).tanh()
+            # norms that were added to a layer whose own forward has none are `hira_attention_forward`'s to apply
+            equal = {True: True, False: getattr(m, "q_norm", None) is not None or getattr(m, "k_norm", None) is not None}
+            try:
+                for logit in (2.0, 200.0):
+                    y = x * (min(max((logit / std) ** 0.5, 1e-3), 1e3) if std > 0 else 1.0)
+                    got = own(m, hidden_states=y, position_embeddings=(cos, sin), attention_mask=mask, past_key_values=None)
+                    got = got[0] if isinstance(got, (tuple, list)) else got
+                    for norms in equal:
+                        want = _plain_forward(m, y, cos, sin, interleaved, norms)
+                        # layers do parts of this in 32 bits: 2^-24 of logits of some 1000, more than ten times over
+                        equal[norms] = equal[norms] and bool(((got - want).norm() <= 1e-3 * want.norm() + 1e-30))
+            except Exception as e:          # of this width; whatever a class's forward may raise
+                why = why or f"cannot be compared with its own forward ({type(e).__name__}: {e})"
+                continue
+            if any(equal.values()):
+                return None
+            why = "computes something else than hira_attention_forward"
+    except Exception as e:
+        why = f"cannot be compared with its own forward ({type(e).__name__}: {e})"
+    return why
+
+
+def _rotary_widths(model, m) -> list:
+    """How many channels a layer may rotate: as its model's tables say, as its config says, all."""
+    widths = [2 * b.numel() for name, b in model.named_buffers() if name.split(".")[-1] == "inv_freq"]
+    config = getattr(m, "config", None)
+    for src in (getattr(config, "rope_parameters", None) or {}, getattr(config, "__dict__", {})):
+        if src.get("partial_rotary_factor"):
+            widths.append(int(m.head_dim * src["partial_rotary_factor"]))
+    return [r for r in dict.fromkeys([*widths, m.head_dim]) if 0 < r <= m.head_dim and r % 2 == 0]
+
+
 def patch_attention(model, hira_config=None, *, interleaved: bool = False) -> int:
     """Gives every attention layer of `model` (a module with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx)
     `hira_attention_forward` as its forward; returns how many there were.  Run the model under `torch.no_grad()` with
-    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.  Layers that compute
-    something else are refused: other norms than RMS norms of single heads, sliding windows, capped logits, sinks, no
-    rotation."""
+    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.
+
+    A layer that computes something else is refused, and then no layer is changed: sliding windows, chunks, capped logits, sinks,
+    no rotation, other norms than RMS norms of single heads, parameters that the new forward does not use; and any layer whose
+    own forward disagrees with the new one on a few random tokens, which are run in 64 bits on a copy of each layer (another
+    pairing of the channels than `interleaved` says is found that way).  q_norm and k_norm that were added to a layer whose own
+    forward has none are applied."""
     layers = [m for m in model.modules()
               if all(hasattr(m, a) for a in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "layer_idx"))]
     if not layers:
         raise ValueError("the model has no attention layer with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx")
     for m in layers:
-        for name in ("sliding_window", "attn_logit_softcapping", "sinks"):
-            if getattr(m, name, None) is not None:
-                raise ValueError(f"layer {m.layer_idx} has {name}, which a HiraCache's attention does not know")
-        if not getattr(m, "use_rope", True):
-            raise ValueError(f"layer {m.layer_idx} does not rotate its heads")
-        for name in ("q_norm", "k_norm"):
-            norm = getattr(m, name, None)
-            if norm is None:
-                continue
-            if not _is_head_rms_norm(norm, m.head_dim):
-                raise ValueError(f"{name} of layer {m.layer_idx} is no RMS norm of single heads")
+        why = _known_difference(m)
+        if why is None:
+            for name in ("q_norm", "k_norm"):
+                norm = getattr(m, name, None)
+                if norm is not None and not _is_head_rms_norm(norm, m.head_dim):
+                    raise ValueError(f"{name} of layer {m.layer_idx} is no RMS norm of single heads")
+            why = _own_forward_differs(m, _rotary_widths(model, m), bool(interleaved))
+        if why is not None:
+            raise ValueError(f"layer {m.layer_idx} {why}" + (f" with interleaved={bool(interleaved)}" if "something else" in why else ""))
     for m in layers:
         def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
             return hira_attention_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values,
