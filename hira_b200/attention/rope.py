@@ -47,9 +47,10 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
                       interleaved: bool = False, out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
     """query (B, H_q, L, D), key (B, H_kv, L, D) -> the two normalised and rotated, in their type.
 
-    `cos`, `sin` (B or 1, L, R) or (L, R), R <= D even: the tables of the first R channels as models hand them out
-    (each pair's value twice); channels i and i + R/2 form a pair, or 2i and 2i + 1 when `interleaved`.  The channels
-    behind R are not rotated.  `q_weight` / `k_weight` (D,): RMS norm of that side's heads with this weight; None:
+    `cos`, `sin` (B or 1, L, R) or (L, R), R <= D even: tables with the factors of each of the first R channels at that
+    channel's own place; channels i and i + R/2 form a pair, or 2i and 2i + 1 when `interleaved`.  (Some models that pair 2i and 2i + 1 hand
+    out tables with the pair's value at i and i + R/2: those have to be laid out by channel first, as `hira_attention_forward`
+    does with `table_halves`.)  The channels behind R are not rotated.  `q_weight` / `k_weight` (D,): RMS norm of that side's heads with this weight; None:
     no norm.  Computed in fp32 and rounded once.
 
     fp32 or bf16; D a multiple of 8 up to 256.  Any strides with contiguous, 16-byte aligned rows (a projection's
@@ -117,10 +118,17 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     return plan(*args, oq, ok)
 
 
+def _by_channel(t: torch.Tensor) -> torch.Tensor:
+    """A table that holds pair i's value at i (and again at i + R/2) as one that holds it at 2i and 2i + 1."""
+    return t[..., :t.shape[-1] // 2].unsqueeze(-1).expand(*t.shape[:-1], t.shape[-1] // 2, 2).flatten(-2)
+
+
 def hira_attention_forward(module, hidden_states: torch.Tensor, position_embeddings, attention_mask: Optional[torch.Tensor] = None,
-                           past_key_values=None, hira_config=None, interleaved: bool = False, **kwargs):
+                           past_key_values=None, hira_config=None, interleaved: bool = False, table_halves: bool = False, **kwargs):
     """Forward of a decoder's attention layer over a HiraCache.  `module` has q_proj, k_proj, v_proj, o_proj, head_dim
-    and layer_idx, and may have q_norm and k_norm (RMS norms of single heads: `weight` (head_dim,) and an epsilon)."""
+    and layer_idx, and may have q_norm and k_norm (RMS norms of single heads: `weight` (head_dim,) and an epsilon).
+    `table_halves`: the model pairs channels 2i and 2i + 1 (`interleaved`), but its tables hold the pair's value at i and
+    i + R/2, as if it paired those."""
     from .hira_attention import hira_attention
     if past_key_values is None:
         raise ValueError("hira_attention_forward needs a HiraCache as past_key_values")
@@ -131,6 +139,8 @@ def hira_attention_forward(module, hidden_states: torch.Tensor, position_embeddi
     q, k, v = heads(module.q_proj), heads(module.k_proj), heads(module.v_proj)
     q_norm, k_norm = getattr(module, "q_norm", None), getattr(module, "k_norm", None)
     cos, sin = position_embeddings
+    if interleaved and table_halves:
+        cos, sin = _by_channel(cos), _by_channel(sin)
     eps = {getattr(m, "variance_epsilon", getattr(m, "eps", None)) for m in (q_norm, k_norm) if m is not None}
     if len(eps) > 1:
         raise ValueError(f"q_norm and k_norm have different epsilons: {sorted(eps)}")
@@ -214,7 +224,7 @@ def _plain_forward(m, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, int
 
 
 @torch.no_grad()
-def _own_forward_differs(layer, widths, interleaved: bool) -> Optional[str]:
+def _own_forward_differs(layer, widths, interleaved: bool, table_halves: bool) -> Optional[str]:
     """Runs a copy of the layer with the forward of its class and with `_plain_forward` on a few random tokens in 64 bits, and
     says what is wrong where they disagree.  The tables have a value of its own for every channel, so that another pairing of
     the channels, or another use of the tables, shows; logits of about 2 and of about 200, so that a cap or a clip shows.
@@ -244,8 +254,9 @@ def _own_forward_differs(layer, widths, interleaved: bool) -> Optional[str]:
                     y = x * (min(max((logit / std) ** 0.5, 1e-3), 1e3) if std > 0 else 1.0)
                     got = own(m, hidden_states=y, position_embeddings=(cos, sin), attention_mask=mask, past_key_values=None)
                     got = got[0] if isinstance(got, (tuple, list)) else got
+                    tables = (_by_channel(cos), _by_channel(sin)) if table_halves else (cos, sin)
                     for norms in equal:
-                        want = _plain_forward(m, y, cos, sin, interleaved, norms)
+                        want = _plain_forward(m, y, *tables, interleaved, norms)
                         # layers do parts of this in 32 bits: 2^-24 of logits of some 1000, more than ten times over
                         equal[norms] = equal[norms] and bool(((got - want).norm() <= 1e-3 * want.norm() + 1e-30))
             except Exception as e:          # of this width; whatever a class's forward may raise
@@ -272,7 +283,8 @@ def _rotary_widths(model, m) -> list:
 def patch_attention(model, hira_config=None, *, interleaved: bool = False) -> int:
     """Gives every attention layer of `model` (a module with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx)
     `hira_attention_forward` as its forward; returns how many there were.  Run the model under `torch.no_grad()` with
-    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.
+    a HiraCache as `past_key_values`.  `interleaved`: how the model pairs the channels it rotates.  How the tables of an
+    interleaved model are laid out (`hira_attention_forward`'s `table_halves`) is found out from its layers.
 
     A layer that computes something else is refused, and then no layer is changed: sliding windows, chunks, capped logits, sinks,
     no rotation, other norms than RMS norms of single heads, parameters that the new forward does not use; and any layer whose
@@ -283,6 +295,7 @@ def patch_attention(model, hira_config=None, *, interleaved: bool = False) -> in
               if all(hasattr(m, a) for a in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "layer_idx"))]
     if not layers:
         raise ValueError("the model has no attention layer with q_proj, k_proj, v_proj, o_proj, head_dim and layer_idx")
+    halves = []
     for m in layers:
         why = _known_difference(m)
         if why is None:
@@ -290,12 +303,16 @@ def patch_attention(model, hira_config=None, *, interleaved: bool = False) -> in
                 norm = getattr(m, name, None)
                 if norm is not None and not _is_head_rms_norm(norm, m.head_dim):
                     raise ValueError(f"{name} of layer {m.layer_idx} is no RMS norm of single heads")
-            why = _own_forward_differs(m, _rotary_widths(model, m), bool(interleaved))
+            widths = _rotary_widths(model, m)
+            why = _own_forward_differs(m, widths, bool(interleaved), False)
+            halves.append(bool(interleaved and why and _own_forward_differs(m, widths, True, True) is None))
+            if halves[-1]:
+                why = None
         if why is not None:
             raise ValueError(f"layer {m.layer_idx} {why}" + (f" with interleaved={bool(interleaved)}" if "something else" in why else ""))
-    for m in layers:
-        def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+    for m, by_half in zip(layers, halves):
+        def forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, _halves=by_half, **kwargs):
             return hira_attention_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values,
-                                          hira_config=hira_config, interleaved=interleaved, **kwargs)
+                                          hira_config=hira_config, interleaved=interleaved, table_halves=_halves, **kwargs)
         m.forward = MethodType(forward, m)
     return len(layers)

@@ -127,6 +127,8 @@ def _with(layer):
                                  "no_rotation", "table_halves"])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_layers_whose_own_forward_differs_are_refused_and_none_is_changed(odd, interleaved):
+    if odd == "table_halves" and interleaved:
+        pytest.skip("taken: test_tables_by_halves_of_interleaved_layers_are_found")
     pairs = _neighbours if interleaved or odd == "table_halves" else _halves
     first, layer = _Layer(pairs=pairs), _Layer(odd, pairs=pairs)
     model = torch.nn.ModuleList([first, layer])
@@ -172,3 +174,17 @@ def test_layers_that_cannot_be_compared_are_refused():
 
 def test_norms_added_to_a_layer_without_any_are_accepted():
     assert patch_attention(_with(_Layer("norms_unused", head_norms=True))) == 2
+
+
+def test_tables_by_halves_of_interleaved_layers_are_found(monkeypatch):
+    from hira_b200.attention import rope
+    seen = []
+    monkeypatch.setattr(rope, "hira_attention_forward", lambda *a, **kw: seen.append((kw["interleaved"], kw["table_halves"])))
+    model = torch.nn.ModuleList([_Layer(pairs=_neighbours), _Layer("table_halves", pairs=_neighbours, rotary=8)])
+    model.register_buffer("inv_freq", torch.ones(4))
+    assert patch_attention(model, interleaved=True) == 2
+    for m in model:
+        m.forward(torch.zeros(1, 1, HIDDEN), (None, None))
+    assert seen == [(True, False), (True, True)]
+    t = torch.arange(6.0).view(1, 1, 6)
+    assert rope._by_channel(t).tolist() == [[[0, 0, 1, 1, 2, 2]]]
