@@ -138,7 +138,8 @@ class IndexState:
         return self._byref
 
     def like(self, n_heads: int) -> "IndexState":
-        """A state of the same shape for another number of heads; its arrays (and its status) are not filled."""
+        """A state of the same shape for another number of heads; its arrays (and its status) are not filled.  It uses the
+        int8 copy where this one does: a copy that is switched off is not kept up by the appends."""
         new = object.__new__(type(self))
         d = new.__dict__
         d.update(self.__dict__)
@@ -148,7 +149,8 @@ class IndexState:
             t = d[name]
             if t is not None:
                 t = d[name] = t.new_empty((n_heads, *t.shape[1:]))
-                setattr(s, name, t.data_ptr())
+                if name not in self.Q8_ARRAYS or self._struct.children_q8:
+                    setattr(s, name, t.data_ptr())
         s.n_heads = new.n_heads = n_heads
         new.status = torch.empty_like(self.status)
         new._append_bytes, new._append_ws = {}, (None, 0)

@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from hira_b200 import HiraCacheLayer, patch_attention
+from hira_b200 import CUDAIndexer, HiraCacheLayer, patch_attention
+from hira_b200 import _lib as L
+from hira_b200 import index_state as S
 from test_patched_layers_host import D, HIDDEN, _Layer, _neighbours
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +36,25 @@ def test_interleaved_layers_rotate_as_their_own_forward_does(odd, rotary):
     assert patch_attention(model, interleaved=True) == 1
     got = layer(x, position_embeddings=(angle.cos(), angle.sin()), past_key_values=_cache_of_one_layer())[0]
     torch.testing.assert_close(got, want, atol=1e-4, rtol=1e-3)
+
+
+@pytest.mark.parametrize("depth", [2, 3])
+def test_a_fork_of_an_index_without_its_int8_copy_finds_the_keys_appended_since(depth):
+    """The appends do not keep up a copy that is switched off, so a fork must not search by it."""
+    gen = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((2, 2, 600, 128), generator=gen).bfloat16().cuda() for _ in range(2))
+    ix = CUDAIndexer(depth, 1, 16, max_context=626).build(k, v)
+    assert ix.state.cap_parents % 64 == 0        # whole tiles, which the search by the copy needs
+    ix.state.enable_int8_copy(False)
+    new = k[:, :, :4] * 3
+    ix.update(new, v[:, :, :4])
+    q = torch.nn.functional.normalize(new.float(), dim=-1)           # four queries a head, each along a new key
+    tau = torch.full((16,), 15.0, device="cuda")
+    flags = L.HIRA_GATE_GE | L.HIRA_LEAF_GE
+    picks = [1, 0]
+    fork = ix.select(picks)
+    got = S.search(fork.state, q[picks].reshape(16, 128), tau, flags=flags, want_compact=True)[1].to_lists()
+    want = S.search(ix.state, q.reshape(16, 128), tau, flags=flags, want_compact=True)[1].to_lists()
+    for i in range(16):
+        j = picks[i // 8] * 8 + i % 8
+        assert len(want[j][0]) > 0 and torch.equal(got[i][0], want[j][0]) and torch.equal(got[i][1], want[j][1])
