@@ -197,12 +197,14 @@ class IndexState:
                          cap_parents=new_cap_parents, dtype=self.dtype, vdtype=self.vdtype, device=self.device,
                          with_values=self.values is not None, int8_copy=self.int8_copy, cleared=self.device.type != "cuda")
         new.status.copy_(self.status)
+        in_use = bool(self._struct.children_q8)        # a copy that is switched off is not kept up by the appends
         if self.device.type == "cuda":
             self.used_on(torch.cuda.current_stream(self.device))     # the caller drops the old arrays right away
             old = L.HiraIndexStruct.from_buffer_copy(self._struct)
             for name in self.Q8_ARRAYS:     # also when enable_int8_copy has left them out of the view
                 setattr(old, name, L.ptr(getattr(self, name)))
             L.check(L.load().hira_grow(C.byref(old), new.struct, L.current_stream(self.device)), "hira_grow")
+            new.enable_int8_copy(in_use)
             return new
         for name in self.ARRAYS + self.Q8_ARRAYS:
             src = getattr(self, name)
@@ -213,6 +215,7 @@ class IndexState:
                 continue
             getattr(new, name)[:, : src.shape[1]].copy_(src)
         new.used.copy_(self.used)
+        new.enable_int8_copy(in_use)
         return new
 
 

@@ -209,3 +209,12 @@ def test_a_forked_state_uses_the_int8_copy_only_if_its_source_does(on):
     assert all(bool(getattr(b._struct, n)) == on for n in S.IndexState.Q8_ARRAYS) and b.children_q8.shape[0] == 6
     b.enable_int8_copy(True)
     assert b._struct.children_q8 == b.children_q8.data_ptr() and bool(a._struct.children_q8) == on
+
+
+@pytest.mark.parametrize("on", [True, False])
+def test_a_grown_state_uses_the_int8_copy_only_if_it_did_before(on):
+    a = S.IndexState(n_heads=2, dim=128, vdim=128, bf=8, depth=2, cap_parents=16, dtype=torch.float32, vdtype=torch.float32, device="cpu",
+                     int8_copy=True)
+    a.enable_int8_copy(on)
+    b = a.grown(32)
+    assert b.cap_parents == 32 and all(bool(getattr(b._struct, n)) == on for n in S.IndexState.Q8_ARRAYS)
