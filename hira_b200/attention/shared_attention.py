@@ -44,6 +44,8 @@ def _lengths(lens, n: int, most: int, device, what: str) -> Optional[torch.Tenso
         raise ValueError(f"{what} must be ({n},) whole numbers, got {tuple(t.shape)} {t.dtype}")
     if not t.is_cuda and n and not (0 <= int(t.min()) and int(t.max()) <= most):
         raise ValueError(f"{what} outside 0..{most}: {t.tolist()}")
+    if t.is_cuda and t.dtype in (torch.int64, torch.uint32):
+        t = t.to(torch.int64).clamp(0, most)          # before 32 bits cut it elsewhere
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 

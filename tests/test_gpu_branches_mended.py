@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from hira_b200 import CUDAIndexer, HiraCacheLayer, patch_attention
+from hira_b200 import CUDAIndexer, HiraCacheLayer, SharedPrompt, hira_shared_attention, patch_attention
 from hira_b200 import _lib as L
 from hira_b200 import index_state as S
 from test_patched_layers_host import D, HIDDEN, _Layer, _neighbours
@@ -58,3 +58,16 @@ def test_a_fork_of_an_index_without_its_int8_copy_finds_the_keys_appended_since(
     for i in range(16):
         j = picks[i // 8] * 8 + i % 8
         assert len(want[j][0]) > 0 and torch.equal(got[i][0], want[j][0]) and torch.equal(got[i][1], want[j][1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lengths_beyond_32_bits_are_cut_like_others(dtype):
+    gen = torch.Generator().manual_seed(2)
+    q, pk, pv, tk, tv = (torch.randn(s, generator=gen).to(dtype).cuda()
+                         for s in ((4, 2, 1, 64), (2, 1, 90, 64), (2, 1, 90, 64), (4, 1, 9, 64), (4, 1, 9, 64)))
+    want = hira_shared_attention(q, pk, pv, tk, tv, prefix_lens=[90, 0], tail_lens=[9, 9, 0, 3])
+    far = torch.tensor([2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31, -2 ** 31 - 1], device="cuda")
+    got = hira_shared_attention(q, pk, pv, tk, tv, prefix_lens=far[:2], tail_lens=torch.stack([far[0], far[2], far[3], far.new_tensor(3)]))
+    assert torch.equal(got, want)
+    prompt = SharedPrompt(pk, pv, 2, prefix_lens=far[:2]).append(tk, tv)
+    assert torch.equal(prompt.attend(q), hira_shared_attention(q, pk, pv, tk, tv, prefix_lens=[90, 0]))
