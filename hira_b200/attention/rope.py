@@ -24,12 +24,20 @@ def _layout(t: torch.Tensor):
     return t.shape, t.stride(), t.dtype, t.get_device()
 
 
-def _check_apart(o: torch.Tensor, x: torch.Tensor, other: torch.Tensor, name: str):
-    if o.data_ptr() == x.data_ptr() and o.stride() == x.stride() and (other.data_ptr() != x.data_ptr() or not o.numel()):
-        return
-    own = o.untyped_storage().data_ptr()
-    if own == x.untyped_storage().data_ptr() or own == other.untyped_storage().data_ptr():
-        raise ValueError(f"{name} must be its own input or memory apart from both inputs")
+def _check_apart(query, key, out_q, out_k, reads):
+    """Rows are read by many threads while others write: an output is its own input, or shares no byte with what is read or written
+    beside it."""
+    for name, o, x, other in (("out_q", out_q, query, key), ("out_k", out_k, key, query)):
+        if o is None:
+            continue
+        same = o.data_ptr() == x.data_ptr() and S.row_strides(o) == S.row_strides(x)
+        if not same and S.share_memory(o, x) or S.share_memory(o, other):
+            raise ValueError(f"{name} must be its own input or memory apart from both inputs")
+        for what, t in reads:
+            if t is not None and S.share_memory(o, t):
+                raise ValueError(f"{name} must be memory apart from {what}")
+    if out_q is not None and out_k is not None and S.share_memory(out_q, out_k):
+        raise ValueError("out_q and out_k are the same memory, at least in part")
 
 
 def _table(t: torch.Tensor, b: int, n: int, name: str) -> torch.Tensor:
@@ -55,7 +63,8 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
 
     fp32 or bf16; D a multiple of 8 up to 256.  Any strides with contiguous, 16-byte aligned rows (a projection's
     transposed view as it is); others are copied.  `out_q` / `out_k`: where to write, with such rows: the input itself,
-    or memory apart from both inputs (part of a cache, say).  No backward pass."""
+    or memory apart from all that the call reads and from one another (part of a cache, say; the heads of one projection
+    are apart although they lie between each other).  No backward pass."""
     if torch.is_grad_enabled():
         refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
     eps, interleaved = float(eps), bool(interleaved)
@@ -66,13 +75,10 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
               None if out_q is None else _layout(out_q), None if out_k is None else _layout(out_k), eps, interleaved)
     plan = _plans.get(layout)
     if plan is not None:
-        if out_q is not None:
-            _check_apart(out_q, query, key, "out_q")
-        if out_k is not None:
-            _check_apart(out_k, key, query, "out_k")
-            if out_q is not None and out_q.data_ptr() == out_k.data_ptr() and out_q.numel():
-                raise ValueError("out_q and out_k are the same memory")
         done = plan(query, key, cos, sin, q_weight, k_weight, out_q, out_k)
+        if done is None and (out_q is not None or out_k is not None):      # address ranges that meet
+            _check_apart(query, key, out_q, out_k, (("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight)))
+            done = plan(query, key, cos, sin, q_weight, k_weight, out_q, out_k, apart=True)
         if done is not None:
             return done
     if query.ndim != 4 or key.ndim != 4:
@@ -103,9 +109,7 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
             continue
         if o.shape != x.shape or o.dtype != x.dtype or not S.writable_rows(o):
             raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype} with aligned contiguous rows")
-        _check_apart(o, x, key if x is query else query, name)
-    if out_q is not None and out_k is not None and out_q.numel() and out_q.data_ptr() == out_k.data_ptr():
-        raise ValueError("out_q and out_k are the same memory")
+    _check_apart(query, key, out_q, out_k, (("cos", given[0]), ("sin", given[1]), ("q_weight", q_weight), ("k_weight", k_weight)))
     if not query.is_cuda:
         raise ValueError("hira_qk_norm_rope needs CUDA tensors (there is no CPU fallback)")
     args = (S.with_rows(query), S.with_rows(key), cos, sin, *(None if w is None else S.aligned(w.contiguous()) for w in (q_weight, k_weight)))
@@ -115,7 +119,7 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     plan = S.RopePlan(*args[:4], eps, interleaved, oq, ok)
     if as_given:
         S.remember(_plans, layout, plan)
-    return plan(*args, oq, ok)
+    return plan(*args, oq, ok, apart=True)
 
 
 def _by_channel(t: torch.Tensor) -> torch.Tensor:

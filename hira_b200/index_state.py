@@ -11,6 +11,7 @@ from dataclasses import dataclass
 from functools import lru_cache
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -627,8 +628,53 @@ def row_strides(t: torch.Tensor) -> Optional[tuple]:
 
 
 def writable_rows(t: torch.Tensor) -> bool:
-    """Whether rows can be written to `t`: as `row_strides`, and no two of them the same."""
-    return row_strides(t) is not None and all(s for n, s in zip(t.shape, t.stride()) if n > 1)
+    """Whether rows can be written to `t`: as `row_strides`, and no two of them seen to share an element (each stride steps over
+    all that the smaller ones reach)."""
+    if row_strides(t) is None:
+        return False
+    reach = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s < reach:
+            return False
+        reach += (n - 1) * s
+    return True
+
+
+def spanned_bytes(t: torch.Tensor) -> int:
+    """From the first byte of `t` to behind its last."""
+    if not t.numel():
+        return 0
+    return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+class _Layout:
+    """A tensor's layout from an address on, for numpy's arithmetic on it; nothing is read there."""
+
+    def __init__(self, address: int, t: torch.Tensor):
+        e = t.element_size()
+        self.__array_interface__ = {"data": (address, False), "shape": tuple(t.shape), "strides": tuple(s * e for s in t.stride()),
+                                    "typestr": f"|V{e}", "version": 3}
+
+
+_shared = {}
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one device have a byte in common.  (Views of one buffer need not: the heads of a fused
+    projection lie between each other.)  What cannot be decided quickly counts as shared."""
+    pa, pb, na, nb = a.data_ptr(), b.data_ptr(), spanned_bytes(a), spanned_bytes(b)
+    if not na or not nb or pa + na <= pb or pb + nb <= pa:
+        return False
+    key = pb - pa, a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype
+    known = _shared.get(key)
+    if known is None:
+        base = max(0, pa - pb) + 4096
+        try:
+            known = bool(np.shares_memory(np.asarray(_Layout(base, a)), np.asarray(_Layout(base + pb - pa, b)), max_work=1 << 16))
+        except np.exceptions.TooHardError:
+            known = True
+        remember(_shared, key, known)
+    return known
 
 
 def with_rows(t: torch.Tensor) -> torch.Tensor:
@@ -770,9 +816,34 @@ class RopePlan:
         a.dtype, a.table_dtype, a.batch, a.n_tokens = L.dtype_code(q.dtype), L.dtype_code(cos.dtype), b, n
         a.q_heads, a.k_heads, a.dim, a.rotary, a.interleaved, a.eps = hq, k.shape[1], d, cos.shape[2], int(bool(interleaved)), float(eps)
         self.index = q.get_device()
+        self.spans = [spanned_bytes(t) for t in (q, k, out_q, out_k, cos, sin)]
+        self.weight_bytes = d * q.element_size()
+        self.in_place = row_strides(q) == row_strides(out_q), row_strides(k) == row_strides(out_k)
 
-    def __call__(self, q, k, cos, sin, q_weight, k_weight, out_q=None, out_k=None):
-        """None where a tensor does not start on a 16-byte boundary."""
+    def _apart(self, q, k, cos, sin, q_weight, k_weight, out_q, out_k) -> bool:
+        """Whether the address ranges of the given outputs meet no other tensor's, their own input's apart where that is all the same."""
+        nq, nk, noq, nok, ncos, nsin = self.spans
+        reads = [(t.data_ptr(), n) for t, n in ((cos, ncos), (sin, nsin), (q_weight, self.weight_bytes), (k_weight, self.weight_bytes))
+                 if t is not None]
+        pq, pk = q.data_ptr(), k.data_ptr()
+        if out_q is not None:
+            at, end = out_q.data_ptr(), out_q.data_ptr() + noq
+            own = [] if at == pq and self.in_place[0] else [(pq, nq)]
+            if any(p < end and at < p + n for p, n in (*own, (pk, nk), *reads)):
+                return False
+        if out_k is not None:
+            at, end = out_k.data_ptr(), out_k.data_ptr() + nok
+            own = [] if at == pk and self.in_place[1] else [(pk, nk)]
+            other = [] if out_q is None else [(out_q.data_ptr(), noq)]
+            if any(p < end and at < p + n for p, n in (*own, (pq, nq), *other, *reads)):
+                return False
+        return True
+
+    def __call__(self, q, k, cos, sin, q_weight, k_weight, out_q=None, out_k=None, apart: bool = False):
+        """None where a tensor does not start on a 16-byte boundary, or (unless they are known to be `apart`) an output's address
+        range meets another tensor's."""
+        if not apart and (out_q is not None or out_k is not None) and not self._apart(q, k, cos, sin, q_weight, k_weight, out_q, out_k):
+            return None
         if out_q is None:
             out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
         if out_k is None:

@@ -218,3 +218,53 @@ def test_a_grown_state_uses_the_int8_copy_only_if_it_did_before(on):
     a.enable_int8_copy(on)
     b = a.grown(32)
     assert b.cap_parents == 32 and all(bool(getattr(b._struct, n)) == on for n in S.IndexState.Q8_ARRAYS)
+
+
+def test_rotation_refuses_outputs_that_overlap_what_is_read_or_written_beside_them():
+    c = _t(2, 4, 64)
+    q, k, buf = _t(2, 4, 4, 64), _t(2, 2, 4, 64), _t(2, 8, 4, 64)
+    for kw, match in ((dict(out_q=buf[:, :4], out_k=buf[:, 3:5]), "same memory"),
+                      (dict(query=buf[:, :4], key=buf[:, 1:3], out_q=buf[:, :4]), "apart"),
+                      (dict(query=buf[:, :4], key=buf[:, 3:5], out_k=buf[:, 3:5]), "apart"),
+                      (dict(out_q=buf[:, :4], cos=buf[:, 2, :, :]), "apart from cos"),
+                      (dict(out_k=buf[:, :2], k_weight=buf[0, 1, 3]), "apart from k_weight"),
+                      (dict(query=buf[:, :4], key=buf[:, 4:6], out_q=buf[:, 4:]), "apart"),
+                      (dict(out_q=buf.flatten().as_strided((2, 4, 4, 64), (2048, 64, 64, 1))), "out_q must be")):
+        with pytest.raises(ValueError, match=match):
+            hira_qk_norm_rope(**{**dict(query=q, key=k, cos=c, sin=c), **kw})
+    # heads of one projection lie between each other, and part of a buffer beside them: all of them apart
+    fused, tokens = _t(2, 4, 10, 64).transpose(1, 2), _t(2, 9, 6, 64)
+    for kw in (dict(query=fused[:, :4], key=fused[:, 4:6], out_q=fused[:, :4], out_k=fused[:, 4:6]),
+               dict(query=fused[:, :4], key=fused[:, 4:6], out_q=fused[:, 6:], out_k=fused[:, 4:6]),
+               dict(out_q=tokens.transpose(1, 2)[:, :4, 1:5], out_k=tokens.transpose(1, 2)[:, 4:, 1:5]),
+               dict(out_q=tokens.transpose(1, 2)[:, :4, 1:5], out_k=tokens.transpose(1, 2)[:, :2, 5:])):
+        with pytest.raises(ValueError, match="CUDA"):
+            hira_qk_norm_rope(**{**dict(query=q, key=k, cos=c, sin=c), **kw})
+
+
+def test_shared_memory_is_found_byte_by_byte():
+    gen = torch.Generator().manual_seed(0)
+    buf = torch.arange(600, dtype=torch.int32)
+
+    def pick(n):
+        return int(torch.randint(n, (1,), generator=gen))
+    met = 0
+    for _ in range(400):
+        views = []
+        for _ in range(2):
+            shape = [1 + pick(4) for _ in range(3)]
+            stride = [pick(40), pick(12), 1 + pick(2)]
+            views.append(buf.as_strided(shape, stride, pick(200)))
+        a, b = views
+        want = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert S.share_memory(a, b) == want == S.share_memory(b, a)
+        met += want
+    assert 50 < met < 350
+    big, accepted = torch.arange(4000, dtype=torch.int32), 0
+    for _ in range(400):         # what passes as writable has no element twice
+        t = big.as_strided((1 + pick(4), 1 + pick(4), 1 + pick(4), 4), (4 * pick(40), 4 * pick(12), 4 * pick(3), 1))
+        if S.writable_rows(t):
+            accepted += 1
+            assert len(set(t.flatten().tolist())) == t.numel()
+    assert accepted > 40
+    assert S.share_memory(buf.view(torch.int8)[3:4], buf[:1]) and not S.share_memory(buf[:0], buf) and not S.share_memory(buf.clone(), buf)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from hira_b200 import CUDAIndexer, HiraCacheLayer, SharedPrompt, hira_shared_attention, patch_attention
+from hira_b200 import CUDAIndexer, HiraCacheLayer, SharedPrompt, hira_qk_norm_rope, hira_shared_attention, patch_attention
 from hira_b200 import _lib as L
 from hira_b200 import index_state as S
 from test_patched_layers_host import D, HIDDEN, _Layer, _neighbours
@@ -71,3 +71,25 @@ def test_lengths_beyond_32_bits_are_cut_like_others(dtype):
     assert torch.equal(got, want)
     prompt = SharedPrompt(pk, pv, 2, prefix_lens=far[:2]).append(tk, tv)
     assert torch.equal(prompt.attend(q), hira_shared_attention(q, pk, pv, tk, tv, prefix_lens=[90, 0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_heads_of_one_projection_rotate_in_place_and_into_each_other(dtype):
+    """Views that lie between each other share no byte; calls of one layout with outputs at other places."""
+    gen = torch.Generator().manual_seed(3)
+    b, n, d = 2, 5, 64
+    qw, kw = (torch.randn(d, generator=gen).to(dtype).cuda() for _ in range(2))
+    angle = torch.randn((b, n, d), generator=gen).cuda()
+    cos, sin = angle.cos(), angle.sin()
+    for _ in range(3):
+        fused = torch.randn((b, n, 12, d), generator=gen).to(dtype).cuda().transpose(1, 2)
+        q, k, old = fused[:, :4], fused[:, 4:6], fused.clone()
+        want = hira_qk_norm_rope(q.clone(), k.clone(), cos, sin, q_weight=qw, k_weight=kw)
+        hira_qk_norm_rope(q, k, cos, sin, q_weight=qw, k_weight=kw, out_q=fused[:, 6:10], out_k=fused[:, 10:])
+        assert torch.equal(fused[:, :6], old[:, :6]) and torch.equal(fused[:, 6:10], want[0]) and torch.equal(fused[:, 10:], want[1])
+        hira_qk_norm_rope(q, k, cos, sin, q_weight=qw, k_weight=kw, out_q=q, out_k=k)
+        assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(fused[:, 6:10], want[0])
+        with pytest.raises(ValueError, match="apart"):        # the layout of the first call, at another place
+            hira_qk_norm_rope(q, k, cos, sin, q_weight=qw, k_weight=kw, out_q=fused[:, 5:9], out_k=fused[:, 10:])
+        with pytest.raises(ValueError, match="same memory"):
+            hira_qk_norm_rope(q, k, cos, sin, q_weight=qw, k_weight=kw, out_q=fused[:, 6:10], out_k=fused[:, 8:10])
