@@ -16,6 +16,7 @@ from .. import index_state as S
 
 _TYPES = (torch.float32, torch.bfloat16)
 _plans = {}
+_NAMES = ("query", "prefix_keys", "prefix_values", "tail_keys", "tail_values", "prefix_lens", "tail_lens")
 
 
 def _layout(t: Optional[torch.Tensor]):
@@ -49,6 +50,14 @@ def _lengths(lens, n: int, most: int, device, what: str) -> Optional[torch.Tenso
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
+def _check_apart(out, query, named):
+    """Rows are read by some blocks while others write theirs: `out` is the query itself, or shares no byte with what is read."""
+    for name, t in named:
+        if t is not None and torch.is_tensor(t) and t.device == out.device and S.share_memory(out, t) and not (
+                t is query and out.data_ptr() == t.data_ptr() and out.shape == t.shape and S.row_strides(out) == S.row_strides(t)):
+            raise ValueError(f"out must be memory apart from {name}" + (", or the query itself" if t is query else ""))
+
+
 def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix_values: torch.Tensor,
                           tail_keys: Optional[torch.Tensor] = None, tail_values: Optional[torch.Tensor] = None, *,
                           prefix_lens=None, tail_lens=None, scaling: Optional[float] = None,
@@ -66,7 +75,8 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
 
     fp32 or bf16, all of one type; D and V multiples of 8 up to 256; B * H_kv up to 65,535.  fp32 is computed in fp32; bf16 with fp32
     sums and statistics.  Rows have to be contiguous and 16-byte aligned: what is not is copied first.  `out` has
-    to be so.  No backward pass.  A key hidden from one query token but not from another has to be finite."""
+    to be so, and to be the query itself (D = V) or memory apart from all that the call reads.  No backward pass.  A key
+    hidden from one query token but not from another has to be finite."""
     if torch.is_grad_enabled():
         refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
     if scaling is not None:
@@ -81,7 +91,11 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
                   _tail_layout(tail_keys), _tail_layout(tail_values), _layout(prefix_lens), _layout(tail_lens), _layout(out), scaling)
         plan = _plans.get(layout)
         if plan is not None:
-            done = plan(query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens, out)
+            given = (query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
+            done = plan(*given, out)
+            if done is None and out is not None:      # address ranges that meet
+                _check_apart(out, query, zip(_NAMES, given))
+                done = plan(*given, out, apart=True)
             if done is not None:
                 return done
     if (tail_keys is None) != (tail_values is None):
@@ -118,19 +132,21 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     prefix_lens = _lengths(prefix_lens, p, n, query.device, "prefix_lens")
     if tail_keys is not None:
         tail_lens = _lengths(tail_lens, b, tail_keys.shape[2], query.device, "tail_lens")
+    if out is not None:
+        if out.shape != (b, hq, n_q, v) or out.dtype != query.dtype or out.device != query.device or not S.writable_rows(out):
+            raise ValueError(f"out must be ({b}, {hq}, {n_q}, {v}) {query.dtype} on {query.device} with aligned contiguous rows")
+        _check_apart(out, query, zip(_NAMES, given))
     if not query.is_cuda:
         raise ValueError("hira_shared_attention needs CUDA tensors (there is no CPU fallback)")
     if out is None:
         out = torch.empty((b, hq, n_q, v), dtype=query.dtype, device=query.device)
-    elif out.shape != (b, hq, n_q, v) or out.dtype != query.dtype or out.device != query.device or not S.writable_rows(out):
-        raise ValueError(f"out must be ({b}, {hq}, {n_q}, {v}) {query.dtype} on {query.device} with aligned contiguous rows")
     if out.numel() == 0:
         return out
     args = tuple(None if t is None else S.with_rows(t) for t in given[:5]) + (prefix_lens, tail_lens)
     plan = S.SharedAttnPlan(*args[:5], d ** -0.5 if scaling is None else scaling, out)
     if layout is not None and all(a is b for a, b in zip(args, given)):
         S.remember(_plans, layout, plan)
-    return plan(*args, out)
+    return plan(*args, out, apart=True)
 
 
 def _keep(*tensors):

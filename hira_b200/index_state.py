@@ -706,12 +706,29 @@ class SharedAttnPlan:
         a.dtype, a.n_prompts, a.n_branches, a.n_kv, a.group = L.dtype_code(q.dtype), p, b // p, h, hq // h
         a.n_q, a.dim, a.vdim, a.sm_scale = n_q, d, vdim, float(sm_scale)
         self.out_shape, self.device, self.index = (b, hq, n_q, vdim), q.device, q.get_device()
+        self.spans = [spanned_bytes(t) for t in (q, prefix_k, prefix_v, out)]
+        self.in_place = d == vdim and row_strides(q) == row_strides(out)
 
-    def __call__(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out=None):
-        """None where a tensor does not start on a 16-byte boundary."""
+    def _apart(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out) -> bool:
+        """Whether the address range of `out` meets no other tensor's, the query's apart where that is all the same."""
+        nq, nk, nv, no = self.spans
+        at = out.data_ptr()
+        end, pq, pk, pv = at + no, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr()
+        if pk < end and at < pk + nk or pv < end and at < pv + nv or pq < end and at < pq + nq and not (at == pq and self.in_place):
+            return False
+        for t in (tail_k, tail_v, prefix_lens, tail_lens):
+            if t is not None and t.data_ptr() < end and at < t.data_ptr() + spanned_bytes(t):
+                return False
+        return True
+
+    def __call__(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out=None, apart: bool = False):
+        """None where a tensor does not start on a 16-byte boundary, or (unless it is known to be `apart`) the output's address
+        range meets another tensor's."""
         lib = L.load()
         if out is None:
             out = q.new_empty(self.out_shape)
+        elif not apart and not self._apart(q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out):
+            return None
         a = L.HiraSharedAttnStruct.from_buffer_copy(self.args)      # one of its own for every call
         pq, pk, pv, po = q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), out.data_ptr()
         every = pq | pk | pv | po

@@ -268,3 +268,19 @@ def test_shared_memory_is_found_byte_by_byte():
             assert len(set(t.flatten().tolist())) == t.numel()
     assert accepted > 40
     assert S.share_memory(buf.view(torch.int8)[3:4], buf[:1]) and not S.share_memory(buf[:0], buf) and not S.share_memory(buf.clone(), buf)
+
+
+def test_shared_attention_refuses_an_output_that_overlaps_what_is_read():
+    a = {k: _t(*s) for k, s in GOOD.items()}
+    buf = _t(6, 9, 3, 64)
+    lens = torch.zeros(2, dtype=torch.int32)
+    for kw, match in ((dict(query=buf[:, :4, :1], out=buf[:, 1:5, :1]), "query"), (dict(tail_keys=buf[:, :2], out=buf[:, 1:5, 2:]), "tail_keys"),
+                      (dict(tail_values=buf[:, 5:7], out=buf[:, 3:7, :1]), "tail_values"),
+                      (dict(prefix_keys=buf.view(2, -1, 9, 64)[:, :2], out=buf[:, :4, :1]), "prefix_keys"),
+                      (dict(prefix_lens=lens, out=lens.as_strided((1,), (1,)).view(torch.bfloat16)), "out must be"),
+                      (dict(out=buf[:, :4, :1].as_strided((6, 4, 1, 64), (64, 64, 64, 1))), "out must be")):
+        with pytest.raises(ValueError, match=match):
+            hira_shared_attention(**{**a, **kw})
+    for kw in (dict(out=a["query"]), dict(query=buf[:, :4, :1], out=buf[:, :4, 1:2]), dict(tail_keys=buf[:, :2], tail_values=buf[:, 2:4], out=buf[:, 4:8, 1:2])):
+        with pytest.raises(ValueError, match="CUDA"):
+            hira_shared_attention(**{**a, **kw})

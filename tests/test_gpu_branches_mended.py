@@ -93,3 +93,21 @@ def test_heads_of_one_projection_rotate_in_place_and_into_each_other(dtype):
             hira_qk_norm_rope(q, k, cos, sin, q_weight=qw, k_weight=kw, out_q=fused[:, 5:9], out_k=fused[:, 10:])
         with pytest.raises(ValueError, match="same memory"):
             hira_qk_norm_rope(q, k, cos, sin, q_weight=qw, k_weight=kw, out_q=fused[:, 6:10], out_k=fused[:, 8:10])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ctx,tail,group,branches", [(300, 7, 2, 3), (40, 9, 5, 20), (6000, 300, 1, 4), (0, 5, 4, 2), (33, 0, 4, 40)])
+def test_attention_over_its_own_query_and_between_others(dtype, ctx, tail, group, branches):
+    gen = torch.Generator().manual_seed(4)
+    h, d = 2, 64
+    kv = [torch.randn(s, generator=gen).to(dtype).cuda() for s in ((1, h, ctx, d), (1, h, ctx, d), (branches, h, tail, d), (branches, h, tail, d))]
+    for _ in range(3):
+        fused = torch.randn((branches, 2 * h * group + 3, 1, d), generator=gen).to(dtype).cuda()
+        q, other, old = fused[:, :h * group], fused[:, h * group:2 * h * group], fused.clone()
+        want = hira_shared_attention(q.clone(), *kv)
+        assert hira_shared_attention(q, *kv, out=other) is other
+        assert torch.equal(other, want) and torch.equal(q, old[:, :h * group]) and torch.equal(fused[:, 2 * h * group:], old[:, 2 * h * group:])
+        with pytest.raises(ValueError, match="query"):
+            hira_shared_attention(q, *kv, out=fused[:, 1:1 + h * group])
+        hira_shared_attention(q, *kv, out=q)
+        assert torch.equal(q, want) and torch.equal(other, want)
