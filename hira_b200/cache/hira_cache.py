@@ -155,11 +155,17 @@ class HiraCacheLayer(CacheLayerMixin):
         self.indexer.wait_pending_update()
         if self.indexer.state.values is None:
             raise ValueError("the index stores no values")
-        self.indexer.state.active_parents = self.indexer.active_parents
-        kv = S.export(self.indexer.state, self.indexed_len)
+        st = self.indexer.state
+        st.active_parents = self.indexer.active_parents
+        kv = S.export(st, self.indexed_len)
         kv = [t.view(self.B, self.H_kv, *t.shape[1:]) for t in kv]
         if self.queued_len:
             kv = [torch.cat([t, q], dim=2) for t, q in zip(kv, (self.queued_keys, self.queued_values))]
+        if st.device.type == "cuda":        # index and queue are dropped below, and perhaps another stream's
+            stream = torch.cuda.current_stream(st.device)
+            st.used_on(stream)
+            for t in (self._queue_k, self._queue_v):
+                t.record_stream(stream)
         self.shared = SharedPrompt(*kv, branches, max_tail=max_tail)
         self.indexed_len += self.queued_len
         self.indexer = self._queue_k = self._queue_v = None

@@ -111,3 +111,28 @@ def test_attention_over_its_own_query_and_between_others(dtype, ctx, tail, group
             hira_shared_attention(q, *kv, out=fused[:, 1:1 + h * group])
         hira_shared_attention(q, *kv, out=q)
         assert torch.equal(q, want) and torch.equal(other, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("queued", [0, 3])
+def test_a_prompt_shared_on_another_stream_is_whole_although_the_index_is_dropped(queued, dtype):
+    gen = torch.Generator().manual_seed(6)
+    k, v = (torch.randn((2, 2, 3000 + queued, 128), generator=gen).to(dtype).cuda() for _ in range(2))
+    layer = HiraCacheLayer("cuda_only", 8, dict(num_levels=3, max_iterations=1, branching_factor=16), {})
+    layer.update(k[:, :, :3000], v[:, :, :3000])
+    if queued:
+        layer.update(k[:, :, 3000:], v[:, :, 3000:])
+    slow = torch.randn((4096, 4096), device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(40):                          # keeps what follows on the side stream waiting
+            slow = torch.nn.functional.normalize(slow @ slow)
+        layer.share_prompt(3)
+    # takes freed memory of the first stream, if any is
+    junk = [torch.full(s, 7.0, dtype=d, device="cuda") for s, d in
+            [((4, 4096, 128), dtype)] * 6 + [((2, 2, 8, 128), dtype)] * 6 + [((4, 4096), torch.float32)] * 6]
+    torch.cuda.synchronize()
+    del junk
+    assert torch.equal(layer.shared.prefix_keys, k) and torch.equal(layer.shared.prefix_values, v)
+    assert layer.get_seq_length() == 3000 + queued
