@@ -251,9 +251,10 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                     }
                 }
                 if (!ok) *fail = 1;
-                // no copy may be in flight when the shared memory is given back: the products waited for each, unless one failed
-                if (*fail)
-                    for (uint32_t p = pos > STAGES ? pos - STAGES : 0; p < pos; ++p) mbar_wait(bar_full + 8 * (p % STAGES), (p / STAGES) & 1);
+                // No copy may be in flight when the shared memory is given back, and who waits for a tile may give up after the
+                // last one is asked for: the tiles that the ring still holds are waited for here, whatever became of the others.
+                // (Where all went well the products of the last one come after this, so it costs nothing.)
+                for (uint32_t p = pos > STAGES ? pos - STAGES : 0; p < pos; ++p) mbar_wait(bar_full + 8 * (p % STAGES), (p / STAGES) & 1);
             }
         } else if (warp == 9) {
             // ---- products ------------------------------------------------------------------------------------
