@@ -12,6 +12,7 @@ from typing import Optional
 
 import torch
 
+from .. import _lib as L
 from .. import index_state as S
 
 _TYPES = (torch.float32, torch.bfloat16)
@@ -247,6 +248,12 @@ class SharedPrompt:
                 raise ValueError(f"indices {host} do not keep {p} prompts apart, with equally many sequences each in their order")
         return idx
 
+    def _report(self, idx: torch.Tensor, status: torch.Tensor):
+        """What the gather would put into `status`, where there is no tail yet to gather."""
+        if idx.is_cuda:
+            bad = ((idx < 0) | (idx >= self.batch)).any()
+            status.bitwise_or_(bad.to(torch.int32) * L.HIRA_STATUS_BAD_INDEX)
+
     def reorder(self, indices):
         """In place: sequence b goes on from what sequence indices[b] was (any may be picked many times).  Sequences
         that pick themselves are not touched, and prompts never are.  An index on the device that is out of range
@@ -256,19 +263,26 @@ class SharedPrompt:
             raise ValueError(f"{idx.numel()} indices for {self.batch} sequences")
         if self._len:
             S.gather_rows(self._moves, idx, self._len, self.status)
+        else:
+            self._report(idx, self.status)
         return self
 
     def select(self, indices) -> "SharedPrompt":
-        """The picked sequences (forked where an index repeats, compacted where some are left out) over the same prompts."""
+        """The picked sequences (forked where an index repeats, compacted where some are left out) over the same prompts.
+        What `check_status` has to report of this one, it has to report of the new one too."""
         idx = self._picks(indices)
         n = idx.numel()
         if n == 0:
             raise ValueError("no sequence picked")
         new = SharedPrompt(self.prefix_keys, self.prefix_values, n // self.prefix_keys.shape[0], max_tail=self._k.shape[2])
         new.prefix_lens, new._len = self.prefix_lens, self._len
+        new.status.copy_(self.status)
+        _keep(self.status)
         if self._len:
             S.gather_rows(S.RowMoves([(self._k, new._k), (self._v, new._v)]), idx, self._len, new.status)
             _keep(self._k, self._v)
+        else:
+            self._report(idx, new.status)
         return new
 
     def check_status(self):

@@ -136,3 +136,39 @@ def test_a_prompt_shared_on_another_stream_is_whole_although_the_index_is_droppe
     del junk
     assert torch.equal(layer.shared.prefix_keys, k) and torch.equal(layer.shared.prefix_values, v)
     assert layer.get_seq_length() == 3000 + queued
+
+
+@pytest.mark.parametrize("tail", [0, 4])
+def test_a_bad_index_is_still_reported_after_forks_and_without_a_tail(tail):
+    k = torch.randn((1, 2, 9, 16), device="cuda")
+
+    def prompt():
+        p = SharedPrompt(k, k, 4)
+        return p.append(*[torch.randn((4, 2, tail, 16), device="cuda")] * 2) if tail else p
+    good, bad = torch.tensor([3, 2, 1, 0], device="cuda"), torch.tensor([0, 1, 2, 4], device="cuda")
+    p = prompt().reorder(good).select(good).select([1, 0, 1])
+    p.check_status()
+    for f in (lambda: prompt().reorder(bad), lambda: prompt().select(bad), lambda: prompt().reorder(bad).select([0, 1]),
+              lambda: prompt().reorder(bad).reorder(good).select(good).select([1]), lambda: prompt().select(bad[3:] - 9)):
+        with pytest.raises(RuntimeError, match="does not exist"):
+            f().check_status()
+    layer = HiraCacheLayer("cuda_only", 4, dict(num_levels=2, max_iterations=1, branching_factor=8), {})
+    layer.update(k.repeat(2, 1, 8, 1).bfloat16(), k.repeat(2, 1, 8, 1).bfloat16())
+    layer.share_prompt(1)
+    layer.batch_repeat_interleave(2)
+    layer.shared.check_status()
+
+
+def test_a_bad_index_of_a_captured_reordering_is_reported_without_a_tail():
+    k = torch.randn((1, 2, 9, 16), device="cuda")
+    p, idx = SharedPrompt(k, k, 4, max_tail=8), torch.arange(4, device="cuda")
+    p.reorder(idx)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p.reorder(idx)
+    g.replay()
+    p.check_status()
+    idx[2] = -1
+    g.replay()
+    with pytest.raises(RuntimeError, match="does not exist"):
+        p.check_status()
