@@ -286,6 +286,6 @@ class SharedPrompt:
         return new
 
     def check_status(self):
-        """Raises if an index on the device was out of range (reads one word from the device)."""
-        if int(self.status.item()):
-            raise RuntimeError("a sequence that does not exist was picked (status bit HIRA_STATUS_BAD_INDEX)")
+        """Raises if an index on the device was out of range, or if the index that the prompts come from had something to report
+        (reads one word from the device)."""
+        S.raise_for_status(int(self.status.item()))

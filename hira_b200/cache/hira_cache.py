@@ -166,7 +166,9 @@ class HiraCacheLayer(CacheLayerMixin):
             st.used_on(stream)
             for t in (self._queue_k, self._queue_v):
                 t.record_stream(stream)
-        self.shared = SharedPrompt(*kv, branches, max_tail=max_tail)
+        shared = SharedPrompt(*kv, branches, max_tail=max_tail)
+        shared.status.copy_(st.status)      # the index goes: what it has to report stays
+        self.shared = shared
         self.indexed_len += self.queued_len
         self.indexer = self._queue_k = self._queue_v = None
         self.queued_keys, self.queued_values, self.queued_len = self.shared.tail_keys, self.shared.tail_values, 0

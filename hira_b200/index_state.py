@@ -615,6 +615,17 @@ def assign(points: torch.Tensor, cents: torch.Tensor, use_tensor_cores: bool = F
     return idx, d2
 
 
+def raise_for_status(code: int):
+    """Raises for what the kernels have put into a status word."""
+    if code & L.HIRA_STATUS_BAD_INDEX:
+        raise RuntimeError("a sequence that does not exist was picked (status bit HIRA_STATUS_BAD_INDEX)")
+    if code & L.HIRA_STATUS_ASSIGN_FAILED:
+        raise RuntimeError("the tensor-core assignment of the build gave up on a bounded wait for some points "
+                           "(status bit HIRA_STATUS_ASSIGN_FAILED); rebuild with use_tensor_cores=False")
+    if code:
+        raise RuntimeError(f"index capacity exhausted during update (status {code}); raise max_context")
+
+
 # ---- several continuations of one prompt ----------------------------------------------------------------
 def row_strides(t: torch.Tensor) -> Optional[tuple]:
     """Element strides of a 4-d tensor's first three dimensions where its rows are contiguous and all start on

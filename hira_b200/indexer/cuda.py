@@ -412,14 +412,7 @@ class CUDAIndexer(BaseIndexer):
     def check_status(self):
         """Raises if an append ran out of pre-allocated slots (reads one word from the device)."""
         self.wait_pending_update() if self.state is not None else None
-        code = int(self.state.status.item())
-        if code & 8:
-            raise RuntimeError("a sequence that does not exist was picked (status bit HIRA_STATUS_BAD_INDEX)")
-        if code & 4:
-            raise RuntimeError("the tensor-core assignment of the build gave up on a bounded wait for some points "
-                               "(status bit HIRA_STATUS_ASSIGN_FAILED); rebuild with use_tensor_cores=False")
-        if code:
-            raise RuntimeError(f"index capacity exhausted during update (status {code}); raise max_context")
+        S.raise_for_status(int(self.state.status.item()))
 
     @torch.no_grad()
     def rebuild(self):

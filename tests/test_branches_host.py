@@ -284,3 +284,12 @@ def test_shared_attention_refuses_an_output_that_overlaps_what_is_read():
     for kw in (dict(out=a["query"]), dict(query=buf[:, :4, :1], out=buf[:, :4, 1:2]), dict(tail_keys=buf[:, :2], tail_values=buf[:, 2:4], out=buf[:, 4:8, 1:2])):
         with pytest.raises(ValueError, match="CUDA"):
             hira_shared_attention(**{**a, **kw})
+
+
+@pytest.mark.parametrize("code,match", [(8, "does not exist"), (4, "gave up"), (1, "capacity"), (2, "capacity"), (9, "does not exist")])
+def test_a_shared_prompt_reports_all_that_an_index_does(code, match):
+    p = SharedPrompt(_t(1, 1, 3, 8), _t(1, 1, 3, 8), 2)
+    p.check_status()
+    p.status.fill_(code)
+    with pytest.raises(RuntimeError, match=match):
+        p.check_status()

@@ -172,3 +172,18 @@ def test_a_bad_index_of_a_captured_reordering_is_reported_without_a_tail():
     g.replay()
     with pytest.raises(RuntimeError, match="does not exist"):
         p.check_status()
+
+
+def test_what_an_index_has_to_report_is_reported_by_its_shared_prompt():
+    k = torch.randn((2, 2, 40, 16), device="cuda").bfloat16()
+    for bad in (False, True):
+        layer = HiraCacheLayer("cuda_only", 4, dict(num_levels=2, max_iterations=1, branching_factor=8), {})
+        layer.update(k, k)
+        layer.reorder_cache(torch.tensor([0, 2 if bad else 1], device="cuda"))
+        layer.share_prompt(2)
+        layer.batch_select_indices([0, 2])
+        if bad:
+            with pytest.raises(RuntimeError, match="does not exist"):
+                layer.shared.check_status()
+        else:
+            layer.shared.check_status()
