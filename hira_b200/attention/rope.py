@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from .. import index_state as S
-from .shared_attention import refuse_grad
+from .shared_attention import differentiating, refuse_grad
 
 _TYPES = (torch.float32, torch.bfloat16)
 _plans = {}
@@ -65,7 +65,7 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     transposed view as it is); others are copied.  `out_q` / `out_k`: where to write, with such rows: the input itself,
     or memory apart from all that the call reads and from one another (part of a cache, say; the heads of one projection
     are apart although they lie between each other).  No backward pass."""
-    if torch.is_grad_enabled():
+    if differentiating():
         refuse_grad("hira_qk_norm_rope", query, key, q_weight, k_weight, cos, sin)
     eps, interleaved = float(eps), bool(interleaved)
     # calls of a layout that has been checked before go straight to the library

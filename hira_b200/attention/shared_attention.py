@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib as L
 from .. import index_state as S
@@ -32,10 +33,17 @@ def _tail_layout(t: Optional[torch.Tensor]):
     return b, h, d, min(n, 2), t.stride(), t.dtype, t.get_device()      # the strides of one row need not fit two
 
 
+def differentiating() -> bool:
+    """Whether a derivative of some kind may be asked for at all: one look for calls that need not look at their tensors."""
+    return torch.is_grad_enabled() or forward_ad._current_level >= 0
+
+
 def refuse_grad(what: str, *tensors):
-    """The kernels have no backward pass: a call that would have to be differentiated is refused."""
+    """The kernels have no backward pass and carry no tangents: a call that would have to be differentiated is refused."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no derivative in forward mode: call it on the primals")
 
 
 def _lengths(lens, n: int, most: int, device, what: str) -> Optional[torch.Tensor]:
@@ -78,7 +86,7 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     sums and statistics.  Rows have to be contiguous and 16-byte aligned: what is not is copied first.  `out` has
     to be so, and to be the query itself (D = V) or memory apart from all that the call reads.  No backward pass.  A key
     hidden from one query token but not from another has to be finite."""
-    if torch.is_grad_enabled():
+    if differentiating():
         refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
     if scaling is not None:
         scaling = float(scaling)      # a tensor's value, not the tensor, goes with the layout

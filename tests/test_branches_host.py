@@ -293,3 +293,22 @@ def test_a_shared_prompt_reports_all_that_an_index_does(code, match):
     p.status.fill_(code)
     with pytest.raises(RuntimeError, match=match):
         p.check_status()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_not_dropped_in_silence(grad):
+    import torch.autograd.forward_ad as fw
+    a = {k: _t(*s, dtype=torch.float32) for k, s in GOOD.items()}
+    q, k, c = _t(2, 4, 4, 64, dtype=torch.float32), _t(2, 2, 4, 64, dtype=torch.float32), _t(2, 4, 64, dtype=torch.float32)
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        for name, t in a.items():
+            with pytest.raises(ValueError, match="forward mode"):
+                hira_shared_attention(**{**a, name: fw.make_dual(t, torch.ones_like(t))})
+        for kw in (dict(query=q), dict(key=k), dict(cos=c), dict(sin=c), dict(q_weight=_t(64, dtype=torch.float32)), dict(k_weight=_t(64, dtype=torch.float32))):
+            for name, t in kw.items():
+                with pytest.raises(ValueError, match="forward mode"):
+                    hira_qk_norm_rope(**{**dict(query=q, key=k, cos=c, sin=c), name: fw.make_dual(t, torch.ones_like(t))})
+        with pytest.raises(ValueError, match="CUDA"):
+            hira_shared_attention(**a)
+        with pytest.raises(ValueError, match="CUDA"):
+            hira_qk_norm_rope(q, k, c, c)
