@@ -226,9 +226,10 @@ class SharedPrompt:
         self._k, self._v = new
         self._moves = S.RowMoves([(self._k, self._k), (self._v, self._v)])
 
-    @torch.no_grad()
     def append(self, keys: torch.Tensor, values: torch.Tensor):
         """keys (B, H_kv, m, D), values (B, H_kv, m, V): the next m tokens of every sequence."""
+        if differentiating():
+            refuse_grad("SharedPrompt.append", keys, values)
         for name, t, buf in (("keys", keys, self._k), ("values", values, self._v)):
             if t.ndim != 4 or t.shape[:2] != buf.shape[:2] or t.shape[3] != buf.shape[3] or t.shape[2] != keys.shape[2]:
                 raise ValueError(f"{name} {tuple(t.shape)} do not continue tails of {tuple(buf.shape)}")

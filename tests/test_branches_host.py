@@ -312,3 +312,17 @@ def test_tangents_are_not_dropped_in_silence(grad):
             hira_shared_attention(**a)
         with pytest.raises(ValueError, match="CUDA"):
             hira_qk_norm_rope(q, k, c, c)
+
+
+def test_a_shared_prompt_takes_no_keys_that_would_have_to_be_differentiated():
+    import torch.autograd.forward_ad as fw
+    p, new = SharedPrompt(_t(1, 1, 3, 8, dtype=torch.float32), _t(1, 1, 3, 8, dtype=torch.float32), 2), _t(2, 1, 1, 8, dtype=torch.float32)
+    for args in ((new.clone().requires_grad_(), new), (new, new.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="no backward"):
+            p.append(*args)
+        assert p.tail_len == 0
+        with torch.no_grad():
+            p.select([0, 1]).append(*args)
+    with fw.dual_level(), torch.no_grad(), pytest.raises(ValueError, match="forward mode"):
+        p.append(new, fw.make_dual(new, new))
+    assert p.append(new, new).tail_len == 1 and not p.tail_keys.requires_grad
