@@ -227,12 +227,15 @@ class SharedPrompt:
         self._moves = S.RowMoves([(self._k, self._k), (self._v, self._v)])
 
     def append(self, keys: torch.Tensor, values: torch.Tensor):
-        """keys (B, H_kv, m, D), values (B, H_kv, m, V): the next m tokens of every sequence."""
+        """keys (B, H_kv, m, D), values (B, H_kv, m, V): the next m tokens of every sequence, in the prompts' type and on
+        their device."""
         if differentiating():
             refuse_grad("SharedPrompt.append", keys, values)
         for name, t, buf in (("keys", keys, self._k), ("values", values, self._v)):
             if t.ndim != 4 or t.shape[:2] != buf.shape[:2] or t.shape[3] != buf.shape[3] or t.shape[2] != keys.shape[2]:
                 raise ValueError(f"{name} {tuple(t.shape)} do not continue tails of {tuple(buf.shape)}")
+            if t.dtype != buf.dtype or t.device != buf.device:
+                raise ValueError(f"{name} are {t.dtype} on {t.device}, the tails {buf.dtype} on {buf.device}")
         m = keys.shape[2]
         if self._len + m > self._k.shape[2]:
             self._reserve(max(self._len + m, 2 * self._k.shape[2], 16))

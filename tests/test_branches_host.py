@@ -326,3 +326,12 @@ def test_a_shared_prompt_takes_no_keys_that_would_have_to_be_differentiated():
     with fw.dual_level(), torch.no_grad(), pytest.raises(ValueError, match="forward mode"):
         p.append(new, fw.make_dual(new, new))
     assert p.append(new, new).tail_len == 1 and not p.tail_keys.requires_grad
+
+
+def test_a_shared_prompt_takes_keys_of_its_own_type_only():
+    p, new = SharedPrompt(_t(1, 1, 3, 8), _t(1, 1, 3, 8), 2), _t(2, 1, 1, 8)
+    for args in ((new.float(), new), (new, new.float()), (new.half(), new.half()), (new.to("meta"), new), (new, new.int())):
+        with pytest.raises(ValueError, match="the tails"):
+            p.append(*args)
+        assert p.tail_len == 0
+    assert p.append(new, new).tail_len == 1
