@@ -148,13 +148,8 @@ class HiraCacheLayer(CacheLayerMixin):
         instead of an index, and attended to as a whole (`hira_shared_attention`); what comes goes to a tail of each
         continuation.  `max_tail` reserves room for that many tokens each."""
         from ..attention.shared_attention import SharedPrompt
-        if not self.is_initialized:
-            raise ValueError("the layer holds no prompt yet")
-        if self.shared is not None:
-            raise ValueError("the layer's prompts are shared already: use batch_repeat_interleave")
+        self.check_share_prompt(branches)
         self.indexer.wait_pending_update()
-        if self.indexer.state.values is None:
-            raise ValueError("the index stores no values")
         st = self.indexer.state
         st.active_parents = self.indexer.active_parents
         kv = S.export(st, self.indexed_len)
@@ -173,6 +168,20 @@ class HiraCacheLayer(CacheLayerMixin):
         self.indexer = self._queue_k = self._queue_v = None
         self.queued_keys, self.queued_values, self.queued_len = self.shared.tail_keys, self.shared.tail_values, 0
         self.B = self.shared.batch
+
+    def check_share_prompt(self, branches: int):
+        """Raises where `share_prompt` would."""
+        if not self.is_initialized:
+            raise ValueError("the layer holds no prompt yet")
+        if self.shared is not None:
+            raise ValueError("the layer's prompts are shared already: use batch_repeat_interleave")
+        if branches < 1:
+            raise ValueError(f"{branches} branches of {self.B} prompts")
+        st = self.indexer.state
+        if st.values is None:
+            raise ValueError("the index stores no values")
+        if st.dtype != st.vdtype:
+            raise ValueError(f"keys are {st.dtype}, values {st.vdtype}: a shared prompt has them in one type")
 
     def reorder_cache(self, beam_idx):
         """In place: sequence b goes on from what sequence beam_idx[b] was."""
@@ -269,7 +278,9 @@ class HiraCache(Cache):
 
     def share_prompt(self, branches: int, max_tail: int = 0):
         """`HiraCacheLayer.share_prompt` for every layer: call it after the prompts' forward pass, and go on with
-        `branches` times as many sequences."""
+        `branches` times as many sequences.  Where one layer refuses, none is changed."""
+        for layer in self.layers:
+            layer.check_share_prompt(branches)
         for layer in self.layers:
             layer.share_prompt(branches, max_tail)
 

@@ -1,8 +1,10 @@
 """Several continuations of one prompt: calls that once went wrong, and the ones beside them."""
 import pytest
 import torch
+from transformers import LlamaConfig
 
-from hira_b200 import CUDAIndexer, HiraCacheLayer, SharedPrompt, hira_qk_norm_rope, hira_shared_attention, patch_attention
+from hira_b200 import (CUDAIndexer, HiraCache, HiraCacheLayer, HiraConfig, SharedPrompt, hira_qk_norm_rope, hira_shared_attention,
+                       patch_attention)
 from hira_b200 import _lib as L
 from hira_b200 import index_state as S
 from test_patched_layers_host import D, HIDDEN, _Layer, _neighbours
@@ -187,3 +189,26 @@ def test_what_an_index_has_to_report_is_reported_by_its_shared_prompt():
                 layer.shared.check_status()
         else:
             layer.shared.check_status()
+
+
+def test_a_cache_shares_the_prompts_of_all_its_layers_or_of_none():
+    cfg = LlamaConfig(vocab_size=8, hidden_size=32, num_hidden_layers=3, num_attention_heads=2, num_key_value_heads=2, head_dim=16)
+    cache = HiraCache(cfg, HiraConfig(device_mode="cuda_only", update_every=4, num_levels=2, branching_factor=8))
+    k = torch.randn((2, 2, 40, 16), device="cuda")
+
+    def unchanged(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            cache.share_prompt(**{**dict(branches=2), **kw})
+        assert all(layer.shared is None for layer in cache.layers)
+    cache.update(k, k, 0)
+    cache.update(k, k, 1)
+    unchanged("no prompt")
+    cache.update(k, k.bfloat16(), 2)
+    unchanged("one type")
+    cache.layers[2].reset()
+    cache.update(k, k, 2)
+    unchanged("branches", branches=0)
+    cache.share_prompt(2)
+    assert all(layer.shared.batch == 4 for layer in cache.layers)
+    with pytest.raises(ValueError, match="already"):
+        cache.share_prompt(2)
