@@ -48,9 +48,8 @@ def _samples_for(indexer, sample_size: int) -> torch.Tensor:
     rows = st.children.gather(1, slots.unsqueeze(-1).expand(-1, -1, st.dim)).contiguous()
     indexer._tau_samples = (st, rows)
     # all that are still in use follow their sequences when those are reordered
-    if cached is None or cached[0] is not st:
-        indexer._tau_drawn = []
-    indexer._tau_drawn.append(weakref.ref(rows))
+    drawn = [] if cached is None or cached[0] is not st else [ref for ref in indexer._tau_drawn if ref() is not None]
+    indexer._tau_drawn = drawn + [weakref.ref(rows)]
     return rows
 
 

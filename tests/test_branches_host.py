@@ -335,3 +335,16 @@ def test_a_shared_prompt_takes_keys_of_its_own_type_only():
             p.append(*args)
         assert p.tail_len == 0
     assert p.append(new, new).tail_len == 1
+
+
+def test_samples_that_nobody_holds_are_not_kept_track_of():
+    from types import SimpleNamespace
+
+    from hira_b200.attention.hira_attention import _samples_for
+    st = S.IndexState(n_heads=2, dim=8, vdim=8, bf=8, depth=2, cap_parents=16, dtype=torch.float32, vdtype=torch.float32, device="cpu")
+    st.slot2token[:] = torch.arange(128, dtype=torch.int32)
+    ix = SimpleNamespace(state=st)
+    held = _samples_for(ix, 16)
+    for s in [32, 64] * 20:
+        assert _samples_for(ix, s).shape == (2, s, 8)
+    assert len(ix._tau_drawn) <= 3 and any(ref() is held for ref in ix._tau_drawn)
