@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libhira_b200.so"
 HIRA_OK = 0
 HIRA_ERR_ARG, HIRA_ERR_SHAPE, HIRA_ERR_DTYPE, HIRA_ERR_CAPACITY, HIRA_ERR_CUDA = -1, -2, -3, -4, -5
 HIRA_F32, HIRA_BF16 = 0, 1
-HIRA_STATUS_PARENTS_FULL, HIRA_STATUS_GP_FULL, HIRA_STATUS_ASSIGN_FAILED, HIRA_STATUS_BAD_INDEX = 1, 2, 4, 8
+HIRA_STATUS_PARENTS_FULL, HIRA_STATUS_GP_FULL, HIRA_STATUS_ASSIGN_FAILED, HIRA_STATUS_BAD_INDEX, HIRA_STATUS_ATTN_FAILED = 1, 2, 4, 8, 16
 HIRA_GATE_GT, HIRA_GATE_GE = 0x0, 0x1
 HIRA_LEAF_CANDIDATES, HIRA_LEAF_GE, HIRA_LEAF_GT = 0x0, 0x2, 0x4
 HIRA_TAU_SAMPLE_MAX, HIRA_TAU_SAMPLE_MEAN_TOPK, HIRA_TAU_SAMPLE_KTH = 0, 1, 2
@@ -75,7 +75,7 @@ class HiraSharedAttnStruct(C.Structure):
                [(n, C.c_int64 * 3) for n in ("q_stride", "prefix_k_stride", "prefix_v_stride", "tail_k_stride", "tail_v_stride",
                                              "out_stride")] + \
                [(n, C.c_int32) for n in ("dtype", "n_prompts", "n_branches", "n_kv", "group", "n_q", "dim", "vdim", "prefix_len",
-                                         "tail_len")] + [("sm_scale", C.c_float)]
+                                         "tail_len")] + [("sm_scale", C.c_float), ("status", C.c_void_p)]
 
 
 class HiraGatherItemStruct(C.Structure):

@@ -70,7 +70,7 @@ def _check_apart(out, query, named):
 def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix_values: torch.Tensor,
                           tail_keys: Optional[torch.Tensor] = None, tail_values: Optional[torch.Tensor] = None, *,
                           prefix_lens=None, tail_lens=None, scaling: Optional[float] = None,
-                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                          out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """query (B, H_q, L_q, D), prefix (P, H_kv, L, D) and (P, H_kv, L, V), tails (B, H_kv, T, D) and (B, H_kv, T, V)
     -> (B, H_q, L_q, V) in the query's type.
 
@@ -85,11 +85,16 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     fp32 or bf16, all of one type; D and V multiples of 8 up to 256; B * H_kv up to 65,535.  fp32 is computed in fp32; bf16 with fp32
     sums and statistics.  Rows have to be contiguous and 16-byte aligned: what is not is copied first.  `out` has
     to be so, and to be the query itself (D = V) or memory apart from all that the call reads.  No backward pass.  A key
-    hidden from one query token but not from another has to be finite."""
+    hidden from one query token but not from another has to be finite.
+
+    `status`: a word (int32, on the query's device) that takes the bit HIRA_STATUS_ATTN_FAILED where a kernel gave up on a
+    bounded wait; the rows it had are NaN then."""
     if differentiating():
         refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
     if scaling is not None:
         scaling = float(scaling)      # a tensor's value, not the tensor, goes with the layout
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or status.device != query.device):
+        raise ValueError(f"status must be one int32 on {query.device}, got {tuple(status.shape)} {status.dtype} on {status.device}")
     # calls of a layout that has been checked before go straight to the library
     layout = None
     if (tail_keys is None or tail_values is not None and tail_keys.shape[:-1] == tail_values.shape[:-1]) \
@@ -101,10 +106,10 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
         plan = _plans.get(layout)
         if plan is not None:
             given = (query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
-            done = plan(*given, out)
+            done = plan(*given, out, status)
             if done is None and out is not None:      # address ranges that meet
                 _check_apart(out, query, zip(_NAMES, given))
-                done = plan(*given, out, apart=True)
+                done = plan(*given, out, status, apart=True)
             if done is not None:
                 return done
     if (tail_keys is None) != (tail_values is None):
@@ -155,7 +160,7 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     plan = S.SharedAttnPlan(*args[:5], d ** -0.5 if scaling is None else scaling, out)
     if layout is not None and all(a is b for a, b in zip(args, given)):
         S.remember(_plans, layout, plan)
-    return plan(*args, out, apart=True)
+    return plan(*args, out, status, apart=True)
 
 
 def _keep(*tensors):
@@ -248,7 +253,7 @@ class SharedPrompt:
         """query (B, H_q, m, D), the tokens appended last (or, before the first append, any): see `hira_shared_attention`."""
         k, v = (self.tail_keys, self.tail_values) if self._len else (None, None)
         return hira_shared_attention(query, self.prefix_keys, self.prefix_values, k, v, prefix_lens=self.prefix_lens,
-                                     scaling=scaling, out=out)
+                                     scaling=scaling, out=out, status=self.status)
 
     def _picks(self, indices) -> torch.Tensor:
         """A sequence continues its own prompt: with several prompts the indices are looked at on the host."""
@@ -298,6 +303,6 @@ class SharedPrompt:
         return new
 
     def check_status(self):
-        """Raises if an index on the device was out of range, or if the index that the prompts come from had something to report
-        (reads one word from the device)."""
+        """Raises if an index on the device was out of range, if a kernel of `attend` gave up on a bounded wait, or if the index
+        that the prompts come from had something to report (reads one word from the device)."""
         S.raise_for_status(int(self.status.item()))

@@ -578,6 +578,7 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
     HIRA_CHECK_ARG(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), HIRA_ERR_ARG, "hira_shared_attn: prefix_k / prefix_v is NULL");
     HIRA_CHECK_ARG(a->tail_len == 0 || (a->tail_k && a->tail_v), HIRA_ERR_ARG, "hira_shared_attn: tail_k / tail_v is NULL");
     const int es = (int)elem_size(a->dtype);
+    HIRA_CHECK_ARG(((uintptr_t)a->status & 3) == 0, HIRA_ERR_ARG, "hira_shared_attn: status is no 4-byte word");
     uintptr_t mis = (uintptr_t)a->q | (uintptr_t)a->out;
     const void* kv[4] = {a->prefix_k, a->prefix_v, a->tail_k, a->tail_v};
     const int64_t* st[6] = {a->prefix_k_stride, a->prefix_v_stride, a->tail_k_stride, a->tail_v_stride, a->q_stride, a->out_stride};
@@ -588,7 +589,7 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
     P = SharedAttn{};
     P.q = a->q; P.out = a->out;
     P.pk = a->prefix_k; P.pv = a->prefix_v; P.tk = a->tail_k; P.tv = a->tail_v;
-    P.prefix_lens = a->prefix_lens; P.tail_lens = a->tail_lens;
+    P.prefix_lens = a->prefix_lens; P.tail_lens = a->tail_lens; P.status = a->status;
     P.n_prompts = a->n_prompts; P.n_branches = a->n_branches; P.n_kv = a->n_kv; P.group = a->group; P.n_q = a->n_q;
     P.dim = a->dim; P.vdim = a->vdim; P.prefix_len = a->prefix_len; P.tail_len = a->tail_len;
     P.n_rows = (int)rows;

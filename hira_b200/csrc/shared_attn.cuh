@@ -32,6 +32,7 @@ struct SharedAttn {
     // The tensor-core kernel deals the key tiles of all (prompt, kv head) items out in `shares` equal runs, so an item's
     // number of partials follows from its position (0: every item has prefix_parts of them).
     int shares, item_tiles;
+    int32_t* status;              // or null: where a wait that ran out is reported
 };
 
 __device__ __forceinline__ int shared_prefix_len(const SharedAttn& P, int prompt) {

@@ -12,7 +12,8 @@
 // (weights up to 256 lose nothing in floating point), and O in TMEM is rescaled in rare tiles instead of each.
 //
 // The tiles of all items are dealt out in equal runs, one to each SM, whatever the items' number: a run may end
-// inside an item and go on in the next one.  Every wait is bounded; a block whose wait ran out leaves NaN.
+// inside an item and go on in the next one.  Every wait is bounded; a block whose wait ran out leaves NaN and says so in the
+// status word.
 //
 // Measured (8 heads of 128): 16 branches x 4 heads a key head at 32,768 keys 27 us (134 MB: 5.0 TB/s; 6.3 in the loop, the
 // rest is some 1.7 us before the first product and 1.6 behind the last); 64 branches at 131,072 keys 130 us (4.1 TB/s and
@@ -521,6 +522,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (tid == 0 && *fail && P.status) atomicOr(P.status, HIRA_STATUS_ATTN_FAILED);
     if (warp == 9) {
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

@@ -622,6 +622,8 @@ def raise_for_status(code: int):
     if code & L.HIRA_STATUS_ASSIGN_FAILED:
         raise RuntimeError("the tensor-core assignment of the build gave up on a bounded wait for some points "
                            "(status bit HIRA_STATUS_ASSIGN_FAILED); rebuild with use_tensor_cores=False")
+    if code & L.HIRA_STATUS_ATTN_FAILED:
+        raise RuntimeError("attention to a shared prompt gave up on a bounded wait and left NaN (status bit HIRA_STATUS_ATTN_FAILED)")
     if code:
         raise RuntimeError(f"index capacity exhausted during update (status {code}); raise max_context")
 
@@ -732,7 +734,7 @@ class SharedAttnPlan:
                 return False
         return True
 
-    def __call__(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out=None, apart: bool = False):
+    def __call__(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out=None, status=None, apart: bool = False):
         """None where a tensor does not start on a 16-byte boundary, or (unless it is known to be `apart`) the output's address
         range meets another tensor's."""
         lib = L.load()
@@ -754,6 +756,8 @@ class SharedAttnPlan:
             a.prefix_lens = prefix_lens.data_ptr()
         if tail_lens is not None:
             a.tail_lens = tail_lens.data_ptr()
+        if status is not None:
+            a.status = status.data_ptr()
         ref = C.byref(a)
         nbytes = lib.hira_shared_attn_workspace_bytes(ref)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device) if nbytes else None

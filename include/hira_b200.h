@@ -53,6 +53,7 @@ extern "C" {
                                        build placed them under centre 0, so the index is valid but
                                        of poor quality: rebuild with use_tensor_cores = 0 */
 #define HIRA_STATUS_BAD_INDEX 8    /* hira_gather, hira_gather_index: a picked sequence does not exist */
+#define HIRA_STATUS_ATTN_FAILED 16 /* hira_shared_attn: a block gave up on a bounded wait; the rows it had are NaN */
 
 /* search flags */
 #define HIRA_GATE_GT 0x0          /* keep node iff q.c + r >  tau (reference Triton kernels, kernels/triton_search_kernels.py:49,114,131) */
@@ -540,6 +541,7 @@ typedef struct hira_shared_attn {
     int64_t q_stride[3], prefix_k_stride[3], prefix_v_stride[3], tail_k_stride[3], tail_v_stride[3], out_stride[3];
     int32_t dtype, n_prompts, n_branches, n_kv, group, n_q, dim, vdim, prefix_len, tail_len;
     float sm_scale;
+    int32_t* status;            /* device word that HIRA_STATUS_ATTN_FAILED is put into, or NULL                */
 } hira_shared_attn_t;
 size_t hira_shared_attn_workspace_bytes(const hira_shared_attn_t* args);
 int hira_shared_attn(const hira_shared_attn_t* args, void* workspace, size_t workspace_bytes, void* stream);

@@ -348,3 +348,21 @@ def test_samples_that_nobody_holds_are_not_kept_track_of():
     for s in [32, 64] * 20:
         assert _samples_for(ix, s).shape == (2, s, 8)
     assert len(ix._tau_drawn) <= 3 and any(ref() is held for ref in ix._tau_drawn)
+
+
+def test_a_wait_that_ran_out_has_a_status_bit_of_its_own():
+    p = SharedPrompt(_t(1, 1, 3, 8), _t(1, 1, 3, 8), 2)
+    p.status.fill_(L.HIRA_STATUS_ATTN_FAILED)
+    for q in (p, p.select([0, 1, 1])):
+        with pytest.raises(RuntimeError, match="HIRA_STATUS_ATTN_FAILED"):
+            q.check_status()
+    a = {k: _t(*s) for k, s in GOOD.items()}
+    for status in (torch.zeros(1), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="status"):
+            hira_shared_attention(**a, status=status)
+    with pytest.raises(ValueError, match="CUDA"):
+        hira_shared_attention(**a, status=torch.zeros(1, dtype=torch.int32))
+    lib, args = L.load(), _args(status=4097)
+    assert lib.hira_shared_attn_workspace_bytes(C.byref(args)) == 0 and lib.hira_shared_attn(C.byref(args), None, 0, None) == L.HIRA_ERR_ARG
+    args.status = 4096
+    assert lib.hira_shared_attn(C.byref(args), None, 0, None) == L.HIRA_ERR_CAPACITY

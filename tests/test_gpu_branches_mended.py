@@ -212,3 +212,15 @@ def test_a_cache_shares_the_prompts_of_all_its_layers_or_of_none():
     assert all(layer.shared.batch == 4 for layer in cache.layers)
     with pytest.raises(ValueError, match="already"):
         cache.share_prompt(2)
+
+
+def test_attention_leaves_what_its_status_holds():
+    gen = torch.Generator().manual_seed(7)
+    k, v, q = (torch.randn(s, generator=gen).bfloat16().cuda() for s in ((1, 2, 40000, 128), (1, 2, 40000, 128), (9, 8, 1, 128)))
+    for word in (0, 2):
+        status = torch.full((1,), word, dtype=torch.int32, device="cuda")
+        out = hira_shared_attention(q, k, v, status=status)
+        assert torch.isfinite(out).all() and int(status) == word and torch.equal(out, hira_shared_attention(q, k, v))
+    prompt = SharedPrompt(k, v, 9)
+    prompt.attend(q)
+    prompt.check_status()
