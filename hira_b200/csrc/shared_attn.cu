@@ -405,7 +405,6 @@ shared_few_kernel(const SharedAttn P) {
 // ---------------------------------------------------------------------------
 constexpr int SA_MERGE_WARPS = 4;
 constexpr int SA_FLIGHT = 8;      // parts of a row on their way at once, for each warp
-constexpr int SA_MAX_PARTS = 512;
 
 template <typename T, int W>
 __global__ void __launch_bounds__(32 * SA_MERGE_WARPS)

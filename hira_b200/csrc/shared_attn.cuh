@@ -69,6 +69,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+constexpr int SA_MAX_PARTS = 512;      // of an output row, prefix and tail together: what the join's kernel has room for
+
 bool shared_tc_supported(const SharedAttn& P);
 void shared_tc_plan(SharedAttn& P);
 int shared_tc_launch(const SharedAttn& P, cudaStream_t s);

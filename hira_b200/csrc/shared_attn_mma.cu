@@ -354,7 +354,10 @@ bool shared_mma_prefers(const SharedAttn& P) {
     const long long row_blocks = ((long long)P.n_branches * P.group * P.n_q + TL_ROWS - 1) / TL_ROWS;
     return row_blocks * P.n_prompts * P.n_kv * P.prefix_len <= 1280ll * SM_COUNT;
 }
-// Splits of the keys: two blocks an SM (one of 256 channels), none with less than two steps of its own.
+// Splits of the keys: two blocks an SM (one of 256 channels), none with less than two steps of its own, and beyond 32 none with less
+// than sixteen: each split is a part that the join reads.  One key head, 8 rows, at most 32 splits against this and tcgen05
+// tiles: 128 channels, 65,536 keys 28.7 / 22.6 / 30.7 us, 131,072 keys 45.1 / 28.7 / 38.9; 256 channels, 131,072 keys 75.8 / 47.1.
+// With eight steps instead of sixteen 131,072 keys take 32.8 (two heads 45.2, with sixteen 42.9).
 int shared_mma_splits(const SharedAttn& P, bool tail) {
     const int len = tail ? P.tail_len : P.prefix_len, rows = P.group * P.n_q * (tail ? 1 : P.n_branches);
     if (len <= 0) return 0;
@@ -362,7 +365,8 @@ int shared_mma_splits(const SharedAttn& P, bool tail) {
     const int steps = (len + TL_STEP - 1) / TL_STEP;
     long long s = (tl_width(P) == 256 ? 1 : 2) * SM_COUNT / blocks;
     if (s > steps / 2) s = steps / 2;
-    if (s > 32) s = 32;
+    if (s > 32 && s > steps / 16) s = steps / 16 > 32 ? steps / 16 : 32;
+    if (s > SA_MAX_PARTS / 2) s = SA_MAX_PARTS / 2;
     return s < 1 ? 1 : (int)s;
 }
 

@@ -366,3 +366,23 @@ def test_a_wait_that_ran_out_has_a_status_bit_of_its_own():
     assert lib.hira_shared_attn_workspace_bytes(C.byref(args)) == 0 and lib.hira_shared_attn(C.byref(args), None, 0, None) == L.HIRA_ERR_ARG
     args.status = 4096
     assert lib.hira_shared_attn(C.byref(args), None, 0, None) == L.HIRA_ERR_CAPACITY
+
+
+def _parts(**kw):
+    """Parts of an output row, from the size of the workspace (a tail that joins the parts itself has none)."""
+    a = _args(**{**dict(group=1, tail_len=0), **kw})
+    rows = a.n_prompts * a.n_branches * a.n_kv * a.group * a.n_q
+    n, rest = divmod(L.load().hira_shared_attn_workspace_bytes(C.byref(a)), 4 * (a.vdim + 2) * rows)
+    assert rest == 0
+    return n
+
+
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 8, 16])
+@pytest.mark.parametrize("n_kv", [1, 2, 3, 8])
+def test_long_prompts_of_few_heads_keep_the_device_busy(n_kv, rows, width):
+    for n in (1, 64, 200, 3000, 32768, 65536, 131072, 1 << 20):
+        parts = _parts(n_kv=n_kv, n_branches=rows, dim=width, vdim=width, prefix_len=n)
+        # all 148 SMs have a block, or the blocks are short (2,048 keys)
+        assert 1 <= parts <= 256 and (n_kv * (parts + 1) > 148 or n / parts <= 2048)
+        assert _parts(n_kv=n_kv, n_branches=rows, dim=width, vdim=width, prefix_len=n, tail_len=n) <= 512
