@@ -224,3 +224,57 @@ def test_attention_leaves_what_its_status_holds():
     prompt = SharedPrompt(k, v, 9)
     prompt.attend(q)
     prompt.check_status()
+
+
+def _counted(p, n, h, g, lq, d, v, ctx, tail, dtype, plens=None, tlens=None):
+    """Every key counts: with queries of 0 all weights are 1, so an output is a number of keys over a number of keys.  Each channel
+    has 1 at 64 keys in turn, so that one key too few or too many moves it by 1/64, four times the rounding of bf16; as many
+    calls as it takes to have every key in some channel."""
+    b = p * n
+    gen = torch.Generator().manual_seed(8)
+    q = torch.zeros((b, h * g, lq, d), dtype=dtype, device="cuda")
+    pk, tk = (torch.randn(s, generator=gen).to(dtype).cuda() for s in ((p, h, ctx, d), (b, h, tail, d)))
+    pl = torch.full((p,), ctx, device="cuda") if plens is None else torch.tensor(plens, device="cuda")
+    tl = torch.full((b,), tail, device="cuda") if tlens is None else torch.tensor(tlens, device="cuda")
+    owner = torch.arange(b, device="cuda") // n
+    seen_t = (tl[:, None] - (lq - 1 - torch.arange(lq, device="cuda"))[None]).clamp(min=0)        # (b, lq)
+    total = (pl[owner][:, None] + seen_t).double()
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    chan = torch.arange(v, device="cuda")
+    for turn in range(-(-max(ctx, tail) // (64 * v))):
+        first = (chan + turn * v) * 64                                  # channel c has 1 at keys first[c] .. first[c] + 63
+
+        def values(rows):
+            at = torch.arange(rows, device="cuda")
+            return ((at[:, None] >= first[None]) & (at[:, None] < first[None] + 64)).to(dtype)
+
+        def among(length):                                              # of the first `length` keys
+            return (length[..., None] - first).clamp(0, 64)
+        pv, tv = values(ctx).expand(p, h, ctx, v).contiguous(), values(tail).expand(b, h, tail, v).contiguous()
+        want = (among(pl[owner])[:, None] + among(seen_t)).double() / total[..., None].clamp(min=1)
+        got = hira_shared_attention(q, pk, pv, tk, tv, prefix_lens=None if plens is None else pl, tail_lens=None if tlens is None else tl)
+        # the quotient as a reciprocal and a product in 32 bits (2^-23), then the rounding
+        off = (got.double() - want[:, None]).abs() - want[:, None] * (half + 2.0 ** -22)
+        assert (off <= 0).all(), f"turn {turn}: off by {off.max().item():.3g} more than a rounding"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [
+    # p, n, h, g, lq, d, v, ctx, tail
+    (1, 8, 1, 1, 1, 128, 128, 131072, 0),         # one key head: many splits
+    (1, 3, 2, 4, 1, 128, 128, 65536, 700),
+    (1, 16, 2, 4, 1, 64, 64, 40000, 130),
+    (1, 16, 8, 4, 1, 128, 128, 20000, 64),        # 64 rows a key head, tiles dealt out in runs
+    (2, 33, 3, 4, 1, 128, 128, 9001, 130),        # 132 rows
+    (3, 5, 4, 3, 3, 64, 64, 9001, 37),
+    (1, 70, 1, 8, 1, 64, 64, 20001, 2),           # 560 rows
+    (1, 4, 1, 2, 1, 256, 256, 70000, 33),
+    (2, 20, 2, 4, 1, 256, 256, 3001, 129),
+    (1, 5, 1, 3, 2, 136, 64, 20000, 260),
+    (1, 2, 1, 1, 1, 128, 128, 0, 70000),          # a long tail alone
+    (1, 2, 1, 2, 1, 128, 128, 70001, 70001),      # both long
+], ids=lambda s: "x".join(map(str, s)))
+def test_every_key_counts(shape, dtype):
+    _counted(*shape, dtype)
+    p, n, _, _, _, _, _, ctx, tail = shape
+    _counted(*shape, dtype, plens=[ctx - 77 * i if i else max(0, ctx - 1) for i in range(p)], tlens=[max(0, tail - 3 * i) for i in range(p * n)])
