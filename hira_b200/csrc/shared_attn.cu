@@ -216,7 +216,7 @@ shared_simt_kernel(const SharedAttn P) {
 // key's products with ALL rows (half of the channels each; the key is read once, the queries are broadcasts), a warp
 // then takes whole rows for their softmax, and for the weighted sums a warp takes 16 of the 64 keys and a lane four
 // channels of all rows.  The four warps' sums are added up once, at the end.
-// 8 rows of 8 heads at 32,768 keys of 128 (268 MB): 82..86 us (3.2 TB/s), 16 rows 160 (the kernel above: 209 both).  Bound by the
+// 8 rows of 8 heads at 32,768 keys of 128 (268 MB): 82..86 us (3.2 TB/s), 16 rows 121 (the kernel above: 209 both).  Bound by the
 // rows' broadcasts: each costs a warp four cycles of shared memory's port, as a row of its own would.
 // ---------------------------------------------------------------------------
 template <int ROWS, int NV, bool TAIL>
@@ -502,12 +502,16 @@ static auto simt_kernel() {      // NV: 64 channels each of 16 lanes, or (few ro
     if constexpr (RPT <= 2) return shared_few_kernel<8 * RPT, NV / 2, TAIL>;
     else return shared_simt_kernel<RPT, NV, TAIL>;
 }
+static size_t simt_smem(int block_rows, int dim, int vdim) {
+    return sizeof(float) * ((size_t)(block_rows + SA_KEYS) * (dim + SA_PAD) + (size_t)SA_KEYS * (vdim + SA_PAD) +
+                            (size_t)SA_KEYS * (block_rows + SA_PAD));
+}
+
 template <int RPT, int NV, bool TAIL>
 static int launch_simt(const SharedAttn& P, bool chained, cudaStream_t s) {
     auto kern = simt_kernel<RPT, NV, TAIL>();
     const int per = P.group * P.n_q, rows = TAIL ? per : P.n_branches * per;
-    const size_t smem = sizeof(float) * ((size_t)(8 * RPT + SA_KEYS) * (P.dim + SA_PAD) + (size_t)SA_KEYS * (P.vdim + SA_PAD) +
-                                         (size_t)SA_KEYS * (8 * RPT + SA_PAD));
+    const size_t smem = simt_smem(8 * RPT, P.dim, P.vdim);
     static SmemLimit limit;
     cudaError_t e = limit.raise(kern, (int)smem);
     if (e != cudaSuccess) {
@@ -546,15 +550,22 @@ static int launch_simt_rows(const SharedAttn& P, bool chained, cudaStream_t s) {
     return launch_simt<8, 2, TAIL>(P, chained, s);
 }
 
-// Splits of the keys: as many blocks as are resident at once (three an SM of those with few rows, else two), none with
-// fewer than two tiles.
-static int simt_splits(int rows, int items, int len, int vdim) {
+// Splits of the keys: as many blocks as are resident at once -- what an SM's shared memory holds, but no more than three of those
+// with few rows and two of the others --, none with fewer than two tiles.  128 channels (three an SM of 8 rows, two of 16 and 32, one
+// of 64), us with one / two / three an SM: 8 heads, 32,768 keys, 8 rows 123 / 88 / 82, 16 rows 162 / 121 / 158, 32 rows 311 / 203 /
+// 272; 9,000 keys, 64 rows 131 / 141 / 162; one head, 32,768 keys, 16 rows 37 / 39 / 35.  256 channels (one), 8 heads, 9,000 keys,
+// 8 rows 61 / 68 / 80.
+constexpr int SA_SM_SMEM = 228 * 1024, SA_BLOCK_RESERVE = 1024;      // bytes an SM has, and keeps for itself of each block's
+static int simt_splits(int rows, int items, int len, int dim, int vdim) {
     if (len <= 0) return 0;
     const int block_rows = simt_rows(rows, vdim), tiles = (len + SA_KEYS - 1) / SA_KEYS;
     const long long blocks = (long long)((rows + block_rows - 1) / block_rows) * items;
-    long long splits = (block_rows <= 16 ? 3 : 2) * SM_COUNT / blocks;
+    long long resident = SA_SM_SMEM / (long long)(simt_smem(block_rows, dim, vdim) + SA_BLOCK_RESERVE);
+    if (resident > (block_rows <= 16 ? 3 : 2)) resident = block_rows <= 16 ? 3 : 2;
+    if (resident < 1) resident = 1;
+    long long splits = resident * SM_COUNT / blocks;
     if (splits > (tiles + 1) / 2) splits = (tiles + 1) / 2;
-    if (splits > 64) splits = 64;
+    if (splits > SA_MAX_PARTS / 2) splits = SA_MAX_PARTS / 2;
     return splits < 1 ? 1 : (int)splits;
 }
 
@@ -604,8 +615,8 @@ static int shared_plan(const hira_shared_attn_t* a, SharedAttn& P) {
         else P.prefix_parts = shared_mma_splits(P, false);
         P.fused = shared_tail_joins(P);
     } else {
-        P.tail_parts = simt_splits(per, branches, a->tail_len, a->vdim);
-        P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->vdim);
+        P.tail_parts = simt_splits(per, branches, a->tail_len, a->dim, a->vdim);
+        P.prefix_parts = simt_splits(a->n_branches * per, a->n_prompts * a->n_kv, a->prefix_len, a->dim, a->vdim);
     }
     return HIRA_OK;
 }

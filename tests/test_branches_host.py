@@ -386,3 +386,16 @@ def test_long_prompts_of_few_heads_keep_the_device_busy(n_kv, rows, width):
         # all 148 SMs have a block, or the blocks are short (2,048 keys)
         assert 1 <= parts <= 256 and (n_kv * (parts + 1) > 148 or n / parts <= 2048)
         assert _parts(n_kv=n_kv, n_branches=rows, dim=width, vdim=width, prefix_len=n, tail_len=n) <= 512
+
+
+@pytest.mark.parametrize("n_kv,rows,width,resident", [
+    # blocks of 8, 16, 32 and 64 rows take 73, 79, 92 and 116 KiB at 128 channels, 145 and more at 256: what 228 hold, at most three
+    (8, 8, 128, 3), (8, 16, 128, 2), (8, 32, 128, 2), (8, 64, 128, 1), (1, 8, 128, 3), (1, 16, 128, 2), (3, 64, 128, 1), (8, 8, 256, 1),
+    (1, 16, 256, 1), (8, 64, 256, 1), (8, 8, 64, 3), (8, 64, 64, 2),
+])
+def test_splits_in_fp32_are_the_blocks_that_are_resident_at_once(n_kv, rows, width, resident):
+    block = 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 or width > 128 else 64
+    blocks = -(-rows // block) * n_kv
+    for n in (64, 1000, 32768, 100000):
+        parts = _parts(dtype=L.HIRA_F32, n_kv=n_kv, n_branches=rows, dim=width, vdim=width, prefix_len=n)
+        assert parts == max(1, min(resident * 148 // blocks, (-(-n // 64) + 1) // 2, 256))
