@@ -3,8 +3,8 @@ import pytest
 import torch
 from transformers import LlamaConfig
 
-from hira_b200 import (CUDAIndexer, HiraCache, HiraCacheLayer, HiraConfig, SharedPrompt, hira_qk_norm_rope, hira_shared_attention,
-                       patch_attention)
+from hira_b200 import (CacheOutput, CUDAIndexer, HiraCache, HiraCacheLayer, HiraConfig, SharedPrompt, hira_attention, hira_qk_norm_rope,
+                       hira_shared_attention, patch_attention)
 from hira_b200 import _lib as L
 from hira_b200 import index_state as S
 from test_patched_layers_host import D, HIDDEN, _Layer, _neighbours
@@ -278,3 +278,69 @@ def test_every_key_counts(shape, dtype):
     _counted(*shape, dtype)
     p, n, _, _, _, _, _, ctx, tail = shape
     _counted(*shape, dtype, plens=[ctx - 77 * i if i else max(0, ctx - 1) for i in range(p)], tlens=[max(0, tail - 3 * i) for i in range(p * n)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("share", [True, False])
+def test_a_captured_step_of_a_cache_reorders_appends_and_attends(share, dtype):
+    """A step of a search over continuations, captured once over a cache of two layers and replayed with other picks and tokens, does
+    what the same calls do one by one (the tail's length is the host's: each replay writes the same row)."""
+    cfg = LlamaConfig(vocab_size=8, hidden_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64)
+    gen = torch.Generator().manual_seed(9)
+
+    def rnd(*shape):
+        return torch.randn(shape, generator=gen).to(dtype).cuda()
+    prompts = [(rnd(1, 2, 230, 64), rnd(1, 2, 230, 64)) for _ in range(2)]
+    queued = [(rnd(1, 2, 3, 64), rnd(1, 2, 3, 64)) for _ in range(2)]           # not yet indexed
+    tokens = [(rnd(6, 2, 5, 64), rnd(6, 2, 5, 64)) for _ in range(2)]
+
+    def cache():
+        c = HiraCache(cfg, HiraConfig(device_mode="cuda_only", update_every=64, num_levels=2, branching_factor=8, max_context=400,
+                                      threshold_method="none"))
+        for i in range(2):
+            c.update(*prompts[i], i)
+            c.update(*queued[i], i)
+        c.share_prompt(6, max_tail=16) if share else c.batch_repeat_interleave(6)
+        for i in range(2):
+            c.update(*tokens[i], i)
+        return c
+
+    def step(c, picks, q, new):
+        c.reorder_cache(picks)
+        outs = []
+        for i in range(2):
+            out, _ = c.update(*new[i], i)
+            outs.append(hira_attention(None, q, out, None, None, scaling=0.2, hira_config=c.hira_config)[0])
+        return outs
+
+    def other_values():
+        return torch.randint(6, (6,), generator=gen).cuda(), rnd(6, 4, 1, 64), [(rnd(6, 2, 1, 64), rnd(6, 2, 1, 64)) for _ in range(2)]
+    c = cache()
+    picks, q, new = other_values()
+    if not share:                  # the search's workspaces come into being
+        for i in range(2):
+            out = c.layers[i]
+            hira_attention(None, q, CacheOutput(out.queued_keys, out.queued_values, None, None, out.indexer, out.searcher), None, None,
+                           scaling=0.2, hira_config=c.hira_config)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(c, picks, q, new)
+    state = cache()                # goes the same way without a graph
+    for _ in range(4):
+        values = other_values()
+        for static, now in zip([picks, q, *new[0], *new[1]], [values[0], values[1], *values[2][0], *values[2][1]]):
+            static.copy_(now)
+        g.replay()
+        want = step(state, *values)
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+        for a, b in zip(c.layers, state.layers):
+            assert torch.equal(a.queued_keys, b.queued_keys) and torch.equal(a.queued_values, b.queued_values)
+        for layer in state.layers:             # back to the length that the graph was captured with
+            if share:
+                layer.shared._len -= 1
+            else:
+                layer.queued_len -= 1
+    for layer in c.layers:
+        (layer.shared if share else layer.indexer).check_status()
