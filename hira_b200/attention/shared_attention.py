@@ -89,7 +89,7 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
 
     `status`: a word (int32, on the query's device) that takes the bit HIRA_STATUS_ATTN_FAILED where a kernel gave up on a
     bounded wait; the rows it had are NaN then."""
-    if differentiating():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         refuse_grad("hira_shared_attention", query, prefix_keys, prefix_values, tail_keys, tail_values)
     if scaling is not None:
         scaling = float(scaling)      # a tensor's value, not the tensor, goes with the layout
@@ -105,9 +105,9 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
                   _tail_layout(tail_keys), _tail_layout(tail_values), _layout(prefix_lens), _layout(tail_lens), _layout(out), scaling)
         plan = _plans.get(layout)
         if plan is not None:
-            given = (query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
-            done = plan(*given, out, status)
+            done = plan(query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens, out, status)
             if done is None and out is not None:      # address ranges that meet
+                given = (query, prefix_keys, prefix_values, tail_keys, tail_values, prefix_lens, tail_lens)
                 _check_apart(out, query, zip(_NAMES, given))
                 done = plan(*given, out, status, apart=True)
             if done is not None:
@@ -165,9 +165,10 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
 
 def _keep(*tensors):
     """For tensors that may be dropped while the current stream still reads them, another stream's among them."""
-    for t in tensors:
-        if t.is_cuda:
-            t.record_stream(torch.cuda.current_stream(t.device))
+    if tensors[0].is_cuda:
+        stream = torch.cuda.current_stream(tensors[0].device)
+        for t in tensors:
+            t.record_stream(stream)
 
 
 class SharedPrompt:
@@ -182,7 +183,7 @@ class SharedPrompt:
     that was captured with them lives."""
 
     def __init__(self, prefix_keys: torch.Tensor, prefix_values: torch.Tensor, branches: int, *, prefix_lens=None,
-                 max_tail: int = 0):
+                 max_tail: int = 0, _status: Optional[torch.Tensor] = None):
         for name, t in (("prefix_keys", prefix_keys), ("prefix_values", prefix_values)):
             if t.ndim != 4:
                 raise ValueError(f"{name} must have 4 dimensions, got {tuple(t.shape)}")
@@ -196,7 +197,7 @@ class SharedPrompt:
         self.prefix_keys, self.prefix_values = S.with_rows(prefix_keys), S.with_rows(prefix_values)
         self.prefix_lens = _lengths(prefix_lens, prefix_keys.shape[0], prefix_keys.shape[2], prefix_keys.device, "prefix_lens")
         self.branches = int(branches)
-        self.status = torch.zeros((1,), dtype=torch.int32, device=prefix_keys.device)
+        self.status = torch.zeros((1,), dtype=torch.int32, device=prefix_keys.device) if _status is None else _status
         self._len = 0
         self._k = self._v = None
         self._reserve(max(0, int(max_tail)))
@@ -291,15 +292,14 @@ class SharedPrompt:
         n = idx.numel()
         if n == 0:
             raise ValueError("no sequence picked")
-        new = SharedPrompt(self.prefix_keys, self.prefix_values, n // self.prefix_keys.shape[0], max_tail=self._k.shape[2])
+        new = SharedPrompt(self.prefix_keys, self.prefix_values, n // self.prefix_keys.shape[0], max_tail=self._k.shape[2],
+                           _status=self.status.clone())
         new.prefix_lens, new._len = self.prefix_lens, self._len
-        new.status.copy_(self.status)
-        _keep(self.status)
         if self._len:
             S.gather_rows(S.RowMoves([(self._k, new._k), (self._v, new._v)]), idx, self._len, new.status)
-            _keep(self._k, self._v)
         else:
             self._report(idx, new.status)
+        _keep(self.status, self._k, self._v)
         return new
 
     def check_status(self):

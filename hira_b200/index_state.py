@@ -719,43 +719,48 @@ class SharedAttnPlan:
         a.dtype, a.n_prompts, a.n_branches, a.n_kv, a.group = L.dtype_code(q.dtype), p, b // p, h, hq // h
         a.n_q, a.dim, a.vdim, a.sm_scale = n_q, d, vdim, float(sm_scale)
         self.out_shape, self.device, self.index = (b, hq, n_q, vdim), q.device, q.get_device()
-        self.spans = [spanned_bytes(t) for t in (q, prefix_k, prefix_v, out)]
         self.in_place = d == vdim and row_strides(q) == row_strides(out)
-
-    def _apart(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out) -> bool:
-        """Whether the address range of `out` meets no other tensor's, the query's apart where that is all the same."""
-        nq, nk, nv, no = self.spans
-        at = out.data_ptr()
-        end, pq, pk, pv = at + no, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr()
-        if pk < end and at < pk + nk or pv < end and at < pv + nv or pq < end and at < pq + nq and not (at == pq and self.in_place):
-            return False
-        for t in (tail_k, tail_v, prefix_lens, tail_lens):
-            if t is not None and t.data_ptr() < end and at < t.data_ptr() + spanned_bytes(t):
-                return False
-        return True
+        self.q_bytes, self.k_bytes, self.v_bytes, self.out_bytes = (spanned_bytes(t) for t in (q, prefix_k, prefix_v, out))
+        # of the tails: from a row to the next, and all of them with one row
+        e = q.element_size()
+        self.tail_bytes = [(t.stride(2) * e, spanned_bytes(t[:, :, :1]) if t.shape[2] else 0) for t in (tail_k, tail_v) if t is not None]
+        self.lens_bytes = 4 * p, 4 * b
 
     def __call__(self, q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out=None, status=None, apart: bool = False):
         """None where a tensor does not start on a 16-byte boundary, or (unless it is known to be `apart`) the output's address
-        range meets another tensor's."""
+        range may meet another tensor's, the query's apart where that is all the same."""
         lib = L.load()
+        alone = apart or out is None
         if out is None:
             out = q.new_empty(self.out_shape)
-        elif not apart and not self._apart(q, prefix_k, prefix_v, tail_k, tail_v, prefix_lens, tail_lens, out):
-            return None
         a = L.HiraSharedAttnStruct.from_buffer_copy(self.args)      # one of its own for every call
         pq, pk, pv, po = q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), out.data_ptr()
+        if not alone:
+            end = po + self.out_bytes
+            if pk < end and po < pk + self.k_bytes or pv < end and po < pv + self.v_bytes or \
+                    pq < end and po < pq + self.q_bytes and not (po == pq and self.in_place):
+                return None
         every = pq | pk | pv | po
         a.q, a.prefix_k, a.prefix_v, a.out = pq, pk, pv, po
         if tail_k is not None:
             tk, tv = tail_k.data_ptr(), tail_v.data_ptr()
             every |= tk | tv
-            a.tail_k, a.tail_v, a.tail_len = tk, tv, tail_k.shape[2]
+            n = tail_k.shape[2]
+            a.tail_k, a.tail_v, a.tail_len = tk, tv, n
+            if not alone:
+                (step_k, rest_k), (step_v, rest_v) = self.tail_bytes
+                if tk < end and po < tk + (n - 1) * step_k + rest_k or tv < end and po < tv + (n - 1) * step_v + rest_v:
+                    return None
         if every & 15:
             return None
         if prefix_lens is not None:
-            a.prefix_lens = prefix_lens.data_ptr()
+            at = a.prefix_lens = prefix_lens.data_ptr()
+            if not alone and at < end and po < at + self.lens_bytes[0]:
+                return None
         if tail_lens is not None:
-            a.tail_lens = tail_lens.data_ptr()
+            at = a.tail_lens = tail_lens.data_ptr()
+            if not alone and at < end and po < at + self.lens_bytes[1]:
+                return None
         if status is not None:
             a.status = status.data_ptr()
         ref = C.byref(a)
@@ -852,36 +857,33 @@ class RopePlan:
         self.weight_bytes = d * q.element_size()
         self.in_place = row_strides(q) == row_strides(out_q), row_strides(k) == row_strides(out_k)
 
-    def _apart(self, q, k, cos, sin, q_weight, k_weight, out_q, out_k) -> bool:
-        """Whether the address ranges of the given outputs meet no other tensor's, their own input's apart where that is all the same."""
-        nq, nk, noq, nok, ncos, nsin = self.spans
-        reads = [(t.data_ptr(), n) for t, n in ((cos, ncos), (sin, nsin), (q_weight, self.weight_bytes), (k_weight, self.weight_bytes))
-                 if t is not None]
-        pq, pk = q.data_ptr(), k.data_ptr()
-        if out_q is not None:
-            at, end = out_q.data_ptr(), out_q.data_ptr() + noq
-            own = [] if at == pq and self.in_place[0] else [(pq, nq)]
-            if any(p < end and at < p + n for p, n in (*own, (pk, nk), *reads)):
-                return False
-        if out_k is not None:
-            at, end = out_k.data_ptr(), out_k.data_ptr() + nok
-            own = [] if at == pk and self.in_place[1] else [(pk, nk)]
-            other = [] if out_q is None else [(out_q.data_ptr(), noq)]
-            if any(p < end and at < p + n for p, n in (*own, (pq, nq), *other, *reads)):
-                return False
-        return True
-
     def __call__(self, q, k, cos, sin, q_weight, k_weight, out_q=None, out_k=None, apart: bool = False):
-        """None where a tensor does not start on a 16-byte boundary, or (unless they are known to be `apart`) an output's address
-        range meets another tensor's."""
-        if not apart and (out_q is not None or out_k is not None) and not self._apart(q, k, cos, sin, q_weight, k_weight, out_q, out_k):
-            return None
+        """None where a tensor does not start on a 16-byte boundary, or (unless they are known to be `apart`) a given output's
+        address range meets another tensor's, its own input's apart where that is all the same."""
+        given_q, given_k = not apart and out_q is not None, not apart and out_k is not None
         if out_q is None:
             out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
         if out_k is None:
             out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
         a = L.HiraRopeStruct.from_buffer_copy(self.args)            # one of its own for every call
         pq, pk, oq, ok = q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr()
+        if given_q or given_k:
+            nq, nk, noq, nok, ncos, nsin = self.spans
+            reads = [(cos.data_ptr(), ncos), (sin.data_ptr(), nsin)]
+            for w in (q_weight, k_weight):
+                if w is not None:
+                    reads.append((w.data_ptr(), self.weight_bytes))
+            for at, end, there in ((oq, oq + noq, given_q), (ok, ok + nok, given_k)):
+                if there:
+                    for p, n in reads:
+                        if p < end and at < p + n:
+                            return None
+            if given_q and (pk < oq + noq and oq < pk + nk or pq < oq + noq and oq < pq + nq and not (oq == pq and self.in_place[0])):
+                return None
+            if given_k and (pq < ok + nok and ok < pq + nq or pk < ok + nok and ok < pk + nk and not (ok == pk and self.in_place[1])):
+                return None
+            if given_q and given_k and ok < oq + noq and oq < ok + nok:
+                return None
         every = pq | pk | oq | ok
         a.q, a.k, a.q_out, a.k_out, a.cos, a.sin = pq, pk, oq, ok, cos.data_ptr(), sin.data_ptr()
         if q_weight is not None:
