@@ -82,9 +82,9 @@ def hira_shared_attention(query: torch.Tensor, prefix_keys: torch.Tensor, prefix
     whatever it holds).  On the host they are checked; on the device they are cut to 0..L and 0..T.  A query that
     sees no key at all gives 0.
 
-    fp32 or bf16, all of one type; D and V multiples of 8 up to 256; B * H_kv up to 65,535.  fp32 is computed in fp32; bf16 with fp32
-    sums and statistics.  Rows have to be contiguous and 16-byte aligned: what is not is copied first.  `out` has
-    to be so, and to be the query itself (D = V) or memory apart from all that the call reads.  No backward pass.  A key
+    fp32 or bf16, all of one type; D and V multiples of 8 up to 256; B * H_kv up to 65,535.  fp32 is computed in fp32; bf16 with
+    fp32 sums and statistics and softmax weights of two bf16 terms (2^-15 of a weight).  Rows have to be contiguous and 16-byte
+    aligned: what is not is copied first.  `out` has to be so, and to be the query itself (D = V) or memory apart from all that the call reads.  No backward pass.  A key
     hidden from one query token but not from another has to be finite.
 
     `status`: a word (int32, on the query's device) that takes the bit HIRA_STATUS_ATTN_FAILED where a kernel gave up on a

@@ -9,7 +9,8 @@
 //
 // Measured behind a prefix of 131,072 keys: 64 branches x 8 heads x 256 keys (134 MB) and the join of 19 parts in 20 us
 // (6.7 TB/s of the tails alone); 16 branches x 64 keys 6 us, a chain of latencies.  As the prefix's kernel: rows of 256 channels,
-// 4 branches of 8 heads at 16,384 keys (134 MB), 8 rows a head 37 us with 16 rows 39 (CUDA cores: 213 and 250).
+// 8 heads at 16,384 keys (134 MB), 8 rows a head 33 us, 16 rows 34 (CUDA cores: 213 and 250), 64 rows 83, 256 rows 309: the keys are
+// read again for every 16 rows.  The weights' second bf16 term (2^-16 of a weight between the two) costs 1 us of 33, 12 of 83.
 #include "shared_attn.cuh"
 #include "tc_common.cuh"
 #include <math_constants.h>
@@ -276,6 +277,10 @@ shared_mma_kernel(const SharedAttn P) {
                     }
             }
             const uint32_t p[4] = {tl_pack(s[0][0], s[0][1]), tl_pack(s[0][2], s[0][3]), tl_pack(s[1][0], s[1][1]), tl_pack(s[1][2], s[1][3])};
+            uint32_t lo[4];      // what the rounding left: the weights' second terms
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                lo[x] = tl_pack(s[x >> 1][2 * (x & 1)] - __uint_as_float(p[x] << 16), s[x >> 1][2 * (x & 1) + 1] - __uint_as_float(p[x] & 0xffff0000u));
 #pragma unroll
             for (int n = 0; n < HD / 16; ++n) {
                 uint32_t vv[4];
@@ -283,6 +288,8 @@ shared_mma_kernel(const SharedAttn P) {
                 tl_ldm4t(vv, sv + r * Lay::ROW + ((c ^ (r & 7)) << 4));
                 tl_mma(o[2 * n], p, vv[0], vv[1]);
                 tl_mma(o[2 * n + 1], p, vv[2], vv[3]);
+                tl_mma(o[2 * n], lo, vv[0], vv[1]);
+                tl_mma(o[2 * n + 1], lo, vv[2], vv[3]);
             }
         }
         __syncwarp();            // the stage is read before it is filled again

@@ -3,7 +3,7 @@
 // A block takes the query rows of one (prompt, kv head) -- 128, or 256 where there are more -- through a run of key
 // tiles of 128.  One warp streams the tiles in by TMA, one thread issues the products
 //   S = Q K^T  (tcgen05.mma, operands in shared memory, fp32 accumulator in TMEM)
-//   O += P V   (P = 2^(S - m) as bf16 in TMEM, where S was; V in shared memory as it lies in memory)
+//   O += P V   (P = 2^(S - m) as two bf16 terms in TMEM, where S was; V in shared memory as it lies in memory)
 // and two groups of four warps turn S into P, each thread one row: no exchange between threads for maximum and sum.
 // The two groups are two independent chains, so that one group's exponentials run under the other's products:
 //   256 rows: a group has 128 rows of its own, both see every tile;
@@ -15,9 +15,12 @@
 // inside an item and go on in the next one.  Every wait is bounded; a block whose wait ran out leaves NaN and says so in the
 // status word.
 //
-// Measured (8 heads of 128): 16 branches x 4 heads a key head at 32,768 keys 27 us (134 MB: 5.0 TB/s; 6.3 in the loop, the
-// rest is some 1.7 us before the first product and 1.6 behind the last); 64 branches at 131,072 keys 130 us (4.1 TB/s and
-// 1.05 PFLOP/s: exponentials of two groups, products and the hand-overs between them, none of which is busy all the time).
+// P takes two bf16 terms, 2^-15 of a weight between them: one alone is off by 2^-8, and the outputs' error against 64 bits
+// was 0.0023 with it where rounding them costs 0.0017 (now 0.0017).  The second term is a third product on the same V.
+//
+// Measured, launch after launch (8 heads of 128): 16 branches x 4 heads a key head at 32,768 keys 30.7 us (134 MB: 4.4 TB/s; some
+// 1.7 us before the first product and 1.6 behind the last), with one term 29.0; 64 branches at 131,072 keys 157 us (3.4 TB/s and
+// 1.31 PFLOP/s, the rate that matrix products keep up under the power limit), with one term 123 (1.11 PFLOP/s of two products).
 #include "shared_attn.cuh"
 #include "tc_common.cuh"
 
@@ -285,6 +288,13 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                         if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
                     }
                 };
+                // 16 keys' part of P V: the weights' first terms, then their second ones
+                auto pv = [&](int w, int k, uint32_t b0, bool accumulate) {
+                    const uint32_t p = tm_s + w * ST_KEYS + k * 8;
+                    const uint64_t v = st_desc_v<HD>(b0 + k * 2048);
+                    st_mma_ts(tm_o + w * HD, p, v, st_idesc(HD, true), accumulate);
+                    st_mma_ts(tm_o + w * HD, p + ST_KEYS / 2, v, st_idesc(HD, true), 1);
+                };
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
                     if (ok && count[w] > 0) {
@@ -308,8 +318,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         if (leader) {
 #pragma unroll
-                            for (int k = 0; k < ST_KEYS / 32; ++k)
-                                st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
+                            for (int k = 0; k < ST_KEYS / 32; ++k) pv(w, k, b0, i > 0 || k > 0);
                         }
                         ok = st_wait(bar_p + 8 * w, n_p[w] & 1);
                         if (!ok) continue;
@@ -317,8 +326,7 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         if (leader) {
 #pragma unroll
-                            for (int k = ST_KEYS / 32; k < ST_KEYS / 16; ++k)
-                                st_mma_ts(tm_o + w * HD, tm_s + w * ST_KEYS + k * 8, st_desc_v<HD>(b0 + k * 2048), st_idesc(HD, true), (i > 0 || k > 0));
+                            for (int k = ST_KEYS / 32; k < ST_KEYS / 16; ++k) pv(w, k, b0, i > 0 || k > 0);
                             if (NT == 1 || w == 1) umma_commit(bar_empty + 8 * stage);
                             if (!more) umma_commit(bar_o + 8 * w);
                         }
@@ -436,15 +444,21 @@ shared_tc_kernel(const SharedAttn P, const __grid_constant__ CUtensorMap map_k, 
                         float2 sum2 = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            uint32_t p[16];
+                            uint32_t hi[16], lo[16];
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 const float2 y = __ffma2_rn(make_float2(__uint_as_float(s[q][2 * e]), __uint_as_float(s[q][2 * e + 1])), sc2, nm2);
                                 const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                                 sum2 = __fadd2_rn(sum2, z);
-                                p[e] = pack_bf16(z.x, z.y);
+                                // the upper 16 bits of each are its first term, what that leaves (exact in fp32) rounded its second
+                                const uint32_t a = __float_as_uint(z.x), b = __float_as_uint(z.y);
+                                hi[e] = __byte_perm(a, b, 0x7632);
+                                const float2 rest = __ffma2_rn(make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)),
+                                                               make_float2(-1.f, -1.f), z);
+                                lo[e] = pack_bf16(rest.x, rest.y);
                             }
-                            st_st16(my_s + q * 16, p);
+                            st_st16(my_s + q * 16, hi);
+                            st_st16(my_s + ST_KEYS / 2 + q * 16, lo);
                             if (q == 1) {
                                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -524,7 +524,7 @@ int hira_assign(const void* points, const void* cents, int32_t dtype,
  *                                                           ++ tail[b][hq / group][0 .. tail_len - (n_q - 1 - t)).
  * The last n_q keys of a tail are those of the query tokens, so token t does not see the ones behind it.  A row that
  * sees no key is 0.  Softmax and sums in fp32, the output rounded once to `dtype`; with bf16 the softmax weights enter
- * the tensor cores as bf16, each off by at most 2^-8 of itself, as the output's own rounding.
+ * the tensor cores as the sum of two bf16 terms, each weight off by at most 2^-15 of itself.
  * What lies behind a length is never used, whatever it holds.
  * All rows start on 16-byte boundaries with their elements one behind another; strides are in elements: (prompt or
  * branch, head, row or token).  Any of them may be 0 or negative (not of the output).

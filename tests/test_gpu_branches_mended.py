@@ -344,3 +344,42 @@ def test_a_captured_step_of_a_cache_reorders_appends_and_attends(share, dtype):
                 layer.queued_len -= 1
     for layer in c.layers:
         (layer.shared if share else layer.indexer).check_status()
+
+
+@pytest.mark.parametrize("shape", [
+    # p, n, h, g, d, v, ctx, tail
+    (1, 2, 2, 4, 128, 128, 300, 9),               # few rows: 16 rows a block
+    (1, 16, 8, 4, 128, 128, 4000, 64),            # 64 rows a key head: two chains over the same rows
+    (1, 40, 8, 4, 128, 128, 4000, 70),            # 160 rows: a chain for each 128
+    (2, 20, 8, 4, 64, 64, 5000, 3),
+    (2, 40, 8, 4, 64, 64, 5000, 3),
+    (1, 4, 2, 2, 256, 256, 900, 70),
+    (1, 3, 1, 2, 128, 128, 0, 700),               # tails alone
+], ids=lambda s: "x".join(map(str, s)))
+def test_softmax_weights_are_not_rounded_to_bf16(shape):
+    """Logits of one product each, exact in 32 bits, so that what is left is the weights' precision: 2^-15 of each in two terms."""
+    p, n, h, g, d, v, ctx, tail = shape
+    gen = torch.Generator().manual_seed(10)
+
+    def rnd(*s):
+        return torch.randn(s, generator=gen).bfloat16().cuda()
+    b = p * n
+    q = torch.zeros((b, h * g, 1, d), dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = rnd(b, h * g, 1)
+    pk, tk = (torch.zeros(s, dtype=torch.bfloat16, device="cuda") for s in ((p, h, ctx, d), (b, h, tail, d)))
+    pk[..., 0], tk[..., 0] = rnd(p, h, ctx), rnd(b, h, tail)
+    pv, tv = rnd(p, h, ctx, v), rnd(b, h, tail, v)
+    scaling = 0.75
+    got = hira_shared_attention(q, pk, pv, tk, tv, scaling=scaling)
+    for s in range(b):
+        for hh in range(h):
+            k, w = (torch.cat([x[s // n, hh], y[s, hh]]).double() for x, y in ((pk, tk), (pv, tv)))
+            x = q[s, hh * g:(hh + 1) * g, 0].double()
+            z = scaling * (x @ k.T)
+            probs = torch.softmax(z, dim=-1)
+            want, mean = probs @ w, probs @ w.abs()
+            # a logit: times the scale and log2(e), less the maximum (2^-24 each of up to 2 x 1.45 |z|), the exponential (2^-22); both in
+            # numerator and denominator.  Sums over the keys in 32 bits, cut where the tensor cores add.  The weights.  The output's rounding
+            off = 2 * (3 * 2.0 ** -24 * 2 * 1.45 * z.abs().amax(-1, keepdim=True) + 2.0 ** -22) + 2.0 ** -23 * (64 + len(k) / 8) + 2.0 ** -15
+            diff = (got[s, hh * g:(hh + 1) * g, 0].double() - want).abs() - (off * mean + 2.0 ** -8 * want.abs())
+            assert (diff <= 0).all(), f"off by {diff.max().item():.3g} more than the bound"
