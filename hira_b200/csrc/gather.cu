@@ -11,7 +11,9 @@
 //
 // Bound by memory.  One sequence of an index of 8 heads, 32,768 keys of 128 bf16 in room for 40,000, forked into 8 (1.9 GB with
 // the int8 copy and the cleared room): 322 us, 5.9 TB/s.  In place, two of 8 sequences of 16,384 keys replaced (340 MB): 64 us,
-// 5.3 TB/s, nothing staged (staged 108 when this was 71).  Tails of 100 tokens, 4 of 8 changed: 10 us, the launch and two round trips.
+// 5.3 TB/s, nothing staged.  Staged, which any changed sequence that another picks asks for: two of the 8 swapped 99 us, permuted (6
+// changed) 276, all 8 rotated 381, 3.4 to 3.7 TB/s: a strip's loads, a barrier, its stores and another barrier, with only the SM's
+// other blocks in flight meanwhile.  Tails of 100 tokens, 4 of 8 replaced: 7 us, the launch and two round trips; rotated 28.
 #include "common.cuh"
 
 namespace hira {

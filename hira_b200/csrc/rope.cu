@@ -12,7 +12,10 @@
 // 8,191 tokens x 40 heads of 128 bf16 with norm (168 MB): 35 us (4.8 TB/s) with 64 rotated channels, 41 with 128; a plain
 // copy of as many bytes takes 32.  What is left is issue slots: two channels an instruction, partners by shuffles instead
 // of the row read again and no division took it from 45 to 35; twice the heads a group, or its next four loaded while
-// four are worked on, leave fewer warps and took 43 to 57.  One token of 40 heads: 6 us, the launch and one round trip.
+// four are worked on, leave fewer warps and took 43 to 57.  One token of 40 heads: 6 us, the launch and one round trip.  Other
+// forms of the same 8,191 tokens: 32 channels 35, interleaved 35 to 42 whatever is rotated; 48 channels 46 and 96 channels 55, whose
+// partners are looked for among all of the group's chunks; 24 channels 77 (half of
+// them no multiple of 8: one head a group, partners read again one by one).  fp32 57 to 68, 66 and 86, 82.
 #include "common.cuh"
 
 namespace hira {
