@@ -262,6 +262,8 @@ def _counted(p, n, h, g, lq, d, v, ctx, tail, dtype, plens=None, tlens=None):
 @pytest.mark.parametrize("shape", [
     # p, n, h, g, lq, d, v, ctx, tail
     (1, 8, 1, 1, 1, 128, 128, 131072, 0),         # one key head: many splits
+    (1, 8, 1, 1, 1, 128, 128, 131072, 1),         # joined by the tails' blocks
+    (1, 4, 1, 2, 1, 64, 64, 400000, 3),
     (1, 3, 2, 4, 1, 128, 128, 65536, 700),
     (1, 16, 2, 4, 1, 64, 64, 40000, 130),
     (1, 16, 8, 4, 1, 128, 128, 20000, 64),        # 64 rows a key head, tiles dealt out in runs
