@@ -56,10 +56,10 @@ def hira_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
     """query (B, H_q, L, D), key (B, H_kv, L, D) -> the two normalised and rotated, in their type.
 
     `cos`, `sin` (B or 1, L, R) or (L, R), R <= D even: tables with the factors of each of the first R channels at that
-    channel's own place; channels i and i + R/2 form a pair, or 2i and 2i + 1 when `interleaved`.  (Some models that pair 2i and 2i + 1 hand
-    out tables with the pair's value at i and i + R/2: those have to be laid out by channel first, as `hira_attention_forward`
-    does with `table_halves`.)  The channels behind R are not rotated.  `q_weight` / `k_weight` (D,): RMS norm of that side's heads with this weight; None:
-    no norm.  Computed in fp32 and rounded once.
+    channel's own place; channels i and i + R/2 form a pair, or 2i and 2i + 1 when `interleaved`.  (Some models that pair
+    2i and 2i + 1 hand out tables with the pair's value at i and i + R/2: those have to be laid out by channel first, as
+    `hira_attention_forward` does with `table_halves`.)  The channels behind R are not rotated.  `q_weight` / `k_weight`
+    (D,): RMS norm of that side's heads with this weight; None: no norm.  Computed in fp32 and rounded once.
 
     fp32 or bf16; D a multiple of 8 up to 256.  Any strides with contiguous, 16-byte aligned rows (a projection's
     transposed view as it is); others are copied.  `out_q` / `out_k`: where to write, with such rows: the input itself,

@@ -179,8 +179,9 @@ class SharedPrompt:
         out = prompt.attend(query)                            # (P * 16, H_q, m, D) -> (P * 16, H_q, m, V)
         prompt.reorder(indices)                               # sequence b goes on from what indices[b] was
 
-    Prompts are not copied, unless their rows are not contiguous or not 16-byte aligned.  Tails grow by doubling; `max_tail` reserves room for that many tokens, so that nothing moves while a graph
-    that was captured with them lives."""
+    Prompts are not copied, unless their rows are not contiguous or not 16-byte aligned.  Tails grow by doubling;
+    `max_tail` reserves room for that many tokens, so that nothing moves while a graph that was captured with them
+    lives."""
 
     def __init__(self, prefix_keys: torch.Tensor, prefix_values: torch.Tensor, branches: int, *, prefix_lens=None,
                  max_tail: int = 0, _status: Optional[torch.Tensor] = None):
