@@ -527,7 +527,8 @@ int hira_assign(const void* points, const void* cents, int32_t dtype,
  * the tensor cores as the sum of two bf16 terms, each weight off by at most 2^-15 of itself.
  * What lies behind a length is never used, whatever it holds.
  * All rows start on 16-byte boundaries with their elements one behind another; strides are in elements: (prompt or
- * branch, head, row or token).  Any of them may be 0 or negative (not of the output).
+ * branch, head, row or token).  Any of them may be 0 or negative (not of the output).  The output is q itself (dim ==
+ * vdim, the same strides) or memory apart from all that is read.
  * `workspace` belongs to the call until it is done; hira_shared_attn_workspace_bytes gives its size (16-byte aligned). */
 typedef struct hira_shared_attn {
     const void* q;              /* [n_prompts * n_branches][n_kv * group][n_q][dim]   */
@@ -579,7 +580,8 @@ int hira_gather_index(const hira_index_t* from, const hira_index_t* to, int32_t 
  *   y_i = x^_i cos_i - x^_p sin_i,  y_p = x^_p cos_p + x^_i sin_p
  * for the channel pairs (i, p) = (i, i + rotary/2), or (2i, 2i + 1) when interleaved, below `rotary`; the channels
  * behind pass through.  fp32, rounded once.  Tables [batch][n_tokens][rotary], strides in elements (0: one for all
- * sequences).  Strides of the heads' rows: (sequence, head, token). */
+ * sequences).  Strides of the heads' rows: (sequence, head, token).  An output is its own input or memory apart from all
+ * that is read and from the other output. */
 typedef struct hira_rope {
     const void* q;         /* [batch][q_heads][n_tokens][dim]  */
     const void* k;         /* [batch][k_heads][n_tokens][dim]  */
